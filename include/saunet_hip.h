@@ -27,7 +27,8 @@ extern "C" {
 
 enum saunet_status { SAUNET_OK = 0, SAUNET_BAD_SHAPE = -1, SAUNET_BAD_DTYPE = -2, SAUNET_LAUNCH_FAILED = -3,
                      SAUNET_BAD_ALIGN = -4, SAUNET_UNSUPPORTED = -5 };
-enum saunet_dtype { SAUNET_F32 = 0, SAUNET_BF16 = 1 };
+enum saunet_dtype { SAUNET_F32 = 0, SAUNET_BF16 = 1,
+                    SAUNET_F16 = 2 /* matrices of saunet_newton_schulz and the int8 products only */ };
 /* weight packings produced by saunet_pack_weight (K = reduction index, contiguous) */
 enum saunet_pack_mode {
     SAUNET_PACK_FWD = 0,       /* Conv2d [Co,Ci,kh,kw]        -> [Co][kh][kw][Ci]                         */
@@ -508,6 +509,49 @@ int saunet_radam_step(const saunet_tensor_list* tl /*0:param 1:grad 2:exp_avg 3:
 int saunet_adam_step(const saunet_tensor_list* tl /*0:param 1:grad 2:exp_avg 3:exp_avg_sq*/, const float* hyper, void* stream);
 /* flat[offset_i : offset_i+n_i] = grad_i (pack=1) or grad_i = flat[...]*scale (pack=0): all-reduce buckets */
 int saunet_bucket_copy(const saunet_tensor_list* tl /*0:tensor 1:flat+offset*/, int pack, float scale, void* stream);
+
+/* Newton-Schulz orthogonalisation of a list of matrices (any shapes, one dtype) in one chain of launches:
+ *   X = G / max(|G|_F, eps), then `steps` times  X <- (a I + b S + c S^2) X,  S = X X^T  (rows <= cols; the transpose otherwise).
+ * Intermediate matrices are float16 pairs (float32-class products); float32 accumulation, float64 norm.  A matrix that holds an Inf or NaN comes
+ * out as NaN and leaves the others alone; a zero matrix stays zero.  SAUNET_UNSUPPORTED, nothing launched: coefficients under which the
+ * iteration leaves the range that the pairs can hold.  src may equal dst.
+ * workspace: saunet_newton_schulz_workspace(d) bytes on a 256-byte border, private to the call until it has completed on `stream`. */
+typedef struct saunet_ns_item {
+    const void* src; void* dst;    /* matrix and result, row-major; Muon: gradient and parameter */
+    float* buf;                    /* Muon: momentum buffer, contiguous */
+    int64_t ld_src, ld_dst;        /* elements between rows */
+    int32_t rows, cols;            /* 1 .. 2^20, the shorter side up to 32768 */
+} saunet_ns_item;
+typedef struct saunet_ns_desc {
+    const saunet_ns_item* item;    /* HOST array of `count` entries, read before the call returns */
+    int32_t count;                 /* 1 .. 4096 */
+    int32_t dtype;                 /* SAUNET_F32 / _BF16 / _F16 of src and dst */
+    int32_t steps;                 /* 1 .. 32 */
+    int32_t adjust;                /* Muon: learning rate times sqrt(max(1, rows / cols)) (0) or 0.2 sqrt(max(rows, cols)) (1) */
+    float a, b, c, eps;
+} saunet_ns_desc;
+int64_t saunet_newton_schulz_workspace(const saunet_ns_desc* d);      /* < 0: saunet_status */
+int saunet_newton_schulz(const saunet_ns_desc* d, void* workspace, int64_t workspace_bytes, void* stream);
+/* One Muon step (float32): buf <- momentum buf + (1 - momentum) g;  u = nesterov ? (1 - momentum) g + momentum buf : buf;
+ * p <- (1 - lr weight_decay) p - lr adjust NewtonSchulz(u).   hyper (DEVICE) = {lr, momentum, weight_decay, nesterov(0/1), grad_scale} */
+int saunet_muon_step(const saunet_ns_desc* d, const float* hyper, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* int8 rows: k elements and zeros up to the row stride's next multiple of 64, 16-byte aligned, one float32 scale a row.
+ * quantize_rows: v = x (scale[c], shift[c] given: x scale[c] + shift[c]; relu: max(v, 0));  s = fl32(max |v| / 127),  q = round-half-even of the
+ * exact v / s.  A row with an Inf or NaN gets s = NaN, q = 0; a row whose s would be subnormal s = 0, q = 0.  ldq: a multiple of 64, padding is
+ * written with zeros.  dtype SAUNET_F32 / _BF16 / _F16, any alignment and row stride of x. */
+int saunet_quantize_rows(int dtype, const void* x, int64_t ldx, int64_t rows, int k, const float* scale, const float* shift, int relu,
+                         void* q, int64_t ldq, float* s, void* stream);
+/* y[m][n] = (sum_k a[m][k] b[n][k]) a_scale[m] b_scale[n] (+ bias[n]) (relu: max(., 0)), the sum exact in int32 */
+typedef struct saunet_int8_desc {
+    const void* a; const float* a_scale; int64_t lda, m;      /* tokens (pixels); strides in bytes, multiples of 16 that cover k rounded up to 64 */
+    const void* b; const float* b_scale; int64_t ldb;         /* n weight rows (channels) */
+    int32_t n, k;                                             /* k <= 131071 */
+    const float* bias;                                        /* or NULL */
+    void* y; int64_t ldy;                                     /* m rows of n, row stride in elements */
+    int32_t dtype, relu;                                      /* of y: SAUNET_F32 / _BF16 / _F16 */
+} saunet_int8_desc;
+int saunet_matmul_int8(const saunet_int8_desc* d, void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,8 +14,9 @@ CSRC = os.path.join(HERE, "csrc")
 ROOT = os.path.dirname(HERE)
 OBJ = os.path.join(HERE, "_obj")
 LIB = os.path.join(HERE, "libsaunet_hip.so")
-SOURCES = ["conv.hip", "conv_igemm.hip", "conv_tile.hip", "conv_mm.hip", "dense_dgrad.hip", "dense_fwd.hip", "norm.hip", "pointwise.hip", "pool.hip", "gate.hip", "expand.hip", "loss.hip", "canny.hip", "augment.hip", "optim.hip"]
+SOURCES = ["conv.hip", "conv_igemm.hip", "conv_tile.hip", "conv_mm.hip", "dense_dgrad.hip", "dense_fwd.hip", "norm.hip", "pointwise.hip", "pool.hip", "gate.hip", "expand.hip", "loss.hip", "canny.hip", "augment.hip", "optim.hip", "muon.hip", "int8.hip"]
 HEADERS = [os.path.abspath(__file__), os.path.join(CSRC, "common.h"), os.path.join(CSRC, "mma_tiles.h"), os.path.join(ROOT, "include", "saunet_hip.h")]
+OWN_HEADERS = {"muon.hip": ["nt_tiles.h"], "int8.hip": ["nt_tiles.h"]}       # headers that only these sources include
 # packed float32 instructions are kept out of the code: some of their forms give wrong results on this hardware now and then (the host pass does
 # not know the feature and says so)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
@@ -50,7 +51,7 @@ def build(force=False, verbose=False, timing=False):
     for s in SOURCES:
         src = os.path.join(CSRC, s)
         obj = os.path.join(OBJ, s.replace(".hip", ".o"))
-        if force or _stale(obj, [src] + HEADERS):
+        if force or _stale(obj, [src] + HEADERS + [os.path.join(CSRC, h) for h in OWN_HEADERS.get(s, [])]):
             jobs.append((src, obj))
 
     def compile_one(job):

@@ -1,0 +1,131 @@
+// Tiles of C = A B^T on the matrix cores, both operands stored with the reduction index contiguous, staged through LDS by DMA.
+//
+// A stage holds RB bytes of every row of the tile (BM rows of A, BN rows of B).  One DMA instruction of a wave lands 1 KB lane-linear in LDS, so the
+// 16-byte XOR swizzle that spreads a fragment read over all banks is applied to the per-lane SOURCE address and again on the read: LDS row r
+// holds source chunk (slot ^ key(r)).  ST buffers form a ring; the loads of stage s + ST - 1 are requested right after the barrier that releases the
+// buffer of stage s - 1 and waited for with a counted vmcnt, so ST - 1 stages of arithmetic cover the memory latency.
+//
+// Operand rows beyond the matrix are clamped to its last row: they are read, multiplied and never stored.  The reduction length is a whole number of
+// stages; what lies behind the real end of a row is zero in memory.
+#pragma once
+#include "common.h"
+
+namespace saunet {
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(16))) int i32x16;
+
+// lane-linear 1 KB from (uniform base + per-lane byte offset) to LDS address lds_dst; M0 is restored for the compiler's own use
+__device__ __forceinline__ void nt_dma16(const char* sbase, unsigned voff, unsigned lds_dst)
+{
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff), "s"(sbase), "s"(lds_dst) : "memory");
+}
+__device__ __forceinline__ const char* nt_uniform(const char* p)
+{
+    const unsigned long long u = (unsigned long long)p;
+    return (const char*)(((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)u));
+}
+// all LDS reads of this wave have returned and at most N of its DMA requests are in flight, then the workgroup barrier
+template <int N> __device__ __forceinline__ void nt_wait_barrier()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(N) : "memory");
+}
+
+// float16 pairs: a row is a sequence of blocks of 32 elements, each 64 bytes of high parts followed by 64 bytes of low parts (x = hi + lo to 2^-24
+// of x).  hi hi + hi lo + lo hi in float32; what is dropped, lo lo, is below 2^-24 of |a| |b|.
+struct NtF16Pair {
+    static constexpr int RB = 128, KSUB = 2, PARTS = 2;
+    typedef f32x16 Acc;
+    static __device__ __forceinline__ int chunk(int ks, int part, int half) { return part * 4 + ks * 2 + half; }
+    static __device__ __forceinline__ void mma(const u32x4 (&a)[2], const u32x4 (&b)[2], Acc& c)
+    {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a[1]), __builtin_bit_cast(f16x8_t, b[0]), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a[0]), __builtin_bit_cast(f16x8_t, b[1]), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a[0]), __builtin_bit_cast(f16x8_t, b[0]), c, 0, 0, 0);
+    }
+};
+// int8, 64 elements a stage
+struct NtI8 {
+    static constexpr int RB = 64, KSUB = 2, PARTS = 1;
+    typedef i32x16 Acc;
+    static __device__ __forceinline__ int chunk(int ks, int, int half) { return ks * 2 + half; }
+    static __device__ __forceinline__ void mma(const u32x4 (&a)[1], const u32x4 (&b)[1], Acc& c)
+    {
+        c = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a[0]), __builtin_bit_cast(i32x4, b[0]), c, 0, 0, 0);
+    }
+};
+
+// BM x BN tile by WGM x WGN waves; wave (wm, wn) owns TM x TN blocks of 32 x 32.  Accumulator element r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4
+// (operand A), column l % 32 (operand B).
+template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore {
+    static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, ST = ST_, RB = Op::RB;
+    static constexpr int NW = WGM * WGN, NT = NW * 64, TM = BM / WGM / 32, TN = BN / WGN / 32;
+    static constexpr int STAGE = (BM + BN) * RB, LDS = ST * STAGE, CPR = RB / 16, RPI = 1024 / RB;
+    static constexpr int QA = BM * RB / 1024 / NW, QB = BN * RB / 1024 / NW, LPW = QA + QB;
+    static_assert(QA * NW * 1024 == BM * RB && QB * NW * 1024 == BN * RB, "every wave requests whole instructions of one operand");
+    static_assert((ST - 2) * LPW < 64, "vmcnt counts to 63");
+    typedef typename Op::Acc Acc;
+
+    static __device__ __forceinline__ int key(int row) { return CPR == 8 ? (row & 7) : ((row >> 1) & 3); }
+
+    // a, b: first byte of the tile's first row at its first stage (uniform); arows, brows: rows that exist from there on (>= 1)
+    static __device__ __forceinline__ void run(const char* a, unsigned lda, int arows, const char* b, unsigned ldb, int brows, int ksteps, unsigned char* smem,
+                                               Acc (&acc)[TM][TN])
+    {
+        a = nt_uniform(a); b = nt_uniform(b);
+        ksteps = __builtin_amdgcn_readfirstlane(ksteps);
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wm = wave / WGN, wn = wave % WGN;
+        const unsigned lds0 = (unsigned)(uintptr_t)smem;
+        unsigned voff[LPW];
+#pragma unroll
+        for (int q = 0; q < LPW; ++q) {
+            const bool isa = q < QA;
+            const int row = ((isa ? q : q - QA) * NW + wave) * RPI + lane / CPR;
+            const int rows = isa ? arows : brows;
+            voff[q] = (unsigned)(row < rows ? row : rows - 1) * (isa ? lda : ldb) + (unsigned)(((lane % CPR) ^ key(row)) * 16);
+        }
+        auto issue = [&](int s) {
+            const unsigned dst = lds0 + (unsigned)(s % ST) * STAGE;
+            const char* pa = a + (long)s * RB;
+            const char* pb = b + (long)s * RB;
+#pragma unroll
+            for (int q = 0; q < LPW; ++q)
+                nt_dma16(q < QA ? pa : pb, voff[q], dst + (q < QA ? q * NW + wave : BM * RB / 1024 + (q - QA) * NW + wave) * 1024);
+        };
+        const int r0 = lane & 31, half = lane >> 5, k0 = key(r0);
+        for (int s = 0; s < ST - 1 && s < ksteps; ++s) issue(s);
+        for (int s = 0; s < ksteps; ++s) {
+            const int left = ksteps - 1 - s;                   // requested stages behind this one: min(left, ST - 2)
+            if (ST < 3 || left >= ST - 2) nt_wait_barrier<(ST - 2) * LPW>();
+            else if (ST > 3 && left == 1) nt_wait_barrier<LPW>();
+            else if (ST > 4 && left == 2) nt_wait_barrier<2 * LPW>();
+            else nt_wait_barrier<0>();
+            if (s + ST - 1 < ksteps) issue(s + ST - 1);
+            const unsigned char* st = smem + (s % ST) * STAGE;
+            const unsigned char* sa = st + (wm * (BM / WGM) + r0) * RB;
+            const unsigned char* sb = st + BM * RB + (wn * (BN / WGN) + r0) * RB;
+#pragma unroll
+            for (int ks = 0; ks < Op::KSUB; ++ks) {
+                u32x4 fa[TM][Op::PARTS], fb[TN][Op::PARTS];
+#pragma unroll
+                for (int p = 0; p < Op::PARTS; ++p) {
+                    const int at = (Op::chunk(ks, p, half) ^ k0) * 16;
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) fa[i][p] = *(const u32x4*)(sa + i * 32 * RB + at);
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) fb[j][p] = *(const u32x4*)(sb + j * 32 * RB + at);
+                }
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) Op::mma(fa[i], fb[j], acc[i][j]);
+            }
+        }
+    }
+};
+
+}  // namespace saunet

@@ -8,7 +8,9 @@ Backward passes are written by hand so that producer/consumer fusion survives di
   * concatenation is a write into a channel slice.
 """
 import ctypes as C
+import math
 import os
+import struct
 import weakref
 
 import torch
@@ -2235,3 +2237,229 @@ def mask_to_edges(seg, num_classes=3):
     out = torch.empty((n, 1, h, w), dtype=torch.float32, device=seg.device)
     L.call("saunet_mask_to_edges", seg.data_ptr(), n, h, w, int(num_classes), out.data_ptr(), L.stream())
     return out
+
+
+# ------------------------------------------------------------------------------------------------ orthogonalised updates
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def ns_desc(rows, dtype, steps, coefficients, eps, adjust=0):
+    """saunet_ns_desc over `rows`, a flat list of (src, dst, buf, ld_src, ld_dst, rows, cols) per matrix; keep the pair referenced until the call returns"""
+    n = len(rows) // 7
+    items = struct.pack("@" + "PPPqqii" * n, *rows)
+    d = L.NsDesc()
+    buf = C.create_string_buffer(items, len(items))
+    d.item, d.count, d.dtype, d.steps, d.adjust = C.addressof(buf), n, dtype, steps, adjust
+    d.a, d.b, d.c = coefficients
+    d.eps = eps
+    return d, buf
+
+
+def ns_workspace(d, device):
+    need = L.load().saunet_newton_schulz_workspace(C.byref(d))
+    if need < 0:
+        L._check(int(need), "saunet_newton_schulz_workspace")
+    return torch.empty(int(need), dtype=torch.uint8, device=device)
+
+
+def ns_check_hyper(steps, coefficients, eps):
+    if int(steps) != steps or not 1 <= steps <= 32:
+        raise ValueError("Newton-Schulz takes 1 to 32 whole steps, got %r" % (steps,))
+    if len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients):
+        raise ValueError("Newton-Schulz coefficients are three finite numbers, got %r" % (coefficients,))
+    if not eps >= 1e-30 or not math.isfinite(eps):
+        raise ValueError("Newton-Schulz eps has to be a positive number, got %r" % (eps,))
+
+
+def newton_schulz(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
+    """The orthogonal factor of a matrix by an odd quintic iteration: X = g / max(|g|_F, eps), then ``steps`` times
+    X <- (a I + b S + c S^2) X with S = X X^T (S = X^T X where a matrix has more rows than columns).
+
+    ``g``: [..., m, n] in float32, bfloat16 or float16 (leading dimensions: a batch), or a list of such tensors of any shapes and one dtype on
+    one device.  Returns the same shapes and dtype (a list for a list).  Every intermediate is of float32 class whatever the dtype; all matrices of the
+    call go through one chain of about twenty launches.  A matrix that holds an Inf or NaN comes out as NaN; a zero matrix stays zero.
+    Coefficients under which singular values in [0, 1] grow out of range are refused.  Not differentiable: an optimiser's update is its use."""
+    ns_check_hyper(steps, coefficients, eps)
+    many = isinstance(g, (list, tuple))
+    ts = list(g) if many else [g]
+    if not ts:
+        return []
+    rows, outs, keep = [], [], []
+    for t in ts:
+        _check_dev(t)
+        if t.dim() < 2:
+            raise RuntimeError("newton_schulz expects matrices [..., m, n], got %s" % (tuple(t.shape),))
+        if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise RuntimeError("newton_schulz takes float32, bfloat16 or float16, not %s" % t.dtype)
+        if t.dtype != ts[0].dtype or t.device != ts[0].device:
+            raise RuntimeError("newton_schulz takes one dtype and one device a call")
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise RuntimeError("newton_schulz is not differentiable: call it on a detached tensor or under torch.no_grad()")
+        t = t.detach()
+        m, n = t.shape[-2:]
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        outs.append(out)
+        if t.numel() == 0:
+            continue
+        # batches are walked as one stack of matrices: any row stride, unit column stride
+        v = t if t.dim() == 2 else t.reshape(-1, m, n)
+        if (n > 1 and v.stride(-1) != 1) or (m > 1 and v.stride(-2) < n):
+            v = v.contiguous()
+        keep.append(v)
+        b = 1 if v.dim() == 2 else v.shape[0]
+        size, ld = t.element_size(), (v.stride(-2) if m > 1 else n)
+        step = 0 if v.dim() == 2 else v.stride(0)
+        for i in range(b):
+            rows += (v.data_ptr() + i * step * size, out.data_ptr() + i * m * n * size, 0, ld, n, m, n)
+    with torch.cuda.device(ts[0].device):
+        for s0 in range(0, len(rows), 7 * L.NS_ITEMS_MAX):
+            d, hold = ns_desc(rows[s0:s0 + 7 * L.NS_ITEMS_MAX], L.matrix_dtype_code(ts[0]), steps, coefficients, eps)
+            ws = ns_workspace(d, ts[0].device)
+            L.call("saunet_newton_schulz", C.byref(d), ws.data_ptr(), ws.numel(), L.stream())
+    return outs if many else outs[0]
+
+
+# ------------------------------------------------------------------------------------------------ int8 matrix products
+INT8_K_MAX = 131071          # 2^31 / 128^2: the integer sum of a product stays inside 32 bits
+
+
+def _int8_stride(k):
+    return (k + 63) // 64 * 64
+
+
+class Int8Rows:
+    """Rows of int8 with one float32 scale each -- quantised tokens (pixels) or the output channels of a weight: row r stands for q[r] * scale[r].
+
+    Storage is padded with zeros to whole 64-byte steps of the reduction, once, so that the products need no tail.  Build it with ``quantize_rows``
+    or from existing ``q`` [..., k] int8 and ``scale`` [...] float32 (copied when the layout asks for it)."""
+
+    def __init__(self, q, scale):
+        _check_dev(q); _check_dev(scale)
+        if q.dtype != torch.int8 or scale.dtype != torch.float32:
+            raise RuntimeError("Int8Rows takes int8 rows and float32 scales, got %s and %s" % (q.dtype, scale.dtype))
+        if q.dim() < 1 or tuple(scale.shape) != tuple(q.shape[:-1]) or scale.device != q.device:
+            raise RuntimeError("Int8Rows: one scale a row, beside it: %s on %s and %s on %s" % (tuple(q.shape), q.device, tuple(scale.shape), scale.device))
+        k = q.shape[-1]
+        if not 1 <= k <= INT8_K_MAX:
+            raise RuntimeError("Int8Rows: rows of 1 to %d elements, not %d" % (INT8_K_MAX, k))
+        rows = q.reshape(-1, k) if q.numel() else q.new_empty(scale.numel(), k)
+        if k % 64 or not rows.is_contiguous() or rows.data_ptr() % 16:
+            data = torch.zeros(rows.shape[0], _int8_stride(k), dtype=torch.int8, device=q.device)
+            data[:, :k] = rows
+        else:
+            data = rows
+        self._set(data, scale.reshape(-1).contiguous(), k, tuple(q.shape[:-1]))
+
+    def _set(self, data, scale, k, lead):
+        self.data, self.scale, self.k, self.lead = data, scale, k, lead
+
+    @classmethod
+    def _wrap(cls, data, scale, k, lead):
+        r = cls.__new__(cls)
+        r._set(data, scale, k, lead)
+        return r
+
+    @property
+    def shape(self):
+        return self.lead + (self.k,)
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def q(self):
+        return self.data[:, :self.k].reshape(self.shape)
+
+    def dequantize(self, dtype=torch.float32):
+        return (self.data[:, :self.k].float() * self.scale[:, None]).to(dtype).view(self.shape)
+
+
+def _float_rows(x, who):
+    """x [..., k] as (row view [rows, k] with unit column stride, k)"""
+    _check_dev(x)
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise RuntimeError("%s takes float32, bfloat16 or float16 rows, not %s" % (who, x.dtype))
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= INT8_K_MAX:
+        raise RuntimeError("%s: rows of 1 to %d elements, got %s" % (who, INT8_K_MAX, tuple(x.shape)))
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError("%s serves inference: call it under torch.no_grad() or on a detached tensor" % who)
+    k = x.shape[-1]
+    v = x.detach().reshape(-1, k) if x.numel() else x.detach().new_empty(0, k)
+    if v.shape[0] and ((k > 1 and v.stride(1) != 1) or (v.shape[0] > 1 and v.stride(0) < k)):
+        v = v.contiguous()
+    return v, k
+
+
+def quantize_rows(x, affine=None, relu=False):
+    """x [..., k] float -> Int8Rows: per row s = fl32(max |v| / 127), q = round-half-even(v / s) of the exact quotient, v = x or, with
+    ``affine`` = (scale [k], shift [k]) and ``relu``, max(x * scale + shift, 0) -- a BatchNorm + ReLU in front of a 1x1 convolution.
+    A row with an Inf or NaN gets s = NaN (its products are NaN); a row of zeros s = 0."""
+    v, k = _float_rows(x, "quantize_rows")
+    if affine is not None:
+        for t in affine:
+            _check_dev(t)
+            if t.dtype != torch.float32 or t.numel() != k or not t.is_contiguous() or t.device != x.device:
+                raise RuntimeError("quantize_rows: affine is two contiguous float32 vectors of %d elements beside x" % k)
+    rows, ld = v.shape[0], _int8_stride(k)
+    data = torch.empty(rows, ld, dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if rows:
+        with torch.cuda.device(x.device):
+            L.call("saunet_quantize_rows", L.matrix_dtype_code(v), v.data_ptr(), v.stride(0) if rows > 1 else k, rows, k,
+                   L.ptr(affine[0]) if affine is not None else None, L.ptr(affine[1]) if affine is not None else None, 1 if relu else 0,
+                   data.data_ptr(), ld, scale.data_ptr(), L.stream())
+    return Int8Rows._wrap(data, scale, k, tuple(x.shape[:-1]))
+
+
+def _int8_out(lead, rows, n, dtype, device, out):
+    """-> (what the caller gets, its [rows, n] view)"""
+    if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise RuntimeError("int8 products come as float32, bfloat16 or float16, not %s" % dtype)
+    if out is None:
+        out = torch.empty(lead + (n,), dtype=dtype, device=device)
+        return out, out.view(rows, n)
+    if tuple(out.shape) != lead + (n,) or out.dtype != dtype or out.device != device:
+        raise RuntimeError("out has to be %s of %s on %s" % (lead + (n,), dtype, device))
+    v = out if out.dim() == 2 else out.view(rows, n)
+    if (n > 1 and v.stride(1) != 1) or (rows > 1 and v.stride(0) < n):
+        raise RuntimeError("out needs rows of unit stride that do not overlap")
+    return out, v
+
+
+def _int8_bias(bias, n, device):
+    if bias is None:
+        return None
+    if bias.numel() != n or bias.device != device:
+        raise RuntimeError("bias has to hold %d elements on %s" % (n, device))
+    return bias.detach().float().contiguous()
+
+
+def matmul_int8(a, b, bias=None, relu=False, dtype=torch.bfloat16, out=None):
+    """y[..., n] = (sum_k a.q[..., k] b.q[n, k]) a.scale[...] b.scale[n] + bias[n], clamped at zero with ``relu``: Int8Rows of tokens (pixels) times
+    Int8Rows of weight channels.  The integer sum is exact; ``dtype`` (float32, bfloat16, float16) is rounded to once.  ``out``: rows of unit stride,
+    a channel slice of a wider buffer among them."""
+    if not isinstance(a, Int8Rows) or not isinstance(b, Int8Rows):
+        raise RuntimeError("matmul_int8 takes Int8Rows (quantize_rows, or Int8Rows(q, scale))")
+    if len(b.lead) != 1:
+        raise RuntimeError("the weight of an int8 product is [n, k], got %s" % (b.shape,))
+    if a.k != b.k or a.device != b.device:
+        raise RuntimeError("matmul_int8: %s on %s does not meet %s on %s" % (a.shape, a.device, b.shape, b.device))
+    rows, n = a.data.shape[0], b.lead[0]
+    y, yv = _int8_out(a.lead, rows, n, dtype, a.device, out)
+    bias = _int8_bias(bias, n, a.device)
+    if rows and n:
+        d = L.Int8Desc()
+        d.a, d.a_scale, d.lda, d.m = a.data.data_ptr(), a.scale.data_ptr(), a.data.shape[1], rows
+        d.b, d.b_scale, d.ldb, d.n, d.k = b.data.data_ptr(), b.scale.data_ptr(), b.data.shape[1], n, a.k
+        d.bias, d.y, d.ldy = L.ptr(bias), yv.data_ptr(), yv.stride(0) if rows > 1 else n
+        d.dtype, d.relu = L.matrix_dtype_code(yv), 1 if relu else 0
+        with torch.cuda.device(a.device):
+            L.call("saunet_matmul_int8", C.byref(d), L.stream())
+    return y
+
+
+def linear_int8(x, w, bias=None, relu=False, dtype=None, out=None):
+    """A linear layer over rows x [..., k] with an int8 weight ``w`` (Int8Rows [n, k]): the rows are quantised on the way (quantize_rows), the product is
+    matmul_int8's.  ``dtype``: the result's, x's by default."""
+    return matmul_int8(quantize_rows(x), w, bias, relu, x.dtype if dtype is None else dtype, out)

@@ -11,7 +11,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SAUNET_HIP_LIB") or os.path.join(_HERE, "libsaunet_hip.so")      # the override serves A/B kernel measurements
 
-F32, BF16 = 0, 1
+F32, BF16, F16 = 0, 1, 2
 PACK_FWD, PACK_DGRAD, PACK_CONVT_FWD, PACK_CONVT_DGRAD = 0, 1, 2, 3
 
 
@@ -85,6 +85,28 @@ class DenseBn1List(C.Structure):
 
 class TensorList(C.Structure):
     _fields_ = [("count", C.c_int32), ("ptrs", (C.c_void_p * 96) * 4), ("numel", C.c_int64 * 96)]
+
+
+class NsItem(C.Structure):
+    """saunet_ns_item"""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("buf", C.c_void_p), ("ld_src", C.c_int64), ("ld_dst", C.c_int64),
+                ("rows", C.c_int32), ("cols", C.c_int32)]
+
+
+NS_ITEMS_MAX = 4096
+
+
+class NsDesc(C.Structure):
+    """saunet_ns_desc"""
+    _fields_ = [("item", C.c_void_p), ("count", C.c_int32), ("dtype", C.c_int32), ("steps", C.c_int32), ("adjust", C.c_int32),
+                ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float)]
+
+
+class Int8Desc(C.Structure):
+    """saunet_int8_desc"""
+    _fields_ = [("a", C.c_void_p), ("a_scale", C.c_void_p), ("lda", C.c_int64), ("m", C.c_int64), ("b", C.c_void_p), ("b_scale", C.c_void_p),
+                ("ldb", C.c_int64), ("n", C.c_int32), ("k", C.c_int32), ("bias", C.c_void_p), ("y", C.c_void_p), ("ldy", C.c_int64),
+                ("dtype", C.c_int32), ("relu", C.c_int32)]
 
 
 vp, i32, i64, f32, f64 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double
@@ -179,6 +201,11 @@ _SIGS = {
     "saunet_sgd_step": [C.POINTER(TensorList), vp, vp],
     "saunet_radam_step": [C.POINTER(TensorList), vp, vp],
     "saunet_adam_step": [C.POINTER(TensorList), vp, vp],
+    "saunet_newton_schulz_workspace": [C.POINTER(NsDesc)],
+    "saunet_newton_schulz": [C.POINTER(NsDesc), vp, i64, vp],
+    "saunet_muon_step": [C.POINTER(NsDesc), vp, vp, i64, vp],
+    "saunet_quantize_rows": [i32, vp, i64, i64, i32, vp, vp, i32, vp, i64, vp, vp],
+    "saunet_matmul_int8": [C.POINTER(Int8Desc), vp],
     "saunet_bucket_copy": [C.POINTER(TensorList), i32, f32, vp],
 }
 ABI_VERSION = 4          # include/saunet_hip.h: SAUNET_ABI_VERSION (the struct layouts below mirror that header)
@@ -236,6 +263,11 @@ def stream():
 
 def ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def matrix_dtype_code(t):
+    """storage type of the matrix operators (newton_schulz, the int8 products): float16 too"""
+    return F16 if t.dtype == torch.float16 else dtype_code(t)
 
 
 def dtype_code(t):

@@ -243,6 +243,69 @@ class FusedAdam(_FusedBase):
         HF.PACKS.invalidate()
 
 
+class FusedMuon(_FusedBase):
+    """Muon: the momentum of a weight matrix, orthogonalised by Newton-Schulz steps, is its update (functional.newton_schulz).
+
+      buf <- momentum buf + (1 - momentum) grad;   u = (1 - momentum) grad + momentum buf  (nesterov)  or  buf
+      p <- (1 - lr weight_decay) p - lr adjust NewtonSchulz(u)
+
+    ``adjust_lr_fn``: "original" (None): sqrt(max(1, rows / cols));  "match_rms_adamw": 0.2 sqrt(max(rows, cols)) -- learning rate and decay tuned for
+    Adam carry over.  Arguments, defaults and state as torch.optim.Muon has them; a convolution weight [O, I, kh, kw] is the matrix O x (I kh kw).
+    Parameters with fewer than two dimensions belong to another optimiser (create_optimizers("muon", ...) pairs it with FusedAdam).  The whole list is
+    one chain of launches, float32-class throughout; the step can be captured (graph.GraphedStep): lr, momentum, weight decay and grad_scale
+    are read from the device array."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=HF.NS_COEFFICIENTS, eps=1e-7, ns_steps=5,
+                 adjust_lr_fn=None):
+        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
+            raise ValueError("adjust_lr_fn is None, 'original' or 'match_rms_adamw', not %r" % (adjust_lr_fn,))
+        if not lr >= 0 or not 0 <= momentum < 1 or not weight_decay >= 0:
+            raise ValueError("Muon takes lr >= 0, 0 <= momentum < 1, weight_decay >= 0, got %r, %r, %r" % (lr, momentum, weight_decay))
+        HF.ns_check_hyper(ns_steps, ns_coefficients, eps)
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov, ns_coefficients=tuple(ns_coefficients),
+                                      eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                del self.param_groups[-1]
+                raise ValueError("Muon updates matrices: a parameter of shape %s belongs to another optimiser" % (tuple(p.shape),))
+
+    def upload_hyper(self):
+        for g in self.param_groups:
+            self._upload(g, [g["lr"], g["momentum"], g["weight_decay"], 1.0 if g["nesterov"] else 0.0, self.grad_scale, 0, 0, 0])
+
+    @torch.no_grad()
+    def step(self, closure=None, upload=True):
+        if upload:
+            self.upload_hyper()
+        for g in self.param_groups:
+            rows = []
+            ps = [p for p in self._live(g) if p.numel()]
+            for p in ps:
+                if p.dtype != torch.float32 or p.device != ps[0].device:
+                    raise RuntimeError("FusedMuon takes float32 parameters on one device a group")
+                st = self.state[p]
+                if "momentum_buffer" not in st:
+                    st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                b = st["momentum_buffer"]
+                if b.dtype != torch.float32 or b.device != p.device or b.shape != p.shape or not b.is_contiguous():
+                    raise RuntimeError("FusedMuon needs contiguous float32 momentum buffers beside their parameters")
+                m = p.shape[0]
+                n = p.numel() // m
+                rows += (p.grad.data_ptr(), p.data_ptr(), b.data_ptr(), n, n, m, n)
+            if not rows:
+                continue
+            with torch.cuda.device(ps[0].device):
+                for s0 in range(0, len(rows), 7 * L.NS_ITEMS_MAX):
+                    d, hold = HF.ns_desc(rows[s0:s0 + 7 * L.NS_ITEMS_MAX], L.F32, g["ns_steps"], g["ns_coefficients"], g["eps"],
+                                         1 if g["adjust_lr_fn"] == "match_rms_adamw" else 0)
+                    ws = HF.ns_workspace(d, ps[0].device)
+                    L.call("saunet_muon_step", C.byref(d), self._hyper(g).data_ptr(), ws.data_ptr(), ws.numel(), L.stream())
+        HF.PACKS.invalidate()
+
+
 def create_optimizers(unet, optimizer="sgd", lr=5e-4, momentum=0.9, weight_decay=1e-4):
     """train.py:187-207 (defaults = train.py's argparse defaults)."""
     groups = group_weight(unet)
@@ -253,4 +316,12 @@ def create_optimizers(unet, optimizer="sgd", lr=5e-4, momentum=0.9, weight_decay
         return [FusedAdam(groups, lr=lr, betas=(0.9, 0.999))]
     if name == "radam":
         return [FusedRAdam(groups, lr=lr, betas=(0.9, 0.999))]
-    raise ValueError("optimizer %s: train.py:187-207 knows sgd, adam and radam" % optimizer)
+    if name == "muon":
+        # matrices (a convolution weight is O x (I kh kw)) to Muon, whose step is scaled to Adam's so that one learning rate serves both;
+        # vectors -- biases, normalisation, weights with a single row or column -- to Adam
+        mats = [p for p in groups[0]["params"] if p.shape[0] > 1 and p.numel() > p.shape[0]]
+        ids = {id(p) for p in mats}
+        rest = [p for g in groups for p in g["params"] if id(p) not in ids]
+        return [FusedMuon(mats, lr=lr, weight_decay=weight_decay, momentum=momentum, adjust_lr_fn="match_rms_adamw"),
+                FusedAdam(rest, lr=lr, betas=(0.9, 0.999))]
+    raise ValueError("optimizer %s: sgd, adam and radam (train.py:187-207) or muon" % optimizer)

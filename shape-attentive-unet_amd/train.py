@@ -108,8 +108,9 @@ def train_one_epoch(sm, loader, optimizers, epoch, args, history, buckets=None, 
     sm.train(not args.fix_bn)
     if epoch == args.start_epoch and args.start_epoch > 1:
         args.running_lr_encoder = poly_resume_lr(args.lr_encoder, epoch, args.num_epoch, args.lr_pow)
-        for g in optimizers[0].param_groups:
-            g["lr"] = args.running_lr_encoder
+        for opt in optimizers:
+            for g in opt.param_groups:
+                g["lr"] = args.running_lr_encoder
     tic = time.time()
     pending = []
     for it, batch in enumerate(loader):
@@ -196,7 +197,7 @@ def build_parser():
     p.add_argument("--num_epoch", type=int, default=120)
     p.add_argument("--start_epoch", type=int, default=1)
     p.add_argument("--batch_size_per_gpu", type=int, default=1)
-    p.add_argument("--optimizer", default="sgd")
+    p.add_argument("--optimizer", default="sgd", help="sgd, adam, radam, or muon (matrices by Muon, vectors by Adam)")
     p.add_argument("--lr_encoder", type=float, default=5e-4)
     p.add_argument("--lr_pow", type=float, default=0.9)
     p.add_argument("--beta1", type=float, default=0.9)
