@@ -56,7 +56,41 @@ __device__ __forceinline__ int q_round(float x, const QScale& s)
     return (int)q;
 }
 
+// four of them as bytes.  x * inv + 1.5 * 2^23 rounds half to even in its last place and holds q in its low byte; only a quotient within rounding of a
+// half takes the exact path.
+__device__ __forceinline__ unsigned q_round4(const float* x, const QScale& s)
+{
+    unsigned w[4];
+    bool close = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float t = fmaf(x[j], s.inv, 12582912.f);
+        close |= fabsf(fmaf(-(t - 12582912.f), s.s, x[j])) >= 0.49999f * s.s;
+        w[j] = __float_as_uint(t);
+    }
+    if (close || !(s.inv > 0.f)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = (unsigned)q_round(x[j], s);
+    }
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x00000400u), __builtin_amdgcn_perm(w[1], w[0], 0x00000400u), 0x05040100u);
+}
+
 struct QArgs { const void* x; long ldx; long rows; int k; const float* scale; const float* shift; int relu; signed char* q; long ldq; float* s; int vec; };
+
+// the largest of `top` over the G lanes of a row (256: the workgroup)
+template <int G> __device__ __forceinline__ unsigned q_top(unsigned top)
+{
+#pragma unroll
+    for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) { const unsigned b = __shfl_xor(top, o, 64); top = b > top ? b : top; }
+    if (G == 256) {
+        __shared__ unsigned s_top[4];
+        if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = s_top[w] > top ? s_top[w] : top;
+    }
+    return top;
+}
 
 // G lanes a row, NV vectors a lane kept in registers (k <= G * NV * V, 16-byte aligned rows); NV == 0: any k and alignment, the row is read twice
 template <typename T, int G, int NV> __global__ __launch_bounds__(256) void quantize_rows_kernel(QArgs a)
@@ -71,33 +105,32 @@ template <typename T, int G, int NV> __global__ __launch_bounds__(256) void quan
     unsigned top = 0;
     if (NV > 0) {
         float f[NV ? NV : 1][V];
+        u32x4 v[NV ? NV : 1];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + lane) * V;
-            u32x4 v = {0u, 0u, 0u, 0u};
-            if (c + V <= a.k) v = *(const u32x4*)(x + c);
-            QElem<T>::unpack(v, f[i]);
-            if (c < a.k && c + V > a.k) for (int j = 0; j < V; ++j) f[i][j] = c + j < a.k ? QElem<T>::load(x + c + j) : 0.f;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (c + j < a.k) f[i][j] = pro(f[i][j], c + j);
-                const unsigned b = __float_as_uint(f[i][j]) & 0x7fffffffu;
-                top = b > top ? b : top;
-            }
+            v[i] = u32x4{0u, 0u, 0u, 0u};
+            if (c + V <= a.k) v[i] = *(const u32x4*)(x + c);
         }
 #pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) { const unsigned b = __shfl_xor(top, o, G); top = b > top ? b : top; }
-        const QScale s = q_scale(top);
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * G + lane) * V;
+            QElem<T>::unpack(v[i], f[i]);
+            if (c < a.k && c + V > a.k) for (int j = 0; j < V; ++j) f[i][j] = c + j < a.k ? QElem<T>::load(x + c + j) : 0.f;
+            if (a.scale || a.relu)
+#pragma unroll
+                for (int j = 0; j < V; ++j) if (c + j < a.k) f[i][j] = pro(f[i][j], c + j);
+#pragma unroll
+            for (int j = 0; j < V; ++j) { const unsigned b = __float_as_uint(f[i][j]) & 0x7fffffffu; top = b > top ? b : top; }
+        }
+        const QScale s = q_scale(q_top<G>(top));
         if (lane == 0) a.s[row] = s.s;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + lane) * V;
             if (c >= a.ldq) continue;
-            unsigned w[2] = {0u, 0u};
-#pragma unroll
-            for (int j = 0; j < V; ++j) w[j >> 2] |= ((unsigned)q_round(f[i][j], s) & 255u) << ((j & 3) * 8);
-            if (V == 8) *(u32x2*)(q + c) = u32x2{w[0], w[1]};
-            else *(unsigned*)(q + c) = w[0];
+            if (V == 8) *(u32x2*)(q + c) = u32x2{q_round4(f[i], s), q_round4(f[i] + (V == 8 ? 4 : 0), s)};
+            else *(unsigned*)(q + c) = q_round4(f[i], s);
         }
         for (int c = (NV * G + lane) * V; c < a.ldq; c += G * V) {       // padding beyond the registers' reach
             if (V == 8) *(u32x2*)(q + c) = u32x2{0u, 0u};
@@ -105,31 +138,32 @@ template <typename T, int G, int NV> __global__ __launch_bounds__(256) void quan
         }
     } else {
         for (int c = lane; c < a.k; c += G) { const unsigned b = __float_as_uint(pro(QElem<T>::load(x + c), c)) & 0x7fffffffu; top = b > top ? b : top; }
-#pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) { const unsigned b = __shfl_xor(top, o, G); top = b > top ? b : top; }
-        const QScale s = q_scale(top);
+        const QScale s = q_scale(q_top<G>(top));
         if (lane == 0) a.s[row] = s.s;
         for (int c = lane * 4; c < a.ldq; c += G * 4) {
-            unsigned w = 0u;
+            float f[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (c + j < a.k) w |= ((unsigned)q_round(pro(QElem<T>::load(x + c + j), c + j), s) & 255u) << (j * 8);
-            *(unsigned*)(q + c) = w;
+            for (int j = 0; j < 4; ++j) f[j] = c + j < a.k ? pro(QElem<T>::load(x + c + j), c + j) : 0.f;
+            *(unsigned*)(q + c) = q_round4(f, s);
         }
     }
 }
 
+// Lanes a row: as few as hold it in one or two vectors each, so that a wave keeps several short rows in flight; a workgroup to a row where there are
+// fewer rows than would fill the card with a wave each
 template <typename T> static void q_launch(const QArgs& a, hipStream_t st)
 {
     constexpr int V = QElem<T>::V;
 #define Q_GO(G, NV) hipLaunchKernelGGL((quantize_rows_kernel<T, G, NV>), dim3((unsigned)((a.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, st, a)
-    if (!a.vec) Q_GO(64, 0);
+    const bool few = a.rows <= 1024 && a.k > 128 * V;
+    if (!a.vec || a.k > 1024 * V) { if (a.rows <= 4096 && a.k > 256) Q_GO(256, 0); else Q_GO(64, 0); }
     else if (a.k <= 16 * V) Q_GO(16, 1);
     else if (a.k <= 32 * V) Q_GO(16, 2);
     else if (a.k <= 64 * V) Q_GO(64, 1);
     else if (a.k <= 128 * V) Q_GO(64, 2);
-    else if (a.k <= 256 * V) Q_GO(64, 4);
-    else if (a.k <= 512 * V) Q_GO(64, 8);
-    else Q_GO(64, 0);
+    else if (a.k <= 256 * V) { if (few) Q_GO(256, 1); else Q_GO(64, 4); }
+    else if (a.k <= 512 * V) { if (few) Q_GO(256, 2); else Q_GO(64, 8); }
+    else Q_GO(256, 4);
 #undef Q_GO
 }
 
@@ -137,26 +171,34 @@ template <typename T> static void q_launch(const QArgs& a, hipStream_t st)
 struct I8Args { const char* a; const float* sa; long lda; long m; const char* b; const float* sb; long ldb; int n; int ksteps; const float* bias; int relu; void* y; long ldy; int vec; int tn; };
 
 template <typename T> struct YElem;
-template <> struct YElem<float> { static __device__ __forceinline__ float cvt(float v) { return v; } };
-template <> struct YElem<u16> { static __device__ __forceinline__ u16 cvt(float v) { return __builtin_bit_cast(u16, (__bf16)v); } };
-template <> struct YElem<_Float16> { static __device__ __forceinline__ _Float16 cvt(float v) { return (_Float16)v; } };
+template <> struct YElem<float> { typedef f32x4 V4; static __device__ __forceinline__ float cvt(float v) { return v; } };
+template <> struct YElem<u16> { typedef __attribute__((ext_vector_type(4))) u16 V4; static __device__ __forceinline__ u16 cvt(float v) { return __builtin_bit_cast(u16, (__bf16)v); } };
+template <> struct YElem<_Float16> { typedef __attribute__((ext_vector_type(4))) _Float16 V4; static __device__ __forceinline__ _Float16 cvt(float v) { return (_Float16)v; } };
 
 // Operand A of the MFMA is the WEIGHT tile (BM channels), operand B the token tile (BN tokens): a lane then holds four consecutive channels of one token.
 // The wave's 32 tokens x (BM / WGM) channels go through LDS so that the stores are whole rows of the tile.
 template <typename T, class Core> __global__ __launch_bounds__(Core::NT) void matmul_int8_kernel(I8Args g)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-    const int tn = g.tn, id = blockIdx.x;                       // channel tiles run fastest: the workgroups beside each other share the token tile
-    const long m0 = (long)(id / tn) * Core::BN;
-    const int n0 = (id % tn) * Core::BM;
+    int tt, tc;
+    nt_place(blockIdx.x, gridDim.x, (int)((g.m + Core::BN - 1) / Core::BN), g.tn, tt, tc);
+    const long m0 = (long)tt * Core::BN;
+    const int n0 = tc * Core::BM;
     typename Core::Acc acc[Core::TM][Core::TN] = {};
     const long ml = g.m - m0;
     Core::run(g.b + (long)n0 * g.ldb, (unsigned)g.ldb, g.n - n0, g.a + m0 * g.lda, (unsigned)g.lda, ml < Core::BN ? (int)ml : Core::BN, g.ksteps, smem, acc);
     __syncthreads();
     constexpr int CH = Core::BM / Core::WGM, PITCH = CH * (int)sizeof(T) + 16;          // one wave: 32 tokens of CH channels
-    static_assert(Core::NW * 32 * PITCH <= 160 * 1024, "the wave's rows fit");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / Core::WGN, wn = wave % Core::WGN, half = lane >> 5, tok = lane & 31;
-    unsigned char* buf = smem + wave * 32 * PITCH;
+    float* s_sb = (float*)smem;
+    float* s_bias = s_sb + Core::BM;
+    for (int c = threadIdx.x; c < Core::BM; c += Core::NT) {
+        const int n = n0 + c < g.n ? n0 + c : g.n - 1;
+        s_sb[c] = g.sb[n];
+        s_bias[c] = g.bias ? g.bias[n] : 0.f;
+    }
+    __syncthreads();
+    unsigned char* buf = smem + Core::BM * 8 + wave * 32 * PITCH;
     const int nw = n0 + wm * CH;
 #pragma unroll
     for (int tj = 0; tj < Core::TN; ++tj) {
@@ -167,17 +209,15 @@ template <typename T, class Core> __global__ __launch_bounds__(Core::NT) void ma
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int c = ti * 32 + q * 8 + half * 4;
-                T o[4];
+                const f32x4 sb = *(const f32x4*)(s_sb + wm * CH + c), bias = *(const f32x4*)(s_bias + wm * CH + c);
+                typename YElem<T>::V4 o;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int n = nw + c + r < g.n ? nw + c + r : g.n - 1;
-                    float v = (float)acc[ti][tj][q * 4 + r] * sa * g.sb[n];
-                    if (g.bias) v += g.bias[n];
+                    float v = fmaf((float)acc[ti][tj][q * 4 + r] * sa, sb[r], bias[r]);
                     if (g.relu && v < 0.f) v = 0.f;
                     o[r] = YElem<T>::cvt(v);
                 }
-                if (sizeof(T) == 4) *(u32x4*)(buf + tok * PITCH + c * sizeof(T)) = *(const u32x4*)o;
-                else *(u32x2*)(buf + tok * PITCH + c * sizeof(T)) = *(const u32x2*)o;
+                *(typename YElem<T>::V4*)(buf + tok * PITCH + c * sizeof(T)) = o;
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the wave's own rows: no other wave reads them
         constexpr int VPR = CH * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);
@@ -196,12 +236,23 @@ template <typename T, class Core> __global__ __launch_bounds__(Core::NT) void ma
     }
 }
 
-typedef NtCore<NtI8, 128, 128, 2, 2, 4> I8Core128;
+// Tile by the amount of work, counted in 64 x 64 tiles (bf16 out; us for channels x tokens of a tile, K the reduction):
+//                                    64x64  128x64  128x128  128x256  256x256
+//   8192 x 4096, K 4096  (8192 tiles)   276     234      178      156      148      a long reduction and work for every CU: operand traffic is the bound
+//   131072 x 128, K 256  (4096 tiles)  21.1    18.2     18.9     16.5     27.9      a short one: memory is, two workgroups a CU overlap loads and stores
+//   2048 x 2048, K 2048  (1024 tiles)  22.4    19.7     18.3     24.9     33.5
+//   8192 x 256, K 8192    (512 tiles)  42.6    36.3     47.6     75.6      101      too few large tiles to fill the card: the smallest that do
+//   512 x 512, K 512       (64 tiles)   4.4     5.4      7.6      8.5     14.1
+typedef NtCore<NtI8, 64, 64, 2, 2, 4> I8Core64;
+typedef NtCore<NtI8, 128, 64, 2, 2, 4> I8CoreTall;
+typedef NtCore<NtI8, 128, 128, 2, 2, 3> I8Core128;
+typedef NtCore<NtI8, 128, 256, 2, 4, 2> I8CoreWide;
+typedef NtCore<NtI8, 256, 256, 2, 4, 4> I8Core256;
 
-template <typename T> static int mm8_launch(I8Args g, hipStream_t st)
+template <typename T, class Core> static int mm8_tiles(I8Args g, hipStream_t st)
 {
-    typedef I8Core128 Core;
-    constexpr int EPI = Core::NW * 32 * (Core::BM / Core::WGM * (int)sizeof(T) + 16), LDS = Core::LDS > EPI ? Core::LDS : EPI;
+    constexpr int EPI = Core::BM * 8 + Core::NW * 32 * (Core::BM / Core::WGM * (int)sizeof(T) + 16), LDS = Core::LDS > EPI ? Core::LDS : EPI;
+    static_assert(LDS <= 160 * 1024, "the wave's rows fit");
     static DeviceOnce once;
     if (once.first()) (void)hipFuncSetAttribute((const void*)matmul_int8_kernel<T, Core>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     g.tn = cdiv(g.n, Core::BM);
@@ -210,6 +261,68 @@ template <typename T> static int mm8_launch(I8Args g, hipStream_t st)
     hipLaunchKernelGGL((matmul_int8_kernel<T, Core>), dim3((unsigned)tiles), dim3(Core::NT), LDS, st, g);
     SAUNET_CHECK_LAUNCH("matmul_int8");
     return SAUNET_OK;
+}
+
+// ---- few tokens: the weight is read once, straight into registers -------------------------------------------------------------------------
+// A workgroup owns 16 channels; its 8 waves take the 64-byte steps of the reduction in turn, mfma_i32_16x16x64_i8 with 16 weight rows against MT x 16
+// tokens, and add their sums through LDS. 
+constexpr int FEW_WAVES = 8, FEW_UNROLL = 8;
+
+template <typename T, int MT> __global__ __launch_bounds__(FEW_WAVES * 64) void matmul_int8_few_kernel(I8Args g)
+{
+    __shared__ int s_red[FEW_WAVES][MT][16][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kq = (lane >> 4) * 16;
+    const int n0 = blockIdx.x * 16;
+    const char* b = g.b + (long)(n0 + r < g.n ? n0 + r : g.n - 1) * g.ldb + kq;
+    const char* a[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) { const long m = t * 16 + r; a[t] = g.a + (m < g.m ? m : g.m - 1) * g.lda + kq; }
+    i32x4 acc[MT] = {};
+    for (int s0 = wave; s0 < g.ksteps; s0 += FEW_WAVES * FEW_UNROLL) {
+        i32x4 fb[FEW_UNROLL];
+#pragma unroll
+        for (int u = 0; u < FEW_UNROLL; ++u) { const int s = s0 + u * FEW_WAVES; fb[u] = s < g.ksteps ? __builtin_nontemporal_load((const i32x4*)(b + (long)s * 64)) : i32x4{0, 0, 0, 0}; }
+#pragma unroll
+        for (int u = 0; u < FEW_UNROLL; ++u) {
+            const int s = s0 + u * FEW_WAVES;
+            if (s >= g.ksteps) break;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[u], *(const i32x4*)(a[t] + (long)s * 64), acc[t], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s_red[wave][t][r][(lane >> 4) * 4 + i] = acc[t][i];
+    __syncthreads();
+    for (int k = threadIdx.x; k < MT * 256; k += FEW_WAVES * 64) {
+        const int c = k & 15, m = k >> 4, n = n0 + c;
+        if (m >= g.m || n >= g.n) continue;
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; ++w) sum += s_red[w][m >> 4][m & 15][c];
+        float v = fmaf((float)sum * g.sa[m], g.sb[n], g.bias ? g.bias[n] : 0.f);
+        if (g.relu && v < 0.f) v = 0.f;
+        ((T*)g.y)[m * g.ldy + n] = YElem<T>::cvt(v);
+    }
+}
+
+template <typename T> static int mm8_launch(const I8Args& g, hipStream_t st)
+{
+    if (g.m <= 64) {
+        const dim3 grid((unsigned)cdiv(g.n, 16)), block(FEW_WAVES * 64);
+        if (g.m <= 16) hipLaunchKernelGGL((matmul_int8_few_kernel<T, 1>), grid, block, 0, st, g);
+        else if (g.m <= 32) hipLaunchKernelGGL((matmul_int8_few_kernel<T, 2>), grid, block, 0, st, g);
+        else hipLaunchKernelGGL((matmul_int8_few_kernel<T, 4>), grid, block, 0, st, g);
+        SAUNET_CHECK_LAUNCH("matmul_int8_few");
+        return SAUNET_OK;
+    }
+    const long t64 = ((g.m + 63) / 64) * ((g.n + 63) / 64);
+    if (t64 >= 192 * 16 && g.ksteps >= 8) return mm8_tiles<T, I8Core256>(g, st);
+    if (t64 >= 512 * 8 && g.ksteps < 8) return mm8_tiles<T, I8CoreWide>(g, st);
+    if (t64 <= 384) return mm8_tiles<T, I8Core64>(g, st);
+    if (t64 <= 768 || g.ksteps < 8) return mm8_tiles<T, I8CoreTall>(g, st);
+    return mm8_tiles<T, I8Core128>(g, st);
 }
 
 }  // namespace saunet

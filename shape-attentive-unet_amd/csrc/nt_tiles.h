@@ -2,8 +2,9 @@
 //
 // A stage holds RB bytes of every row of the tile (BM rows of A, BN rows of B).  One DMA instruction of a wave lands 1 KB lane-linear in LDS, so the
 // 16-byte XOR swizzle that spreads a fragment read over all banks is applied to the per-lane SOURCE address and again on the read: LDS row r
-// holds source chunk (slot ^ key(r)).  ST buffers form a ring; the loads of stage s + ST - 1 are requested right after the barrier that releases the
-// buffer of stage s - 1 and waited for with a counted vmcnt, so ST - 1 stages of arithmetic cover the memory latency.
+// holds source chunk (slot ^ key(r)).  ST buffers form a ring.  A stage is two half steps; the fragments of each are read while the MFMAs of the one before
+// run.  The one barrier of a stage stands between its halves, when its last fragments are in registers: behind it the buffer takes the requests of stage
+// s + ST, and stage s + 1, whose requests every wave has waited for with a counted vmcnt, is read.
 //
 // Operand rows beyond the matrix are clamped to its last row: they are read, multiplied and never stored.  The reduction length is a whole number of
 // stages; what lies behind the real end of a row is zero in memory.
@@ -32,6 +33,17 @@ __device__ __forceinline__ const char* nt_uniform(const char* p)
 template <int N> __device__ __forceinline__ void nt_wait_barrier()
 {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(N) : "memory");
+}
+
+// Workgroup id -> tile (r, c) of a rows x cols grid.  Ids go round the eight XCDs, each with an L2 of its own: XCD x takes the x-th eighth of the tiles, and
+// walks it in bands of eight tile rows, so that the tiles in flight on one L2 share both operands.
+__device__ __forceinline__ void nt_place(int id, int total, int rows, int cols, int& r, int& c)
+{
+    const int x = id & 7, q = total >> 3, rest = total & 7;
+    const int t = x * q + (x < rest ? x : rest) + (id >> 3);
+    const int band = t / (8 * cols), h = rows - band * 8 < 8 ? rows - band * 8 : 8, in = t - band * 8 * cols;
+    r = band * 8 + in % h;
+    c = in / h;
 }
 
 // float16 pairs: a row is a sequence of blocks of 32 elements, each 64 bytes of high parts followed by 64 bytes of low parts (x = hi + lo to 2^-24
@@ -66,10 +78,11 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
     static constexpr int STAGE = (BM + BN) * RB, LDS = ST * STAGE, CPR = RB / 16, RPI = 1024 / RB;
     static constexpr int QA = BM * RB / 1024 / NW, QB = BN * RB / 1024 / NW, LPW = QA + QB;
     static_assert(QA * NW * 1024 == BM * RB && QB * NW * 1024 == BN * RB, "every wave requests whole instructions of one operand");
-    static_assert((ST - 2) * LPW < 64, "vmcnt counts to 63");
+    static_assert(ST >= 2 && ST <= 4 && (ST - 1) * LPW < 64 && Op::KSUB == 2, "vmcnt counts to 63");
     typedef typename Op::Acc Acc;
 
-    static __device__ __forceinline__ int key(int row) { return CPR == 8 ? (row & 7) : ((row >> 1) & 3); }
+    // 256 bytes of LDS answer at once: 2 (4) rows of the tile beside each other, so rows that agree modulo 2 (4) have to differ in their key
+    static __device__ __forceinline__ int key(int row) { return CPR == 8 ? ((row >> 1) & 7) : ((row >> 2) & 3); }
 
     // a, b: first byte of the tile's first row at its first stage (uniform); arows, brows: rows that exist from there on (>= 1)
     static __device__ __forceinline__ void run(const char* a, unsigned lda, int arows, const char* b, unsigned ldb, int brows, int ksteps, unsigned char* smem,
@@ -97,33 +110,49 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
                 nt_dma16(q < QA ? pa : pb, voff[q], dst + (q < QA ? q * NW + wave : BM * RB / 1024 + (q - QA) * NW + wave) * 1024);
         };
         const int r0 = lane & 31, half = lane >> 5, k0 = key(r0);
-        for (int s = 0; s < ST - 1 && s < ksteps; ++s) issue(s);
-        for (int s = 0; s < ksteps; ++s) {
-            const int left = ksteps - 1 - s;                   // requested stages behind this one: min(left, ST - 2)
-            if (ST < 3 || left >= ST - 2) nt_wait_barrier<(ST - 2) * LPW>();
-            else if (ST > 3 && left == 1) nt_wait_barrier<LPW>();
-            else if (ST > 4 && left == 2) nt_wait_barrier<2 * LPW>();
-            else nt_wait_barrier<0>();
-            if (s + ST - 1 < ksteps) issue(s + ST - 1);
+        u32x4 fa[2][TM][Op::PARTS], fb[2][TN][Op::PARTS];
+        auto read = [&](int s, int ks) {
             const unsigned char* st = smem + (s % ST) * STAGE;
             const unsigned char* sa = st + (wm * (BM / WGM) + r0) * RB;
             const unsigned char* sb = st + BM * RB + (wn * (BN / WGN) + r0) * RB;
 #pragma unroll
-            for (int ks = 0; ks < Op::KSUB; ++ks) {
-                u32x4 fa[TM][Op::PARTS], fb[TN][Op::PARTS];
+            for (int p = 0; p < Op::PARTS; ++p) {
+                const int at = (Op::chunk(ks, p, half) ^ k0) * 16;
 #pragma unroll
-                for (int p = 0; p < Op::PARTS; ++p) {
-                    const int at = (Op::chunk(ks, p, half) ^ k0) * 16;
+                for (int i = 0; i < TM; ++i) fa[ks][i][p] = *(const u32x4*)(sa + i * 32 * RB + at);
 #pragma unroll
-                    for (int i = 0; i < TM; ++i) fa[i][p] = *(const u32x4*)(sa + i * 32 * RB + at);
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) fb[j][p] = *(const u32x4*)(sb + j * 32 * RB + at);
-                }
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) Op::mma(fa[i], fb[j], acc[i][j]);
+                for (int j = 0; j < TN; ++j) fb[ks][j][p] = *(const u32x4*)(sb + j * 32 * RB + at);
             }
+        };
+        auto mma = [&](int ks) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) Op::mma(fa[ks][i], fb[ks][j], acc[i][j]);
+        };
+        // this wave's LDS reads are in registers, its requests of all but the newest `young` stages have landed; then the workgroup's have
+        auto settle = [&](int young) {
+            if (young >= 3 && ST > 3) nt_wait_barrier<(ST > 3 ? 3 : 0) * LPW>();
+            else if (young == 2 && ST > 2) nt_wait_barrier<(ST > 2 ? 2 : 0) * LPW>();
+            else if (young == 1) nt_wait_barrier<LPW>();
+            else nt_wait_barrier<0>();
+        };
+        for (int s = 0; s < ST && s < ksteps; ++s) issue(s);
+        settle((ksteps < ST ? ksteps : ST) - 1);
+        read(0, 0);
+        for (int s = 0; s < ksteps; ++s) {
+            read(s, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (s + 1 < ksteps) {
+                settle(ksteps - 2 - s < ST - 2 ? ksteps - 2 - s : ST - 2);          // stage s + 1 is there; nobody reads stage s any more
+                if (s + ST < ksteps) issue(s + ST);
+                read(s + 1, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            mma(1);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
