@@ -181,7 +181,7 @@ template <typename T, class Core> __global__ __launch_bounds__(Core::NT) void ma
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     int tt, tc;
-    nt_place(blockIdx.x, gridDim.x, (int)((g.m + Core::BN - 1) / Core::BN), g.tn, tt, tc);
+    nt_band(nt_xcd(blockIdx.x, gridDim.x), (int)((g.m + Core::BN - 1) / Core::BN), g.tn, tt, tc);
     const long m0 = (long)tt * Core::BN;
     const int n0 = tc * Core::BM;
     typename Core::Acc acc[Core::TM][Core::TN] = {};

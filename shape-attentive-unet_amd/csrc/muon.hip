@@ -20,23 +20,27 @@
 
 namespace saunet {
 
-struct NsItem {            // 72 bytes: one matrix, as the host lays it out
+struct NsSplit { int p, full, s, c; };    // first workgroup, tiles done whole, parts of each of the others, first of those others in the finishing launch
+enum { NS_GRAM = 0, NS_ONE, NS_TWO, NS_KINDS };
+struct NsItem {            // one matrix, as the host lays it out
     const void* src; void* dst; float* buf; char* ws;
-    int ld_src, ld_dst, rows, cols, splits;
-    int p_norm, p_pack, p_sym, p_gram, p_app;       // index of the matrix's first workgroup in the launches of each kind
+    int ld_src, ld_dst, rows, cols;
+    int p_norm, p_pack, p_app;       // index of the matrix's first workgroup in the launches of each kind
+    NsSplit split[NS_KINDS];
 };
-constexpr int NS_CHUNK = 52;
+constexpr int NS_CHUNK = 36;                 // of them are kernel arguments
 struct NsItems { NsItem it[NS_CHUNK]; };
-constexpr int NS_TILE = 128, NS_NORM = 8192;        // elements a workgroup of the norm pass takes
+static_assert(sizeof(NsItems) <= 4064, "kernel arguments end at 4 KB");
+constexpr int NS_NORM = 8192;                // elements a workgroup of the norm pass takes
 
-enum { NS_A = 0, NS_P, NS_R, NS_Q0, NS_Q1, NS_NSYM };
+enum { NS_X = -1, NS_A = 0, NS_P, NS_R, NS_Q0, NS_Q1, NS_NSYM };
 struct NsView {
     int m, n, mp, np, tall;
     char *x, *xt[2], *sym[NS_NSYM]; float* part;
-    __host__ __device__ static long bytes(int rows, int cols, int splits)
+    static long bytes(int rows, int cols)
     {
-        const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows, mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32, t = (m + NS_TILE - 1) / NS_TILE;
-        return 3 * mp * np * 4 + NS_NSYM * mp * mp * 4 + (splits > 1 ? (long)splits * (t * (t + 1) / 2) * NS_TILE * NS_TILE * 4 : 0);
+        const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows, mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
+        return 3 * mp * np * 4 + NS_NSYM * mp * mp * 4;
     }
     __device__ explicit NsView(const NsItem& it)
     {
@@ -51,17 +55,17 @@ struct NsView {
     }
 };
 
-// the matrix whose workgroups include `id` of the launches of this kind; two rounds of one load a lane (count <= 4096)
-template <int NsItem::*P> __device__ __forceinline__ int ns_find(const NsItem* __restrict__ tab, int count, int id)
+// the matrix whose workgroups include `id`: the last whose first(i) is not above it; two rounds of one load a lane (count <= 4096)
+template <typename F> __device__ __forceinline__ int ns_find(int count, int id, F first)
 {
     const int lane = threadIdx.x & 63, step = (count + 63) >> 6;
     int base = 0;
     if (step > 1) {
         const int i = lane * step;
-        base = (__popcll(__ballot(i < count && tab[i].*P <= id)) - 1) * step;
+        base = (__popcll(__ballot(i < count && first(i < count ? i : 0) <= id)) - 1) * step;
     }
     const int i = base + lane;
-    return __builtin_amdgcn_readfirstlane(base + __popcll(__ballot(lane < step * (step > 1) + 64 * (step <= 1) && i < count && tab[i].*P <= id)) - 1);
+    return __builtin_amdgcn_readfirstlane(base + __popcll(__ballot((step == 1 || lane < step) && i < count && first(i < count ? i : 0) <= id)) - 1);
 }
 
 __global__ void ns_setup_kernel(NsItems items, int count, NsItem* __restrict__ tab)
@@ -93,7 +97,7 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_norm_
 {
     __shared__ double s_sum[4];
     const int id = blockIdx.x;
-    const NsItem it = tab[ns_find<&NsItem::p_norm>(tab, count, id)];
+    const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].p_norm; })];
     const long total = (long)it.rows * it.cols, e0 = (long)(id - it.p_norm) * NS_NORM;
     float h[5] = {0.f, 0.f, 0.f, 0.f, 1.f};
     if (MUON) for (int i = 0; i < 5; ++i) h[i] = hyper[i];
@@ -123,7 +127,7 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_
     __shared__ float s_t[64][65];
     __shared__ double s_sum[4];
     const int tid = threadIdx.x, id = blockIdx.x;
-    const NsItem it = tab[ns_find<&NsItem::p_pack>(tab, count, id)];
+    const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].p_pack; })];
     const NsView v(it);
     const int nblk = (int)(((long)it.rows * it.cols + NS_NORM - 1) / NS_NORM);
     double sum = 0.0;
@@ -168,28 +172,33 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_
 }
 
 // ---- products -----------------------------------------------------------------------------------------------------------------------
-typedef NtCore<NtF16Pair, NS_TILE, NS_TILE, 2, 2, 2> NsCore;
+// Both tiles take 64 KB of LDS, two workgroups a CU
+typedef NtCore<NtF16Pair, 128, 128, 2, 2, 2> NsCore128;
+typedef NtCore<NtF16Pair, 64, 64, 2, 2, 4> NsCore64;
+constexpr int NS_SLOTS = 512;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4_t;
 
-struct NsTile { int i0, j0; };          // the wave's corner in C
-// calls f(i, j, value[4]) for the 4 consecutive rows i .. i + 3 and the column j of every accumulator quad inside [0, mlim) x [0, nlim) (multiples of 32)
-template <typename F> __device__ __forceinline__ void ns_for_quads(f32x16 (&acc)[NsCore::TM][NsCore::TN], int i0, int j0, int mlim, int nlim, F f)
-{
-    const int lane = threadIdx.x & 63;
+// Accumulator quad b of a thread: the four rows i .. i + 3 of column j, relative to the tile
+template <class Core> struct NsQuads {
+    static constexpr int N = Core::TM * Core::TN * 4, FLOATS = Core::BM * Core::BN;
+    static __device__ __forceinline__ void at(int b, int& i, int& j)
+    {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ti = b / (4 * Core::TN), tj = b / 4 % Core::TN, g = b & 3;
+        i = (wave / Core::WGN) * (Core::BM / Core::WGM) + ti * 32 + g * 8 + (lane >> 5) * 4;
+        j = (wave % Core::WGN) * (Core::BN / Core::WGN) + tj * 32 + (lane & 31);
+    }
+    template <typename F> static __device__ __forceinline__ void each(f32x16 (&acc)[Core::TM][Core::TN], F f)
+    {
 #pragma unroll
-    for (int ti = 0; ti < NsCore::TM; ++ti)
-#pragma unroll
-        for (int tj = 0; tj < NsCore::TN; ++tj) {
-            if (i0 + ti * 32 >= mlim || j0 + tj * 32 >= nlim) continue;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                float q[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) q[r] = acc[ti][tj][g * 4 + r];
-                f(i0 + ti * 32 + g * 8 + (lane >> 5) * 4, j0 + tj * 32 + (lane & 31), q);
-            }
+        for (int b = 0; b < N; ++b) {
+            int i, j;
+            at(b, i, j);
+            const f32x16& c = acc[b / (4 * Core::TN)][b / 4 % Core::TN];
+            const float q[4] = {c[(b & 3) * 4], c[(b & 3) * 4 + 1], c[(b & 3) * 4 + 2], c[(b & 3) * 4 + 3]};
+            f(b, i, j, q);
         }
-}
+    }
+};
 // four consecutive elements (row j, columns i .. i + 3) of a pair matrix with lda bytes a row
 __device__ __forceinline__ void ns_read4(const char* p, long ldb, int j, int i, float (&v)[4])
 {
@@ -235,113 +244,107 @@ __device__ __forceinline__ void ns_lower(int t, int& ti, int& tj)
     tj = t - ti * (ti + 1) / 2;
 }
 
-// S = X X^T: lower tiles, the columns in it.splits parts.  One part: straight to S.  More: float32 partials in accumulator order for ns_gram_finish.
-__global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsItem* __restrict__ tab, int count, float alpha)
-{
-    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-    const int id = blockIdx.x;
-    const NsItem it = tab[ns_find<&NsItem::p_gram>(tab, count, id)];
-    const NsView v(it);
-    const int t = (id - it.p_gram) / it.splits, sp = (id - it.p_gram) % it.splits;
-    int ti, tj;
-    ns_lower(t, ti, tj);
-    const int steps = v.np / 32, k0 = (int)((long)steps * sp / it.splits), k1 = (int)((long)steps * (sp + 1) / it.splits);
-    f32x16 acc[NsCore::TM][NsCore::TN] = {};
-    const long ld = (long)v.np * 4;
-    NsCore::run(v.x + ti * NS_TILE * ld + k0 * 128, (unsigned)ld, v.mp - ti * NS_TILE, v.x + tj * NS_TILE * ld + k0 * 128, (unsigned)ld, v.mp - tj * NS_TILE, k1 - k0, smem, acc);
-    const int wave = threadIdx.x >> 6, i0 = ti * NS_TILE + (wave >> 1) * 64, j0 = tj * NS_TILE + (wave & 1) * 64;
-    if (it.splits > 1) {
-        float* p = v.part + ((long)t * it.splits + sp) * NS_TILE * NS_TILE + threadIdx.x * 4;
-#pragma unroll
-        for (int b = 0; b < 16; ++b) *(f32x4*)(p + b * 1024) = f32x4{acc[b >> 3][(b >> 2) & 1][(b & 3) * 4], acc[b >> 3][(b >> 2) & 1][(b & 3) * 4 + 1], acc[b >> 3][(b >> 2) & 1][(b & 3) * 4 + 2], acc[b >> 3][(b >> 2) & 1][(b & 3) * 4 + 3]};
-        return;
-    }
-    char* s = v.sym[NS_A];
-    ns_for_quads(acc, i0, j0, v.mp, v.mp, [&](int i, int j, const float (&q)[4]) {
-        const float w[4] = {alpha * q[0], alpha * q[1], alpha * q[2], alpha * q[3]};
-        ns_write4_sym(s, v.mp * 4L, ti == tj, i, j, w);
-    });
-}
-__global__ __launch_bounds__(256) void ns_gram_finish_kernel(const NsItem* __restrict__ tab, int count, float alpha)
-{
-    const int id = blockIdx.x;
-    const NsItem it = tab[ns_find<&NsItem::p_sym>(tab, count, id)];
-    if (it.splits < 2) return;
-    const NsView v(it);
-    const int t = id - it.p_sym;
-    int ti, tj;
-    ns_lower(t, ti, tj);
-    f32x16 acc[NsCore::TM][NsCore::TN] = {};
-    const float* p = v.part + (long)t * it.splits * NS_TILE * NS_TILE + threadIdx.x * 4;
-    for (int sp = 0; sp < it.splits; ++sp, p += NS_TILE * NS_TILE)
-#pragma unroll
-        for (int b = 0; b < 16; ++b) {
-            const f32x4 w = *(const f32x4*)(p + b * 1024);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[b >> 3][(b >> 2) & 1][(b & 3) * 4 + r] += w[r];
-        }
-    const int wave = threadIdx.x >> 6, i0 = ti * NS_TILE + (wave >> 1) * 64, j0 = tj * NS_TILE + (wave & 1) * 64;
-    char* s = v.sym[NS_A];
-    ns_for_quads(acc, i0, j0, v.mp, v.mp, [&](int i, int j, const float (&q)[4]) {
-        const float w[4] = {alpha * q[0], alpha * q[1], alpha * q[2], alpha * q[3]};
-        ns_write4_sym(s, v.mp * 4L, ti == tj, i, j, w);
-    });
-}
-
-// D = alpha A B + beta E + gamma F over symmetric matrices that commute (so D is symmetric): lower tiles, both halves written.  blockIdx.y picks the
-// product: the two of one phase are independent.
+// D = alpha A B^T (+ beta E + gamma F) for a symmetric D -- X X^T, or a product of symmetric matrices that commute: lower tiles, both halves
+// written.  blockIdx.y picks the product: the two of one phase are independent.  The tiles behind the first split.full are cut along the reduction into
+// split.s parts, whose float32 sums go to memory in accumulator order for ns_finish_kernel.
 struct NsProd { int a, b, e, f, d; float alpha, beta, gamma; };
 struct NsProds { NsProd p[2]; };
-__global__ __launch_bounds__(256, 2) void ns_sym_kernel(const NsItem* __restrict__ tab, int count, NsProds pr)
+
+__device__ __forceinline__ void ns_prod_store(const NsView& v, const NsProd& p, int ti, int tj, int i, int j, const float (&q)[4])
+{
+    if (i >= v.mp || j >= v.mp) return;                                    // whole 32 x 32 blocks
+    const long ld = (long)v.mp * 4;
+    float w[4], x[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) w[r] = p.alpha * q[r];
+    if (p.e >= 0) {
+        ns_read4(v.sym[p.e], ld, j, i, x);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] = fmaf(p.beta, x[r], w[r]);
+    }
+    if (p.f >= 0) {
+        ns_read4(v.sym[p.f], ld, j, i, x);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] = fmaf(p.gamma, x[r], w[r]);
+    }
+    ns_write4_sym(v.sym[p.d], ld, ti == tj, i, j, w);
+}
+
+template <class Core> __global__ __launch_bounds__(256, 2) void ns_prod_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+    constexpr int T = Core::BM;
     const int id = blockIdx.x;
     const NsProd p = pr.p[blockIdx.y];
-    const NsItem it = tab[ns_find<&NsItem::p_sym>(tab, count, id)];
+    const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].split[kind].p; })];
     const NsView v(it);
-    int ti, tj;
-    ns_lower(id - it.p_sym, ti, tj);
-    f32x16 acc[NsCore::TM][NsCore::TN] = {};
-    const long ld = (long)v.mp * 4;
-    NsCore::run(v.sym[p.a] + ti * NS_TILE * ld, (unsigned)ld, v.mp - ti * NS_TILE, v.sym[p.b] + tj * NS_TILE * ld, (unsigned)ld, v.mp - tj * NS_TILE, v.mp / 32, smem, acc);
-    const int wave = threadIdx.x >> 6, i0 = ti * NS_TILE + (wave >> 1) * 64, j0 = tj * NS_TILE + (wave & 1) * 64;
-    const char* e = v.sym[p.e];
-    const char* f = p.f < 0 ? nullptr : v.sym[p.f];
-    char* d = v.sym[p.d];
-    ns_for_quads(acc, i0, j0, v.mp, v.mp, [&](int i, int j, const float (&q)[4]) {
-        float w[4], x[4];
-        ns_read4(e, ld, j, i, x);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) w[r] = fmaf(p.alpha, q[r], p.beta * x[r]);
-        if (f) {
-            ns_read4(f, ld, j, i, x);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) w[r] = fmaf(p.gamma, x[r], w[r]);
-        }
-        ns_write4_sym(d, ld, ti == tj, i, j, w);
-    });
+    const NsSplit sl = it.split[kind];
+    int t = id - sl.p, sp = 0, parts = 1, ti, tj;
+    if (count == 1 && t < sl.full) t = nt_xcd(t, sl.full);                 // (a list is dealt out tile by tile: its tiles differ in cost)
+    if (t >= sl.full) { sp = (t - sl.full) % sl.s; t = sl.full + (t - sl.full) / sl.s; parts = sl.s; }
+    ns_lower(t, ti, tj);
+    const int steps = (p.a == NS_X ? v.np : v.mp) / 32, k0 = (int)((long)steps * sp / parts), k1 = (int)((long)steps * (sp + 1) / parts);
+    const long ld = steps * 128L;
+    const char* a = (p.a == NS_X ? v.x : v.sym[p.a]) + k0 * 128L;
+    const char* b = (p.a == NS_X ? v.x : v.sym[p.b]) + k0 * 128L;
+    f32x16 acc[Core::TM][Core::TN] = {};
+    Core::run(a + ti * T * ld, (unsigned)ld, v.mp - ti * T, b + tj * T * ld, (unsigned)ld, v.mp - tj * T, k1 - k0, smem, acc);
+    if (parts > 1) {
+        const int nt = (v.mp + T - 1) / T, cut = nt * (nt + 1) / 2 - sl.full;
+        float* d = v.part + (((long)blockIdx.y * cut + t - sl.full) * parts + sp) * NsQuads<Core>::FLOATS + threadIdx.x * 4;
+        NsQuads<Core>::each(acc, [&](int q, int, int, const float (&c)[4]) { *(f32x4*)(d + q * 1024) = f32x4{c[0], c[1], c[2], c[3]}; });
+        return;
+    }
+    NsQuads<Core>::each(acc, [&](int, int i, int j, const float (&c)[4]) { ns_prod_store(v, p, ti, tj, ti * T + i, tj * T + j, c); });
+}
+// one accumulator quad of a cut tile a thread; blockIdx.x = tile * quads + quad
+template <class Core> __global__ __launch_bounds__(256) void ns_finish_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr)
+{
+    constexpr int T = Core::BM, N = NsQuads<Core>::N;
+    const int id = blockIdx.x / N, q = blockIdx.x % N;
+    const NsProd p = pr.p[blockIdx.y];
+    const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].split[kind].c; })];
+    const NsSplit sl = it.split[kind];
+    const int t = sl.full + id - sl.c;
+    const NsView v(it);
+    int ti, tj, i, j;
+    ns_lower(t, ti, tj);
+    NsQuads<Core>::at(q, i, j);
+    const int nt = (v.mp + T - 1) / T, cut = nt * (nt + 1) / 2 - sl.full;
+    const float* s = v.part + (((long)blockIdx.y * cut + t - sl.full) * sl.s) * NsQuads<Core>::FLOATS + q * 1024 + threadIdx.x * 4;
+    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int sp = 0; sp < sl.s; ++sp) { const f32x4 w = *(const f32x4*)(s + (long)sp * NsQuads<Core>::FLOATS); for (int r = 0; r < 4; ++r) c[r] += w[r]; }
+    const float w[4] = {c[0], c[1], c[2], c[3]};
+    ns_prod_store(v, p, ti, tj, ti * T + i, tj * T + j, w);
+}
+
+__device__ __forceinline__ void ns_rates(const float* hyper, int rows, int cols, int adjust, float& keep, float& rate)
+{
+    const float lr = hyper[0];
+    keep = 1.f - lr * hyper[2];
+    rate = lr * (adjust ? 0.2f * sqrtf((float)(rows > cols ? rows : cols)) : rows > cols ? sqrtf((float)rows / (float)cols) : 1.f);
 }
 
 // X <- alpha Q X + beta X.  MODE 0: back to X and the other X^T; 1: to the caller's matrix; 2: the Muon update of the caller's parameter
-template <typename T, int MODE> __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsItem* __restrict__ tab, int count, int q, int xt, float alpha, float beta, const float* __restrict__ hyper, int adjust)
+template <class Core, typename T, int MODE> __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsItem* __restrict__ tab, int count, int q, int xt, float alpha, float beta, const float* __restrict__ hyper, int adjust)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-    const int id = blockIdx.x;
-    const NsItem it = tab[ns_find<&NsItem::p_app>(tab, count, id)];
+    constexpr int B = Core::BM;
+    const int id = count == 1 ? nt_xcd(blockIdx.x, gridDim.x) : blockIdx.x;
+    const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].p_app; })];
     const NsView v(it);
-    const int tm = (v.mp + NS_TILE - 1) / NS_TILE, t = id - it.p_app, ti = t % tm, tj = t / tm;
-    f32x16 acc[NsCore::TM][NsCore::TN] = {};
+    int ti, tj;
+    nt_band(id - it.p_app, (v.np + B - 1) / B, (v.mp + B - 1) / B, tj, ti);
+    f32x16 acc[Core::TM][Core::TN] = {};
     const long ld = (long)v.mp * 4;
-    NsCore::run(v.sym[q] + ti * NS_TILE * ld, (unsigned)ld, v.mp - ti * NS_TILE, v.xt[xt] + tj * NS_TILE * ld, (unsigned)ld, v.np - tj * NS_TILE, v.mp / 32, smem, acc);
-    const int wave = threadIdx.x >> 6, i0 = ti * NS_TILE + (wave >> 1) * 64, j0 = tj * NS_TILE + (wave & 1) * 64;
+    Core::run(v.sym[q] + ti * B * ld, (unsigned)ld, v.mp - ti * B, v.xt[xt] + tj * B * ld, (unsigned)ld, v.np - tj * B, v.mp / 32, smem, acc);
     const char* x = v.xt[xt];
     float keep = 0.f, rate = 0.f;
-    if (MODE == 2) {
-        const float lr = hyper[0], big = (float)(it.rows > it.cols ? it.rows : it.cols);
-        keep = 1.f - lr * hyper[2];
-        rate = lr * (adjust ? 0.2f * sqrtf(big) : it.rows > it.cols ? sqrtf((float)it.rows / (float)it.cols) : 1.f);
-    }
-    ns_for_quads(acc, i0, j0, v.mp, v.np, [&](int i, int j, const float (&a)[4]) {
+    if (MODE == 2) ns_rates(hyper, it.rows, it.cols, adjust, keep, rate);
+    NsQuads<Core>::each(acc, [&](int, int i, int j, const float (&a)[4]) {
+        i += ti * B; j += tj * B;
+        if (i >= v.mp || j >= v.np) return;                                // whole 32 x 32 blocks
         float w[4], o[4];
         ns_read4(x, ld, j, i, o);
 #pragma unroll
@@ -359,15 +362,189 @@ template <typename T, int MODE> __global__ __launch_bounds__(256, 2) void ns_app
     });
 }
 
-// ---- host side --------------------------------------------------------------------------------------------------------------------------------
-struct NsPlan { long norm, pack, sym, gram, app, tab_bytes, part_bytes, bytes, shortest; bool split; };
+// ---- short matrices: up to 32 rows (or columns), three launches -----------------------------------------------------------------------------
+// The iteration is W(S) X0 with one polynomial W of S = X0 X0^T.  With 32 rows S is so small that it can be kept in FLOAT64, where composing ALL steps is
+// sound (an error grows by a^2 = 12 a step from 2^-53): one pass over the matrix for S, whose trace is the norm, one workgroup for W, one pass
+// for W X0.  The float64 rate of the vector units equals the float32 one, and both passes move little else than the matrix.
+constexpr int NSS_COLS = 64;                   // columns of the long side a workgroup stages at once
+struct NssItem { const void* src; void* dst; float* buf; double* ws; int ld_src, ld_dst, rows, cols, p, tiles; };       // tiles: of NSS_COLS, a workgroup
+constexpr int NSS_CHUNK = 64;
+struct NssItems { NssItem it[NSS_CHUNK]; };
+static_assert(sizeof(NssItems) <= 4032, "kernel arguments end at 4 KB");
 
+// columns c0 .. c0 + 63 of the matrix (long side) into s[32][68], zeros outside
+template <typename T, bool MUON, bool STORE> __device__ __forceinline__ void nss_stage(const NssItem& it, int c0, const float* __restrict__ hyper, float (*s)[68])
+{
+    const bool tall = it.rows > it.cols;
+    const int m = tall ? it.cols : it.rows, n = tall ? it.rows : it.cols;
+    float h[5] = {0.f, 0.f, 0.f, 0.f, 1.f};
+    if (MUON) for (int i = 0; i < 5; ++i) h[i] = hyper[i];
+#pragma unroll
+    for (int q = 0; q < 32 * NSS_COLS / 256; ++q) {
+        const int k = threadIdx.x + q * 256, i = tall ? k & 31 : k >> 6, c = tall ? k >> 5 : k & 63, j = c0 + c;
+        float u = 0.f;
+        if (i < m && j < n) {
+            const long r = tall ? j : i, e = tall ? i : j;
+            u = ns_load((const T*)it.src + r * it.ld_src + e);
+            if (MUON) {
+                float* b = it.buf + r * it.cols + e;
+                float o = *b;
+                if (STORE) { o = ns_momentum(u, o, h); *b = o; }
+                u = ns_update(u, o, h);
+            }
+        }
+        s[i][c] = u;
+    }
+}
+template <typename T, bool MUON> __global__ __launch_bounds__(256) void nss_gram_kernel(NssItems items, int count, const float* __restrict__ hyper)
+{
+    __shared__ __attribute__((aligned(16))) float s_x[32][68];
+    __shared__ double s_g[4][32][33];
+    const int id = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, a0 = (tid >> 3 & 7) * 4, b0 = (tid & 7) * 4;
+    const NssItem it = items.it[ns_find(count, id, [&](int i) { return items.it[i].p; })];
+    double acc[4][4] = {};
+    const int n = it.rows > it.cols ? it.rows : it.cols, first = (id - it.p) * it.tiles;
+    for (int t = 0; t < it.tiles && (first + t) * NSS_COLS < n; ++t) {
+        if (t) __syncthreads();
+        nss_stage<T, MUON, true>(it, (first + t) * NSS_COLS, hyper, s_x);
+        __syncthreads();
+        // a wave: 16 of the columns, a thread 4 x 4 of the sums
+#pragma unroll 2
+        for (int k = wave * 16; k < wave * 16 + 16; k += 4) {
+            f32x4 a[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { a[i] = *(const f32x4*)&s_x[a0 + i][k]; b[i] = *(const f32x4*)&s_x[b0 + i][k]; }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = fma((double)a[i][e], (double)b[j][e], acc[i][j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s_g[wave][a0 + i][b0 + j] = acc[i][j];
+    __syncthreads();
+    double* g = it.ws + (long)(1 + id - it.p) * 1024;
+    for (int k = tid; k < 1024; k += 256) g[k] = (s_g[0][k >> 5][k & 31] + s_g[1][k >> 5][k & 31]) + (s_g[2][k >> 5][k & 31] + s_g[3][k >> 5][k & 31]);
+}
+
+typedef __attribute__((ext_vector_type(4))) double f64x4;
+typedef double NssMat[32][36];          // rows 32 bytes apart in the banks
+// quadrant `quad` of A B for symmetric A, B: element r of lane l is (row l / 16 + 4 r, column l % 16) of it
+__device__ __forceinline__ f64x4 nss_product(const NssMat& a, const NssMat& b, int quad)
+{
+    const int lane = threadIdx.x & 63, i = (quad >> 1) * 16 + (lane & 15), j = (quad & 1) * 16 + (lane & 15), k = lane >> 4;
+    f64x4 c = {0.0, 0.0, 0.0, 0.0}, d = c;                                 // two chains: the MFMAs of one wait for each other
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        c = __builtin_amdgcn_mfma_f64_16x16x4f64(a[i][s * 4 + k], b[j][s * 4 + k], c, 0, 0, 0);
+        d = __builtin_amdgcn_mfma_f64_16x16x4f64(a[i][16 + s * 4 + k], b[j][16 + s * 4 + k], d, 0, 0, 0);
+    }
+    return c + d;
+}
+// W / norm from the sums of nss_gram_kernel: a workgroup a matrix, waves 0 - 3 and 4 - 7 a product each.  S' = (a I + P)^2 S, W' = (a I + P) W.
+__global__ __launch_bounds__(512) void nss_poly_kernel(NssItems items, int steps, double a, double b, double c, float eps)
+{
+    __shared__ NssMat S, P, R, W;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = wave & 3;
+    const NssItem it = items.it[blockIdx.x];
+    const int n = it.rows > it.cols ? it.rows : it.cols, parts = (n + it.tiles * NSS_COLS - 1) / (it.tiles * NSS_COLS);
+    for (int k = tid; k < 1024; k += 512) {
+        double sum = 0.0;
+#pragma unroll 8
+        for (int p = 0; p < parts; ++p) sum += it.ws[(long)(1 + p) * 1024 + k];
+        S[k >> 5][k & 31] = sum;
+    }
+    __syncthreads();
+    double trace = 0.0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) trace += S[i][i];
+    double norm = sqrt(trace);
+    if (norm <= (double)eps) norm = (double)eps;                          // a NaN norm stays NaN
+    const double inv = 1.0 / (norm * norm);
+    __syncthreads();
+    for (int k = tid; k < 1024; k += 512) { S[k >> 5][k & 31] *= inv; W[k >> 5][k & 31] = (k >> 5) == (k & 31) ? 1.0 / norm : 0.0; }
+    __syncthreads();
+    const int j = (quad & 1) * 16 + (lane & 15), i0 = (quad >> 1) * 16 + (lane >> 4);
+    for (int st = 0; st < steps; ++st) {
+        f64x4 x = {0.0, 0.0, 0.0, 0.0};
+        if (wave < 4) {
+            x = nss_product(S, S, quad);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) P[i0 + 4 * r][j] = b * S[i0 + 4 * r][j] + c * x[r] + (i0 + 4 * r == j ? a : 0.0);      // a I + b S + c S^2
+        }
+        __syncthreads();
+        x = wave < 4 ? nss_product(P, S, quad) : nss_product(P, W, quad);
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) (wave < 4 ? R : W)[i0 + 4 * r][j] = x[r];
+        __syncthreads();
+        if (wave < 4 && st + 1 < steps) {
+            x = nss_product(R, P, quad);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[i0 + 4 * r][j] = x[r];
+        }
+        __syncthreads();
+    }
+    for (int k = tid; k < 1024; k += 512) it.ws[k] = W[k >> 5][k & 31];
+}
+template <typename T, bool MUON> __global__ __launch_bounds__(256) void nss_apply_kernel(NssItems items, int count, const float* __restrict__ hyper, int adjust)
+{
+    __shared__ __attribute__((aligned(16))) float s_x[32][68];
+    __shared__ __attribute__((aligned(16))) double s_w[32][34];
+    const int id = blockIdx.x, tid = threadIdx.x;
+    const NssItem it = items.it[ns_find(count, id, [&](int i) { return items.it[i].p; })];
+    for (int k = tid; k < 1024; k += 256) s_w[k >> 5][k & 31] = it.ws[k];
+    const bool tall = it.rows > it.cols;
+    const int m = tall ? it.cols : it.rows, n = tall ? it.rows : it.cols, first = (id - it.p) * it.tiles;
+    float keep = 0.f, rate = 0.f;
+    if (MUON) ns_rates(hyper, it.rows, it.cols, adjust, keep, rate);
+    // a thread: 2 rows x 4 columns; lanes run along the caller's contiguous side
+    const int i0 = (tall ? tid & 15 : tid >> 4) * 2, c0 = (tall ? tid >> 4 : tid & 15) * 4;
+    for (int t = 0; t < it.tiles && (first + t) * NSS_COLS < n; ++t) {
+        __syncthreads();
+        const int base = (first + t) * NSS_COLS;
+        nss_stage<T, MUON, false>(it, base, hyper, s_x);
+        __syncthreads();
+        T old[2][4];
+        auto at = [&](int i, int j) { return (T*)it.dst + (tall ? (long)(base + c0 + j) * it.ld_dst + i0 + i : (long)(i0 + i) * it.ld_dst + base + c0 + j); };
+        if (MUON)                                                          // on its way while the sums are formed
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) old[i][j] = i0 + i < m && base + c0 + j < n ? *at(i, j) : T(0);
+        double acc[2][4] = {};
+#pragma unroll 8
+        for (int k = 0; k < 32; ++k) {
+            const f32x4 x = *(const f32x4*)&s_x[k][c0];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const double w = s_w[k][i0 + i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = fma(w, (double)x[j], acc[i][j]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (i0 + i >= m || base + c0 + j >= n) continue;
+                if (MUON) *at(i, j) = (T)fmaf(-rate, (float)acc[i][j], keep * (float)old[i][j]);
+                else ns_store(at(i, j), (float)acc[i][j]);
+            }
+    }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------------------------------
 static int ns_check(const saunet_ns_desc* d, const char* who)
 {
     if (!d || !d->item || d->count < 1 || d->count > 4096) return set_error(SAUNET_BAD_SHAPE, "%s: 1 to 4096 matrices, not %d", who, d ? d->count : 0);
     if (d->dtype != SAUNET_F32 && d->dtype != SAUNET_BF16 && d->dtype != SAUNET_F16) return set_error(SAUNET_BAD_DTYPE, "%s: dtype %d", who, d->dtype);
     if (d->steps < 1 || d->steps > 32) return set_error(SAUNET_BAD_SHAPE, "%s: 1 to 32 steps, not %d", who, d->steps);
-    if (!(d->eps > 0.f)) return set_error(SAUNET_BAD_SHAPE, "%s: eps has to be positive", who);
+    if (!(d->eps > 0.f) || !(fabsf(d->a) <= 4096.f) || !(fabsf(d->b) <= 4096.f) || !(fabsf(d->c) <= 4096.f)) return set_error(SAUNET_BAD_SHAPE, "%s: eps has to be positive, the coefficients finite and below 4096", who);
     for (int i = 0; i < d->count; ++i) {
         const saunet_ns_item& t = d->item[i];
         if (t.rows < 1 || t.cols < 1 || t.rows > (1 << 20) || t.cols > (1 << 20) || (t.rows > 32768 && t.cols > 32768))
@@ -377,154 +554,249 @@ static int ns_check(const saunet_ns_desc* d, const char* who)
     return SAUNET_OK;
 }
 
-// tile counts, prefixes (into `out` when given) and the workspace: table | norm partials | matrices
-static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* out, char* ws)
+// One call: the matrices with up to 32 rows go one way, the others the other way
+struct NsPlan { long small, large, norm, pack, tile, app, grid[NS_KINDS], cut[NS_KINDS], tab_at, part_at, bytes, shortest; int tile_m, tile_n; };
+
+static bool ns_is_small(const saunet_ns_desc* d, const saunet_ns_item& t)
 {
-    p = NsPlan();
-    for (int i = 0; i < d->count; ++i) {
-        const saunet_ns_item& t = d->item[i];
-        const long m = t.rows < t.cols ? t.rows : t.cols, n = t.rows < t.cols ? t.cols : t.rows;
-        const long tm = (m + NS_TILE - 1) / NS_TILE;
-        p.sym += tm * (tm + 1) / 2;
-        p.norm += (m * n + NS_NORM - 1) / NS_NORM;
-        if (i == 0 || m < p.shortest) p.shortest = m;
-    }
-    p.tab_bytes = ((long)sizeof(NsItem) * d->count + 255) / 256 * 256;
-    p.part_bytes = (p.norm * 8 + 255) / 256 * 256;
-    // a Gram tile walks the whole long side: it is split until the launch has about 1024 workgroups, each part 512 columns at least
-    const long want = p.sym < 1024 ? 1024 / p.sym : 1;
-    long at = p.tab_bytes + p.part_bytes;
-    long norm = 0, sym = 0;
-    for (int i = 0; i < d->count; ++i) {
-        const saunet_ns_item& t = d->item[i];
-        const long m = t.rows < t.cols ? t.rows : t.cols, n = t.rows < t.cols ? t.cols : t.rows;
-        const long tm = (m + NS_TILE - 1) / NS_TILE, tn = (n + NS_TILE - 1) / NS_TILE, mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
-        long splits = np / 512 < want ? np / 512 : want;
-        if (splits < 1) splits = 1;
-        if (splits > 1) p.split = true;
-        if (out) {
-            NsItem& o = out[i];
-            o.src = t.src; o.dst = t.dst; o.buf = (float*)t.buf; o.ws = ws + at;
-            o.ld_src = (int)t.ld_src; o.ld_dst = (int)t.ld_dst; o.rows = t.rows; o.cols = t.cols; o.splits = (int)splits;
-            o.p_norm = (int)norm; o.p_pack = (int)p.pack; o.p_sym = (int)sym; o.p_gram = (int)p.gram; o.p_app = (int)p.app;
+    // all steps composed in float64: 2^-53 a^(2 (steps - 1)) has to stay below float32's rounding
+    double grow = 1.0;
+    for (int i = 1; i < d->steps; ++i) grow *= (double)d->a * d->a;
+    return (t.rows < t.cols ? t.rows : t.cols) <= 32 && grow <= 1e8;
+}
+// Cuts along the reduction, for one kind of launch (ny products a tile, steps(i) reduction steps of matrix i).  A launch that fills less than half of
+// the NS_SLOTS workgroups that run at once is cut until it fills them, eight steps a part and four parts at least (six 1000 x 1024 matrices in two
+// parts: 41 -> 33 us and 14 for the finishing launch); one of a few rounds whose last round is less than half full has that round's tiles cut.  4096 x 4096: 528 tiles on 512
+// slots were 262 us, with sixteen of them cut sixteen-fold 170 us.
+static void ns_cut(int kind, int ny, NsPlan& p, const int* tiles, const int* steps, int count, NsItem* out)
+{
+    long total = 0, at = 0;
+    int longest = 1;
+    for (int i = 0; i < count; ++i) { total += (long)tiles[i] * ny; if (steps[i] > longest) longest = steps[i]; }
+    int part = longest;                          // steps a part
+    long tail = 0, tail_s = 1;
+    if (total <= NS_SLOTS / 2) {
+        int lo = 8, hi = longest;
+        while (lo < hi) {                        // the smallest part for which the launch still fits
+            const int mid = (lo + hi) / 2;
+            long w = 0;
+            for (int i = 0; i < count; ++i) w += (long)tiles[i] * ny * ((steps[i] + mid - 1) / mid);
+            if (w <= NS_SLOTS) hi = mid; else lo = mid + 1;
         }
-        norm += (m * n + NS_NORM - 1) / NS_NORM;
-        sym += tm * (tm + 1) / 2;
-        p.pack += ((mp + 63) / 64) * ((np + 63) / 64);
-        p.gram += tm * (tm + 1) / 2 * splits;
-        p.app += tm * tn;
-        at += (NsView::bytes(t.rows, t.cols, (int)splits) + 255) / 256 * 256;
+        part = lo;
+        if (part > longest / 4) part = longest;
+    } else if (total > NS_SLOTS && total < 4 * NS_SLOTS && total % NS_SLOTS && total % NS_SLOTS <= NS_SLOTS / 2) {
+        tail = (total % NS_SLOTS + ny - 1) / ny;
+        if (tail > tiles[count - 1]) tail = 0;
+        else { tail_s = NS_SLOTS / (tail * ny); if (tail_s > steps[count - 1] / 8) tail_s = steps[count - 1] / 8; if (tail_s < 2) { tail = 0; tail_s = 1; } }
     }
-    p.bytes = at;
-    if (p.norm > 0x7fffffff || p.pack > 0x7fffffff || p.gram > 0x7fffffff || p.app > 0x7fffffff || p.sym > 0x7fffffff) return set_error(SAUNET_BAD_SHAPE, "newton_schulz: the list is too large for one call");
+    p.cut[kind] = 0;
+    for (int i = 0; i < count; ++i) {
+        NsSplit s = {(int)at, tiles[i], 1, (int)p.cut[kind]};
+        if (i == count - 1 && tail) { s.full = tiles[i] - (int)tail; s.s = (int)tail_s; }
+        else if (steps[i] > part) { s.full = 0; s.s = (steps[i] + part - 1) / part; }
+        p.cut[kind] += tiles[i] - s.full;
+        at += s.full + (long)(tiles[i] - s.full) * s.s;
+        out[i].split[kind] = s;
+    }
+    p.grid[kind] = at;
+}
+
+// `large` and `small`: the items of either way (capacity 4096), laid out against workspace `ws`.  Workspace: table | norm partials | matrices
+static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* small, char* ws)
+{
+    static thread_local int tiles[4096], gram[4096], sym[4096];
+    p = NsPlan();
+    long t128 = 0, a128 = 0;
+    for (int i = 0; i < d->count; ++i) {
+        const saunet_ns_item& t = d->item[i];
+        const long m = t.rows < t.cols ? t.rows : t.cols, n = t.rows < t.cols ? t.cols : t.rows;
+        if (ns_is_small(d, t)) {
+            NssItem& o = small[p.small++];
+            o.src = t.src; o.dst = t.dst; o.buf = (float*)t.buf; o.ld_src = (int)t.ld_src; o.ld_dst = (int)t.ld_dst; o.rows = t.rows; o.cols = t.cols;
+            const long cols = (n + NSS_COLS - 1) / NSS_COLS;
+            o.tiles = (int)((cols + 63) / 64);                  // 64 workgroups a matrix at most: their sums are added by one
+            o.p = (int)((cols + o.tiles - 1) / o.tiles);        // (a count for now)
+            continue;
+        }
+        NsItem& o = large[p.large++];
+        o.src = t.src; o.dst = t.dst; o.buf = (float*)t.buf; o.ld_src = (int)t.ld_src; o.ld_dst = (int)t.ld_dst; o.rows = t.rows; o.cols = t.cols;
+        t128 += (m + 127) / 128 * ((m + 127) / 128 + 1) / 2;
+        a128 += (m + 127) / 128 * ((n + 127) / 128);
+        if (p.large == 1 || m < p.shortest) p.shortest = m;
+    }
+    p.tile_m = ab_env_int("SAUNET_NS_TILE", t128 <= 128 ? 64 : 128);
+    p.tile_n = ab_env_int("SAUNET_NS_ATILE", a128 <= 128 ? 64 : 128);
+    for (long i = 0; i < p.large; ++i) {
+        NsItem& o = large[i];
+        const long m = o.rows < o.cols ? o.rows : o.cols, n = o.rows < o.cols ? o.cols : o.rows, mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
+        const long tm = (m + p.tile_m - 1) / p.tile_m;
+        o.p_norm = (int)p.norm; o.p_pack = (int)p.pack; o.p_app = (int)p.app;
+        tiles[i] = (int)(tm * (tm + 1) / 2); gram[i] = (int)(np / 32); sym[i] = (int)(mp / 32);
+        p.norm += (m * n + NS_NORM - 1) / NS_NORM;
+        p.pack += ((mp + 63) / 64) * ((np + 63) / 64);
+        p.app += ((m + p.tile_n - 1) / p.tile_n) * ((n + p.tile_n - 1) / p.tile_n);
+        p.tile += tiles[i];
+        if (p.norm > 0x3fffffff || p.pack > 0x3fffffff || p.app > 0x3fffffff || p.tile > 0x3ffffff) return set_error(SAUNET_BAD_SHAPE, "newton_schulz: the list is too large for one call");
+    }
+    if (p.large) {
+        ns_cut(NS_GRAM, 1, p, tiles, gram, (int)p.large, large);
+        ns_cut(NS_ONE, 1, p, tiles, sym, (int)p.large, large);
+        ns_cut(NS_TWO, 2, p, tiles, sym, (int)p.large, large);
+    }
+    long at = 0;
+    auto take = [&](long bytes) { const long r = at; at += (bytes + 255) / 256 * 256; return r; };
+    p.tab_at = take((long)sizeof(NsItem) * p.large);
+    p.part_at = take(p.norm * 8);
+    for (long i = 0; i < p.large; ++i) {
+        long cut = 0;
+        for (int k = 0; k < NS_KINDS; ++k) {
+            const NsSplit& s = large[i].split[k];
+            const long c = s.s > 1 ? (long)(tiles[i] - s.full) * s.s * (k == NS_TWO ? 2 : 1) : 0;
+            if (c > cut) cut = c;
+        }
+        large[i].ws = ws + take(NsView::bytes(large[i].rows, large[i].cols) + cut * p.tile_m * p.tile_m * 4);
+    }
+    for (long i = 0; i < p.small; ++i) small[i].ws = (double*)(ws + take((long)(small[i].p + 1) * 1024 * 8));
+    p.bytes = at + 256;
     return SAUNET_OK;
 }
 
 // Largest magnitude that a matrix with eigenvalue f(s), s in [0, 1] the first singular values, can hold: its power-of-two scale leaves a factor of two
-// below the largest float16.  The grid is even in s^(1/4): small singular values grow fastest.
-constexpr int NS_GRID = 2048;
+// below the largest float16.  The grid is even in s^(1/4): small singular values grow fastest.  0: out of range.
+constexpr int NS_GRID = 256;
 static float ns_scale(const double* v)
 {
     double top = 1e-3;
-    for (int i = 0; i <= NS_GRID; ++i) { const double a = v[i] < 0 ? -v[i] : v[i]; if (!(a <= 1e30)) return 0.f; if (a > top) top = a; }
-    double s = 32768.0;
+    for (int i = 0; i <= NS_GRID; ++i) { const double a = v[i] < 0 ? -v[i] : v[i]; if (!(a <= 4096.0)) return 0.f; if (a > top) top = a; }
+    double s = 1.0;
     while (s * top > 32768.0) s *= 0.5;
-    while (s * top * 2.0 <= 32768.0 && s < 16384.0 * 64) s *= 2.0;
+    while (s * top * 2.0 <= 32768.0) s *= 2.0;
     return (float)s;
+}
+
+// The launches behind the pack pass
+struct NsOp { int apply, ny; NsProds pr; int q, xt; float alpha, beta; bool gram, last; };
+struct NsSchedule { int count; float sx; NsOp op[32 * 4]; };
+
+static bool ns_schedule(const saunet_ns_desc* d, bool compose, NsSchedule& w)
+{
+    double x[NS_GRID + 1], S[NS_GRID + 1], P[NS_GRID + 1], Q[NS_GRID + 1], R[NS_GRID + 1];
+    const double a = d->a, b = d->b, c = d->c;
+    for (int i = 0; i <= NS_GRID; ++i) { const double u = (double)i / NS_GRID; x[i] = u * u * u * u * (1.0 + 1e-6); }
+    float sx = w.sx = ns_scale(x);
+    w.count = 0;
+    int xt = 0;
+    auto push = [&](int ny, const NsProds& pr, bool gram) { w.op[w.count++] = NsOp{0, ny, pr, 0, 0, 0.f, 0.f, gram, false}; };
+    for (int done = 0; done < d->steps;) {
+        // three steps at a time on the Gram matrix while a^2 each keeps its rounding error below 2^8 of itself, else one
+        const int left = d->steps - done, nb = compose ? (left == 4 ? 2 : left < 3 ? left : 3) : 1;
+        for (int i = 0; i <= NS_GRID; ++i) S[i] = x[i] * x[i];
+        float sa = ns_scale(S), sp, sq = 0;
+        if (sa == 0.f) return false;
+        push(1, NsProds{{{NS_X, NS_X, -1, -1, NS_A, sa / (sx * sx), 0.f, 0.f}, {}}}, true);
+        double q = 0;
+        int Qb = NS_Q0;
+        for (int j = 0; j < nb; ++j) {
+            for (int i = 0; i <= NS_GRID; ++i) P[i] = b * S[i] + c * S[i] * S[i];
+            sp = ns_scale(P);
+            if (sp == 0.f) return false;
+            const int Pb = j ? NS_P : NS_Q0;
+            push(1, NsProds{{{NS_A, NS_A, NS_A, -1, Pb, (float)(c * sp / ((double)sa * sa)), (float)(b * sp / sa), 0.f}, {}}}, false);
+            NsProds pr = {};
+            int ny = 0;
+            if (j == 0) { for (int i = 0; i <= NS_GRID; ++i) Q[i] = P[i]; sq = sp; q = a; }
+            else {
+                for (int i = 0; i <= NS_GRID; ++i) Q[i] = a * Q[i] + q * P[i] + P[i] * Q[i];
+                const float s2 = ns_scale(Q);
+                if (s2 == 0.f) return false;
+                const int to = Qb == NS_Q0 ? NS_Q1 : NS_Q0;
+                pr.p[ny++] = {NS_P, Qb, Qb, NS_P, to, (float)(s2 / ((double)sp * sq)), (float)(a * s2 / sq), (float)(q * s2 / sp)};
+                Qb = to; sq = s2; q *= a;
+            }
+            float sr = 0;
+            if (j < nb - 1) {
+                for (int i = 0; i <= NS_GRID; ++i) R[i] = (a + P[i]) * S[i];
+                sr = ns_scale(R);
+                if (sr == 0.f) return false;
+                pr.p[ny++] = {Pb, NS_A, NS_A, -1, NS_R, (float)(sr / ((double)sp * sa)), (float)(a * sr / sa), 0.f};
+            }
+            if (ny) push(ny, pr, false);
+            if (j < nb - 1) {
+                for (int i = 0; i <= NS_GRID; ++i) S[i] = (a + P[i]) * R[i];
+                const float s2 = ns_scale(S);
+                if (s2 == 0.f) return false;
+                push(1, NsProds{{{NS_R, Pb, NS_R, -1, NS_A, (float)(s2 / ((double)sr * sp)), (float)(a * s2 / sr), 0.f}, {}}}, false);
+                sa = s2;
+            }
+        }
+        for (int i = 0; i <= NS_GRID; ++i) x[i] = (q + Q[i]) * x[i];
+        done += nb;
+        const bool last = done >= d->steps;
+        const float s2 = last ? 1.f : ns_scale(x);
+        if (s2 == 0.f) return false;
+        w.op[w.count++] = NsOp{1, 0, {}, Qb, xt, (float)(s2 / ((double)sq * sx)), (float)(q * s2 / sx), false, last};
+        xt ^= 1; sx = s2;
+    }
+    return true;
+}
+
+template <class Core, typename T, bool MUON> static void ns_launch_apply(const saunet_ns_desc* d, const NsPlan& p, const NsItem* tab, const NsOp& o, const float* hyper, hipStream_t st)
+{
+    if (!o.last) hipLaunchKernelGGL((ns_apply_kernel<Core, T, 0>), dim3((unsigned)p.app), dim3(256), Core::LDS, st, tab, (int)p.large, o.q, o.xt, o.alpha, o.beta, hyper, 0);
+    else hipLaunchKernelGGL((ns_apply_kernel<Core, T, MUON ? 2 : 1>), dim3((unsigned)p.app), dim3(256), Core::LDS, st, tab, (int)p.large, o.q, o.xt, o.alpha, o.beta, hyper, d->adjust);
+}
+template <class Core> static void ns_launch_prod(const NsPlan& p, const NsItem* tab, const NsOp& o, hipStream_t st)
+{
+    const int kind = o.gram ? NS_GRAM : o.ny == 2 ? NS_TWO : NS_ONE;
+    hipLaunchKernelGGL((ns_prod_kernel<Core>), dim3((unsigned)p.grid[kind], o.ny), dim3(256), Core::LDS, st, tab, (int)p.large, kind, o.pr);
+    if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(256), 0, st, tab, (int)p.large, kind, o.pr);
 }
 
 template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
 {
+    static thread_local NsItem large[4096];
+    static thread_local NssItem small[4096];
     NsPlan p;
-    int rc = ns_plan(d, p, nullptr, nullptr);
+    char* ws = (char*)workspace;
+    int rc = ns_plan(d, p, large, small, ws);
     if (rc) return rc;
     if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255)) return set_error(SAUNET_BAD_SHAPE, "%s: the workspace has to hold %ld bytes on a 256-byte border", who, p.bytes);
-    // the scalar iteration on a grid of singular values: ranges of every intermediate matrix, from which its scale follows
-    static thread_local double x[NS_GRID + 1], S[NS_GRID + 1], P[NS_GRID + 1], Q[NS_GRID + 1], R[NS_GRID + 1];
-    static thread_local NsItem items[4096];
-    char* ws = (char*)workspace;
-    rc = ns_plan(d, p, items, ws);
-    if (rc) return rc;
-    NsItem* tab = (NsItem*)ws;
-    double* part = (double*)(ws + p.tab_bytes);
-    const int n = d->count;
-    const double a = d->a, b = d->b, c = d->c;
-    // first check that every scale exists, launching nothing; then the same walk with launches
-    for (int go = 0; go < 2; ++go) {
-        for (int i = 0; i <= NS_GRID; ++i) { const double u = (double)i / NS_GRID; x[i] = u * u * u * u * (1.0 + 1e-6); }
-        float sx = ns_scale(x);
-        if (go) {
-            for (int i = 0; i < n; i += NS_CHUNK) {
-                NsItems ch;
-                const int k = n - i < NS_CHUNK ? n - i : NS_CHUNK;
-                memcpy(ch.it, items + i, sizeof(NsItem) * k);
-                hipLaunchKernelGGL(ns_setup_kernel, dim3(1), dim3(64), 0, st, ch, k, tab + i);
-            }
-            hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)p.norm), dim3(256), 0, st, tab, n, hyper, part);
-            hipLaunchKernelGGL((ns_pack_kernel<T, MUON>), dim3((unsigned)p.pack), dim3(256), 0, st, tab, n, hyper, part, d->eps, sx);
-            SAUNET_CHECK_LAUNCH("ns_pack");
-        }
-        int xt = 0;
-        for (int done = 0; done < d->steps;) {
-            // three steps at a time on the Gram matrix while a^2 each keeps its rounding error below 2^8 of itself, else one
-            const int left = d->steps - done;
-            int nb = a * a <= 16.0 && p.shortest >= 32 ? (left == 4 ? 2 : left < 3 ? left : 3) : 1;
-            for (int i = 0; i <= NS_GRID; ++i) S[i] = x[i] * x[i];
-            float sa = ns_scale(S), sp = 0, sq = 0;
-            if (sa == 0.f || sx == 0.f) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
-            if (go) {
-                const float alpha = sa / (sx * sx);
-                hipLaunchKernelGGL(ns_gram_kernel, dim3((unsigned)p.gram), dim3(256), NsCore::LDS, st, tab, n, alpha);
-                SAUNET_CHECK_LAUNCH("ns_gram");
-                if (p.split) { hipLaunchKernelGGL(ns_gram_finish_kernel, dim3((unsigned)p.sym), dim3(256), 0, st, tab, n, alpha); SAUNET_CHECK_LAUNCH("ns_gram_finish"); }
-            }
-            double q = 0;
-            int Qb = NS_Q0;
-            auto launch = [&](NsProds pr, int ny) { if (go) hipLaunchKernelGGL(ns_sym_kernel, dim3((unsigned)p.sym, ny), dim3(256), NsCore::LDS, st, tab, n, pr); };
-            for (int j = 0; j < nb; ++j) {
-                for (int i = 0; i <= NS_GRID; ++i) P[i] = b * S[i] + c * S[i] * S[i];
-                sp = ns_scale(P);
-                if (sp == 0.f) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
-                const int Pb = j ? NS_P : NS_Q0;
-                launch(NsProds{{{NS_A, NS_A, NS_A, -1, Pb, (float)(c * sp / ((double)sa * sa)), (float)(b * sp / sa), 0.f}, {}}}, 1);
-                NsProds pr = {};
-                int ny = 0;
-                if (j == 0) { for (int i = 0; i <= NS_GRID; ++i) Q[i] = P[i]; sq = sp; q = a; }
-                else {
-                    for (int i = 0; i <= NS_GRID; ++i) Q[i] = a * Q[i] + q * P[i] + P[i] * Q[i];
-                    const float s2 = ns_scale(Q);
-                    if (s2 == 0.f) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
-                    pr.p[ny++] = {NS_P, Qb, Qb, NS_P, Qb == NS_Q0 ? NS_Q1 : NS_Q0, (float)(s2 / ((double)sp * sq)), (float)(a * s2 / sq), (float)(q * s2 / sp)};
-                    Qb = Qb == NS_Q0 ? NS_Q1 : NS_Q0; sq = s2; q *= a;
-                }
-                float sr = 0;
-                if (j < nb - 1) {
-                    for (int i = 0; i <= NS_GRID; ++i) R[i] = (a + P[i]) * S[i];
-                    sr = ns_scale(R);
-                    if (sr == 0.f) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
-                    pr.p[ny++] = {Pb, NS_A, NS_A, -1, NS_R, (float)(sr / ((double)sp * sa)), (float)(a * sr / sa), 0.f};
-                }
-                if (ny) launch(pr, ny);
-                if (j < nb - 1) {
-                    for (int i = 0; i <= NS_GRID; ++i) S[i] = (a + P[i]) * R[i];
-                    const float s2 = ns_scale(S);
-                    if (s2 == 0.f) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
-                    launch(NsProds{{{NS_R, Pb, NS_R, -1, NS_A, (float)(s2 / ((double)sr * sp)), (float)(a * s2 / sr), 0.f}, {}}}, 1);
-                    sa = s2;
-                }
-                if (go) SAUNET_CHECK_LAUNCH("ns_sym");
-            }
-            for (int i = 0; i <= NS_GRID; ++i) x[i] = (q + Q[i]) * x[i];
-            done += nb;
-            const float s2 = ns_scale(x);
-            if (done < d->steps) {
-                if (s2 == 0.f) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
-                if (go) hipLaunchKernelGGL((ns_apply_kernel<T, 0>), dim3((unsigned)p.app), dim3(256), NsCore::LDS, st, tab, n, Qb, xt, (float)(s2 / ((double)sq * sx)), (float)(q * s2 / sx), hyper, 0);
-                xt ^= 1; sx = s2;
-            } else if (go) {
-                hipLaunchKernelGGL((ns_apply_kernel<T, MUON ? 2 : 1>), dim3((unsigned)p.app), dim3(256), NsCore::LDS, st, tab, n, Qb, xt, (float)(1.0 / ((double)sq * sx)), (float)(q / sx), hyper, d->adjust);
-            }
-            if (go) SAUNET_CHECK_LAUNCH("ns_apply");
+    NsSchedule w;
+    if (!ns_schedule(d, (double)d->a * d->a <= 16.0 && p.shortest >= 32, w)) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
+    for (long i = 0; i < p.small; i += NSS_CHUNK) {
+        NssItems ch;
+        const int k = (int)(p.small - i < NSS_CHUNK ? p.small - i : NSS_CHUNK);
+        int grid = 0;
+        for (int j = 0; j < k; ++j) { ch.it[j] = small[i + j]; ch.it[j].p = grid; grid += small[i + j].p; }
+        hipLaunchKernelGGL((nss_gram_kernel<T, MUON>), dim3(grid), dim3(256), 0, st, ch, k, hyper);
+        hipLaunchKernelGGL(nss_poly_kernel, dim3(k), dim3(512), 0, st, ch, d->steps, (double)d->a, (double)d->b, (double)d->c, d->eps);
+        hipLaunchKernelGGL((nss_apply_kernel<T, MUON>), dim3(grid), dim3(256), 0, st, ch, k, hyper, d->adjust);
+        SAUNET_CHECK_LAUNCH("nss_apply");
+    }
+    if (!p.large) return SAUNET_OK;
+    NsItem* tab = (NsItem*)(ws + p.tab_at);
+    double* part = (double*)(ws + p.part_at);
+    const int n = (int)p.large;
+    for (int i = 0; i < n; i += NS_CHUNK) {
+        NsItems ch;
+        const int k = n - i < NS_CHUNK ? n - i : NS_CHUNK;
+        memcpy(ch.it, large + i, sizeof(NsItem) * k);
+        hipLaunchKernelGGL(ns_setup_kernel, dim3(1), dim3(64), 0, st, ch, k, tab + i);
+    }
+    hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)p.norm), dim3(256), 0, st, tab, n, hyper, part);
+    hipLaunchKernelGGL((ns_pack_kernel<T, MUON>), dim3((unsigned)p.pack), dim3(256), 0, st, tab, n, hyper, part, d->eps, w.sx);
+    SAUNET_CHECK_LAUNCH("ns_pack");
+    for (int i = 0; i < w.count; ++i) {
+        const NsOp& o = w.op[i];
+        if (o.apply) {
+            if (p.tile_n == 64) ns_launch_apply<NsCore64, T, MUON>(d, p, tab, o, hyper, st);
+            else ns_launch_apply<NsCore128, T, MUON>(d, p, tab, o, hyper, st);
+            SAUNET_CHECK_LAUNCH("ns_apply");
+        } else {
+            if (p.tile_m == 64) ns_launch_prod<NsCore64>(p, tab, o, st);
+            else ns_launch_prod<NsCore128>(p, tab, o, st);
+            SAUNET_CHECK_LAUNCH("ns_prod");
         }
     }
     return SAUNET_OK;
@@ -538,9 +810,11 @@ extern "C" {
 
 int64_t saunet_newton_schulz_workspace(const saunet_ns_desc* d)
 {
+    static thread_local NsItem large[4096];
+    static thread_local NssItem small[4096];
     NsPlan p;
     int rc = ns_check(d, "newton_schulz");
-    if (!rc) rc = ns_plan(d, p, nullptr, nullptr);
+    if (!rc) rc = ns_plan(d, p, large, small, nullptr);
     return rc ? rc : p.bytes;
 }
 

@@ -35,12 +35,15 @@ template <int N> __device__ __forceinline__ void nt_wait_barrier()
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(N) : "memory");
 }
 
-// Workgroup id -> tile (r, c) of a rows x cols grid.  Ids go round the eight XCDs, each with an L2 of its own: XCD x takes the x-th eighth of the tiles, and
-// walks it in bands of eight tile rows, so that the tiles in flight on one L2 share both operands.
-__device__ __forceinline__ void nt_place(int id, int total, int rows, int cols, int& r, int& c)
+// Workgroup ids go round the eight XCDs, each with an L2 of its own: XCD x takes the x-th eighth of the work, so that neighbours share an L2
+__device__ __forceinline__ int nt_xcd(int id, int total)
 {
     const int x = id & 7, q = total >> 3, rest = total & 7;
-    const int t = x * q + (x < rest ? x : rest) + (id >> 3);
+    return x * q + (x < rest ? x : rest) + (id >> 3);
+}
+// t-th tile of a rows x cols grid walked in bands of eight tile rows: the tiles in flight share both operands
+__device__ __forceinline__ void nt_band(int t, int rows, int cols, int& r, int& c)
+{
     const int band = t / (8 * cols), h = rows - band * 8 < 8 ? rows - band * 8 : 8, in = t - band * 8 * cols;
     r = band * 8 + in % h;
     c = in / h;
