@@ -156,14 +156,15 @@ template <typename T> static void q_launch(const QArgs& a, hipStream_t st)
     constexpr int V = QElem<T>::V;
 #define Q_GO(G, NV) hipLaunchKernelGGL((quantize_rows_kernel<T, G, NV>), dim3((unsigned)((a.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, st, a)
     const bool few = a.rows <= 1024 && a.k > 128 * V;
-    if (!a.vec || a.k > 1024 * V) { if (a.rows <= 4096 && a.k > 256) Q_GO(256, 0); else Q_GO(64, 0); }
+    if (!a.vec || a.k > 2048 * V) { if (a.rows <= 4096 && a.k > 256) Q_GO(256, 0); else Q_GO(64, 0); }
     else if (a.k <= 16 * V) Q_GO(16, 1);
     else if (a.k <= 32 * V) Q_GO(16, 2);
     else if (a.k <= 64 * V) Q_GO(64, 1);
     else if (a.k <= 128 * V) Q_GO(64, 2);
     else if (a.k <= 256 * V) { if (few) Q_GO(256, 1); else Q_GO(64, 4); }
     else if (a.k <= 512 * V) { if (few) Q_GO(256, 2); else Q_GO(64, 8); }
-    else Q_GO(256, 4);
+    else if (a.k <= 1024 * V) Q_GO(256, 4);
+    else Q_GO(256, 8);
 #undef Q_GO
 }
 
@@ -307,13 +308,96 @@ template <typename T, int MT> __global__ __launch_bounds__(FEW_WAVES * 64) void 
     }
 }
 
+// The same for up to 8 floating-point rows: every workgroup quantises all of them into LDS, 512 / (rows rounded up to a power of two) threads a row,
+// while its first weight loads are in flight.  One launch instead of two, us: one row of 4096 through 4096 channels 7.7 against 9.1, of 1024 through 512
+// 4.1 against 5.4; two rows of 2048 5.9 against 6.2.  Re-quantising in every workgroup costs more than the second launch beyond some 4096 values in
+// several rows: two of 4096 9.6 against 9.0, eight of 2048 13.2 against 6.7.
+constexpr int FEW_LDS = 16384;
+
+template <typename X, typename T> __global__ __launch_bounds__(FEW_WAVES * 64) void linear_int8_few_kernel(I8Args g, QArgs q, int group)
+{
+    __shared__ __attribute__((aligned(16))) signed char s_q[FEW_LDS];
+    __shared__ int s_red[FEW_WAVES][16][17];
+    __shared__ unsigned s_top[FEW_WAVES];
+    __shared__ float s_sa[8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, kq = (lane >> 4) * 16, n0 = blockIdx.x * 16;
+    const char* b = g.b + (long)(n0 + r < g.n ? n0 + r : g.n - 1) * g.ldb + kq;
+    i32x4 fb[FEW_UNROLL];
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < FEW_UNROLL; ++u) { const int s = s0 + u * FEW_WAVES; fb[u] = s < g.ksteps ? __builtin_nontemporal_load((const i32x4*)(b + (long)s * 64)) : i32x4{0, 0, 0, 0}; }
+    };
+    fetch(wave);
+    {
+        const int row = tid / group, at = tid % group;
+        const bool mine = row < q.rows;
+        const X* x = (const X*)q.x + (mine ? row : 0) * q.ldx;
+        unsigned top = 0;
+        if (mine)
+            for (int c = at; c < q.k; c += group) { const unsigned t = __float_as_uint(QElem<X>::load(x + c)) & 0x7fffffffu; top = t > top ? t : top; }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) { const unsigned t = __shfl_xor(top, o, 64); top = t > top ? t : top; }
+        if (lane == 0) s_top[wave] = top;
+        __syncthreads();
+        const int w0 = wave / (group / 64) * (group / 64);
+        top = 0;
+        for (int w = 0; w < group / 64; ++w) top = s_top[w0 + w] > top ? s_top[w0 + w] : top;
+        const QScale s = q_scale(top);
+        if (mine) {
+            if (at == 0) s_sa[row] = s.s;
+            const int kp = g.ksteps * 64;
+            for (int c = at * 4; c < kp; c += group * 4) {
+                float f[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[j] = c + j < q.k ? QElem<X>::load(x + c + j) : 0.f;
+                *(unsigned*)(s_q + row * kp + c) = q_round4(f, s);
+            }
+        }
+    }
+    __syncthreads();
+    const signed char* a = s_q + (r < q.rows ? r : (int)q.rows - 1) * (g.ksteps * 64) + kq;
+    i32x4 acc = {0, 0, 0, 0};
+    for (int s0 = wave; s0 < g.ksteps; s0 += FEW_WAVES * FEW_UNROLL) {
+        if (s0 != wave) fetch(s0);
+#pragma unroll
+        for (int u = 0; u < FEW_UNROLL; ++u) {
+            const int s = s0 + u * FEW_WAVES;
+            if (s < g.ksteps) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[u], *(const i32x4*)(a + s * 64), acc, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_red[wave][r][(lane >> 4) * 4 + i] = acc[i];
+    __syncthreads();
+    if (tid < 256) {
+        const int c = tid & 15, m = tid >> 4, n = n0 + c;
+        if (m < g.m && n < g.n) {
+            int sum = 0;
+#pragma unroll
+            for (int w = 0; w < FEW_WAVES; ++w) sum += s_red[w][m][c];
+            float v = fmaf((float)sum * s_sa[m], g.sb[n], g.bias ? g.bias[n] : 0.f);
+            if (g.relu && v < 0.f) v = 0.f;
+            ((T*)g.y)[m * g.ldy + n] = YElem<T>::cvt(v);
+        }
+    }
+}
+template <typename X> static void linear_few(const I8Args& g, const QArgs& q, int dtype, hipStream_t st)
+{
+    int group = FEW_WAVES * 64;
+    for (int m = 1; m < g.m; m *= 2) group /= 2;
+    const dim3 grid((unsigned)cdiv(g.n, 16)), block(FEW_WAVES * 64);
+    if (dtype == SAUNET_F32) hipLaunchKernelGGL((linear_int8_few_kernel<X, float>), grid, block, 0, st, g, q, group);
+    else if (dtype == SAUNET_BF16) hipLaunchKernelGGL((linear_int8_few_kernel<X, u16>), grid, block, 0, st, g, q, group);
+    else hipLaunchKernelGGL((linear_int8_few_kernel<X, _Float16>), grid, block, 0, st, g, q, group);
+}
+
 template <typename T> static int mm8_launch(const I8Args& g, hipStream_t st)
 {
-    if (g.m <= 64) {
+    // a workgroup of the streaming kernel reads all tokens again: above 16 x 16384 of them times channels the tiles win (us: 24 tokens of 4096 through
+    // 4096 channels 12.9 against 17.6, 64 tokens through 16384 channels 53 against 24)
+    if (g.m <= 32 && (long)g.n * ((g.m + 15) / 16) <= 16384) {
         const dim3 grid((unsigned)cdiv(g.n, 16)), block(FEW_WAVES * 64);
         if (g.m <= 16) hipLaunchKernelGGL((matmul_int8_few_kernel<T, 1>), grid, block, 0, st, g);
-        else if (g.m <= 32) hipLaunchKernelGGL((matmul_int8_few_kernel<T, 2>), grid, block, 0, st, g);
-        else hipLaunchKernelGGL((matmul_int8_few_kernel<T, 4>), grid, block, 0, st, g);
+        else hipLaunchKernelGGL((matmul_int8_few_kernel<T, 2>), grid, block, 0, st, g);
         SAUNET_CHECK_LAUNCH("matmul_int8_few");
         return SAUNET_OK;
     }
@@ -323,6 +407,31 @@ template <typename T> static int mm8_launch(const I8Args& g, hipStream_t st)
     if (t64 <= 384) return mm8_tiles<T, I8Core64>(g, st);
     if (t64 <= 768 || g.ksteps < 8) return mm8_tiles<T, I8CoreTall>(g, st);
     return mm8_tiles<T, I8Core128>(g, st);
+}
+
+static int int8_check(const saunet_int8_desc* d, const char* who)
+{
+    if (!d || d->m < 0 || d->n < 1 || d->k < 1 || d->k > 131071) return set_error(SAUNET_BAD_SHAPE, "%s: bad sizes", who);
+    const int64_t kp = (d->k + 63) / 64 * 64;
+    if (d->ldb < kp || (d->ldb & 15) || d->ldb > (1 << 22) || d->ldy < d->n) return set_error(SAUNET_BAD_SHAPE, "%s: bad strides (%lld, %lld)", who, (long long)d->ldb, (long long)d->ldy);
+    if (d->dtype != SAUNET_F32 && d->dtype != SAUNET_BF16 && d->dtype != SAUNET_F16) return set_error(SAUNET_BAD_DTYPE, "%s: dtype %d", who, d->dtype);
+    if (d->m == 0) return SAUNET_OK;
+    if (!d->b || !d->b_scale || !d->y) return set_error(SAUNET_BAD_SHAPE, "%s: missing memory", who);
+    if ((uintptr_t)d->b & 15) return set_error(SAUNET_BAD_ALIGN, "%s: operands have to lie on a 16-byte border", who);
+    return SAUNET_OK;
+}
+static I8Args int8_args(const saunet_int8_desc* d, const void* a, const float* sa, int64_t lda)
+{
+    const int size = d->dtype == SAUNET_F32 ? 4 : 2;
+    return I8Args{(const char*)a, sa, lda, d->m, (const char*)d->b, d->b_scale, d->ldb, d->n, (d->k + 63) / 64, d->bias, d->relu, d->y, d->ldy,
+                  !((uintptr_t)d->y & 15) && !(d->ldy * size & 15), 0};
+}
+static int int8_product(const saunet_int8_desc* d, const void* a, const float* sa, int64_t lda, hipStream_t st)
+{
+    const I8Args g = int8_args(d, a, sa, lda);
+    if (d->dtype == SAUNET_F32) return mm8_launch<float>(g, st);
+    if (d->dtype == SAUNET_BF16) return mm8_launch<u16>(g, st);
+    return mm8_launch<_Float16>(g, st);
 }
 
 }  // namespace saunet
@@ -351,20 +460,39 @@ int saunet_quantize_rows(int dtype, const void* x, int64_t ldx, int64_t rows, in
 
 int saunet_matmul_int8(const saunet_int8_desc* d, void* stream)
 {
-    if (!d || d->m < 0 || d->n < 1 || d->k < 1 || d->k > 131071) return set_error(SAUNET_BAD_SHAPE, "matmul_int8: bad sizes");
+    const int rc = int8_check(d, "matmul_int8");
+    if (rc) return rc;
     const int64_t kp = (d->k + 63) / 64 * 64;
-    if (d->lda < kp || d->ldb < kp || (d->lda & 15) || (d->ldb & 15) || d->lda > (1 << 22) || d->ldb > (1 << 22) || d->ldy < d->n) return set_error(SAUNET_BAD_SHAPE, "matmul_int8: bad strides (%lld, %lld, %lld)", (long long)d->lda, (long long)d->ldb, (long long)d->ldy);
-    if (d->dtype != SAUNET_F32 && d->dtype != SAUNET_BF16 && d->dtype != SAUNET_F16) return set_error(SAUNET_BAD_DTYPE, "matmul_int8: dtype %d", d->dtype);
+    if (d->lda < kp || (d->lda & 15) || d->lda > (1 << 22)) return set_error(SAUNET_BAD_SHAPE, "matmul_int8: bad stride %lld", (long long)d->lda);
     if (d->m == 0) return SAUNET_OK;
-    if (!d->a || !d->b || !d->a_scale || !d->b_scale || !d->y) return set_error(SAUNET_BAD_SHAPE, "matmul_int8: missing memory");
-    if (((uintptr_t)d->a | (uintptr_t)d->b) & 15) return set_error(SAUNET_BAD_ALIGN, "matmul_int8: operands have to lie on a 16-byte border");
-    const int size = d->dtype == SAUNET_F32 ? 4 : 2;
-    I8Args g = {(const char*)d->a, d->a_scale, d->lda, d->m, (const char*)d->b, d->b_scale, d->ldb, d->n, (int)(kp / 64), d->bias, d->relu, d->y, d->ldy,
-                !((uintptr_t)d->y & 15) && !(d->ldy * size & 15), 0};
+    if (!d->a || !d->a_scale) return set_error(SAUNET_BAD_SHAPE, "matmul_int8: missing memory");
+    if ((uintptr_t)d->a & 15) return set_error(SAUNET_BAD_ALIGN, "matmul_int8: operands have to lie on a 16-byte border");
+    return int8_product(d, d->a, d->a_scale, d->lda, (hipStream_t)stream);
+}
+
+int saunet_linear_int8(const saunet_int8_desc* d, int x_dtype, const void* x, int64_t ldx, void* workspace, int64_t workspace_bytes, void* stream)
+{
+    const int rc = int8_check(d, "linear_int8");
+    if (rc) return rc;
+    if (x_dtype != SAUNET_F32 && x_dtype != SAUNET_BF16 && x_dtype != SAUNET_F16) return set_error(SAUNET_BAD_DTYPE, "linear_int8: dtype %d", x_dtype);
+    if (ldx < d->k) return set_error(SAUNET_BAD_SHAPE, "linear_int8: bad stride %lld", (long long)ldx);
+    if (d->m == 0) return SAUNET_OK;
+    const int64_t kp = (d->k + 63) / 64 * 64;
+    if (!x) return set_error(SAUNET_BAD_SHAPE, "linear_int8: missing memory");
     hipStream_t st = (hipStream_t)stream;
-    if (d->dtype == SAUNET_F32) return mm8_launch<float>(g, st);
-    if (d->dtype == SAUNET_BF16) return mm8_launch<u16>(g, st);
-    return mm8_launch<_Float16>(g, st);
+    if (d->m <= 8 && d->m * kp <= (d->m == 1 ? FEW_LDS : 4096)) {
+        const I8Args g = int8_args(d, nullptr, nullptr, 0);
+        const QArgs q = {x, ldx, d->m, d->k, nullptr, nullptr, 0, nullptr, 0, nullptr, 0};
+        if (x_dtype == SAUNET_F32) linear_few<float>(g, q, d->dtype, st);
+        else if (x_dtype == SAUNET_BF16) linear_few<u16>(g, q, d->dtype, st);
+        else linear_few<_Float16>(g, q, d->dtype, st);
+        SAUNET_CHECK_LAUNCH("linear_int8_few");
+        return SAUNET_OK;
+    }
+    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < d->m * (kp + 4)) return set_error(SAUNET_BAD_SHAPE, "linear_int8: the workspace has to hold %lld bytes on a 16-byte border", (long long)(d->m * (kp + 4)));
+    float* s = (float*)((char*)workspace + d->m * kp);
+    const int qc = saunet_quantize_rows(x_dtype, x, ldx, d->m, d->k, nullptr, nullptr, 0, workspace, kp, s, stream);
+    return qc ? qc : int8_product(d, workspace, s, kp, st);
 }
 
 }  // extern "C"

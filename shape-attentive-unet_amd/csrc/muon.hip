@@ -36,7 +36,7 @@ constexpr int NS_NORM = 8192;                // elements a workgroup of the norm
 enum { NS_X = -1, NS_A = 0, NS_P, NS_R, NS_Q0, NS_Q1, NS_NSYM };
 struct NsView {
     int m, n, mp, np, tall;
-    char *x, *xt[2], *sym[NS_NSYM]; float* part;
+    char *x, *s0; long bx, bs;
     static long bytes(int rows, int cols)
     {
         const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows, mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
@@ -47,12 +47,12 @@ struct NsView {
         tall = it.rows > it.cols;
         m = tall ? it.cols : it.rows; n = tall ? it.rows : it.cols;
         mp = (m + 31) / 32 * 32; np = (n + 31) / 32 * 32;
-        const long bx = (long)mp * np * 4, bs = (long)mp * mp * 4;
-        char* p = it.ws;
-        x = p; p += bx; xt[0] = p; p += bx; xt[1] = p; p += bx;
-        for (int i = 0; i < NS_NSYM; ++i) { sym[i] = p; p += bs; }
-        part = (float*)p;
+        bx = (long)mp * np * 4; bs = (long)mp * mp * 4;
+        x = it.ws; s0 = x + 3 * bx;
     }
+    __device__ __forceinline__ char* xt(int i) const { return x + (1 + i) * bx; }
+    __device__ __forceinline__ char* sym(int i) const { return s0 + i * bs; }
+    __device__ __forceinline__ float* part() const { return (float*)(s0 + NS_NSYM * bs); }
 };
 
 // the matrix whose workgroups include `id`: the last whose first(i) is not above it; two rounds of one load a lane (count <= 4096)
@@ -154,8 +154,8 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_
     }
     __syncthreads();
     // 8 consecutive elements a thread: 16 bytes of high and of low parts; along[] runs along the caller's rows, across[] along its columns
-    char* along = v.tall ? v.xt[0] : v.x;
-    char* across = v.tall ? v.x : v.xt[0];
+    char* along = v.tall ? v.xt(0) : v.x;
+    char* across = v.tall ? v.x : v.xt(0);
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
         for (int k = tid; k < 64 * 8; k += 256) {
@@ -172,7 +172,7 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_
 }
 
 // ---- products -----------------------------------------------------------------------------------------------------------------------
-// Both tiles take 64 KB of LDS, two workgroups a CU
+// 64 KB of LDS, two workgroups a CU.  (Twice the stages in one workgroup a CU brought nothing, also where a launch has fewer workgroups than CUs.)
 typedef NtCore<NtF16Pair, 128, 128, 2, 2, 2> NsCore128;
 typedef NtCore<NtF16Pair, 64, 64, 2, 2, 4> NsCore64;
 constexpr int NS_SLOTS = 512;
@@ -187,16 +187,30 @@ template <class Core> struct NsQuads {
         i = (wave / Core::WGN) * (Core::BM / Core::WGM) + ti * 32 + g * 8 + (lane >> 5) * 4;
         j = (wave % Core::WGN) * (Core::BN / Core::WGN) + tj * 32 + (lane & 31);
     }
-    template <typename F> static __device__ __forceinline__ void each(f32x16 (&acc)[Core::TM][Core::TN], F f)
+    template <typename F> static __device__ __forceinline__ void each(F f)
     {
 #pragma unroll
-        for (int b = 0; b < N; ++b) {
-            int i, j;
-            at(b, i, j);
-            const f32x16& c = acc[b / (4 * Core::TN)][b / 4 % Core::TN];
-            const float q[4] = {c[(b & 3) * 4], c[(b & 3) * 4 + 1], c[(b & 3) * 4 + 2], c[(b & 3) * 4 + 3]};
-            f(b, i, j, q);
-        }
+        for (int b = 0; b < N; ++b) { int i, j; at(b, i, j); f(b, i, j); }
+    }
+    // acc <- alpha acc + beta E over the tile at (i0, j0), E[j][i .. i + 3] a pair matrix of ld bytes a row.  All loads are under way before the first is
+    // used: a load behind another quad's stores would wait for them, sixteen memory latencies in a row (20 of the 50 us of such a launch).
+    static __device__ __forceinline__ void blend(f32x16 (&acc)[Core::TM][Core::TN], float alpha, float beta, const char* e, long ld, int i0, int j0, int mlim, int nlim)
+    {
+        f16x4_t h[N], l[N];
+        each([&](int b, int i, int j) {
+            i += i0; j += j0;
+            if (i < mlim && j < nlim) { const char* s = e + (long)j * ld + (i >> 5) * 128 + (i & 31) * 2; h[b] = *(const f16x4_t*)s; l[b] = *(const f16x4_t*)(s + 64); }
+        });
+        each([&](int b, int, int) {
+            f32x16& c = acc[b / (4 * Core::TN)][b / 4 % Core::TN];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) c[(b & 3) * 4 + r] = fmaf(alpha, c[(b & 3) * 4 + r], beta * ((float)h[b][r] + (float)l[b][r]));
+        });
+    }
+    static __device__ __forceinline__ void quad(const f32x16 (&acc)[Core::TM][Core::TN], int b, float (&q)[4])
+    {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) q[r] = acc[b / (4 * Core::TN)][b / 4 % Core::TN][(b & 3) * 4 + r];
     }
 };
 // four consecutive elements (row j, columns i .. i + 3) of a pair matrix with lda bytes a row
@@ -235,13 +249,35 @@ __device__ __forceinline__ void ns_write4_sym(char* d, long ld, bool diag, int i
         *(_Float16*)q = s.h; *(_Float16*)(q + 64) = s.l;
     }
 }
-// tile t of the lower triangle, row by row: (ti, tj), tj <= ti
-__device__ __forceinline__ void ns_lower(int t, int& ti, int& tj)
+// tile t of the lower triangle of nt x nt tiles: (ti, tj), tj <= ti.  Walked in blocks of 8 x 8 tiles, so that the tiles in flight on one XCD share
+// eight row panels of either operand.
+__device__ __forceinline__ int ns_row(int t)          // row of t in a triangle walked row by row
 {
-    ti = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-    while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-    while (ti * (ti + 1) / 2 > t) --ti;
-    tj = t - ti * (ti + 1) / 2;
+    int i = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+    while ((i + 1) * (i + 2) / 2 <= t) ++i;
+    while (i * (i + 1) / 2 > t) --i;
+    return i;
+}
+__device__ __forceinline__ void ns_lower(int t, int nt, int& ti, int& tj)
+{
+    int I = (int)((sqrtf(16.f + 128.f * (float)t) - 4.f) * (1.f / 64.f));         // block rows before I hold 32 I^2 + 4 I tiles
+    while (32 * (I + 1) * (I + 1) + 4 * (I + 1) <= t) ++I;
+    while (32 * I * I + 4 * I > t) --I;
+    t -= 32 * I * I + 4 * I;
+    const int h = nt - 8 * I < 8 ? nt - 8 * I : 8;
+    if (t < h * 8 * I) { ti = 8 * I + t % h; tj = t / h; return; }
+    t -= h * 8 * I;
+    const int r = ns_row(t);
+    ti = 8 * I + r; tj = 8 * I + t - r * (r + 1) / 2;
+}
+
+// Workgroup ids go round the eight XCDs, each with an L2 of its own.  XCD x takes the x-th of eight runs of equal cost of the list, so that the tiles of a
+// matrix meet in one L2: dealt out one by one, six 1000 x 1024 matrices were read into all eight (220 MB a launch, 45 us at the rate of the fabric).
+struct NsDeal { int b[9]; };
+__device__ __forceinline__ int ns_dealt(const NsDeal& d, int id)
+{
+    const int x = id & 7, t = d.b[x] + (id >> 3);
+    return t < d.b[x + 1] ? t : -1;
 }
 
 // D = alpha A B^T (+ beta E + gamma F) for a symmetric D -- X X^T, or a product of symmetric matrices that commute: lower tiles, both halves
@@ -250,52 +286,47 @@ __device__ __forceinline__ void ns_lower(int t, int& ti, int& tj)
 struct NsProd { int a, b, e, f, d; float alpha, beta, gamma; };
 struct NsProds { NsProd p[2]; };
 
-__device__ __forceinline__ void ns_prod_store(const NsView& v, const NsProd& p, int ti, int tj, int i, int j, const float (&q)[4])
-{
-    if (i >= v.mp || j >= v.mp) return;                                    // whole 32 x 32 blocks
-    const long ld = (long)v.mp * 4;
-    float w[4], x[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) w[r] = p.alpha * q[r];
-    if (p.e >= 0) {
-        ns_read4(v.sym[p.e], ld, j, i, x);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) w[r] = fmaf(p.beta, x[r], w[r]);
-    }
-    if (p.f >= 0) {
-        ns_read4(v.sym[p.f], ld, j, i, x);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) w[r] = fmaf(p.gamma, x[r], w[r]);
-    }
-    ns_write4_sym(v.sym[p.d], ld, ti == tj, i, j, w);
-}
-
-template <class Core> __global__ __launch_bounds__(256, 2) void ns_prod_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr)
+template <class Core> __global__ __launch_bounds__(256, 2) void ns_prod_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr, NsDeal deal, int tail)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     constexpr int T = Core::BM;
-    const int id = blockIdx.x;
+    // (deal ends at the first cut tile of a single matrix: its parts follow in launch order, behind a whole number of rounds)
+    const int id = (int)blockIdx.x < tail ? ns_dealt(deal, blockIdx.x) : deal.b[8] + (int)blockIdx.x - tail;
+    if (id < 0) return;
     const NsProd p = pr.p[blockIdx.y];
     const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].split[kind].p; })];
     const NsView v(it);
     const NsSplit sl = it.split[kind];
+    const int nt = (v.mp + T - 1) / T, cut = nt * (nt + 1) / 2 - sl.full;
     int t = id - sl.p, sp = 0, parts = 1, ti, tj;
-    if (count == 1 && t < sl.full) t = nt_xcd(t, sl.full);                 // (a list is dealt out tile by tile: its tiles differ in cost)
-    if (t >= sl.full) { sp = (t - sl.full) % sl.s; t = sl.full + (t - sl.full) / sl.s; parts = sl.s; }
-    ns_lower(t, ti, tj);
+    if (t >= sl.full) { sp = (t - sl.full) / cut; t = sl.full + (t - sl.full) % cut; parts = sl.s; }       // neighbours work on one stretch of the reduction
+    ns_lower(t, nt, ti, tj);
     const int steps = (p.a == NS_X ? v.np : v.mp) / 32, k0 = (int)((long)steps * sp / parts), k1 = (int)((long)steps * (sp + 1) / parts);
     const long ld = steps * 128L;
-    const char* a = (p.a == NS_X ? v.x : v.sym[p.a]) + k0 * 128L;
-    const char* b = (p.a == NS_X ? v.x : v.sym[p.b]) + k0 * 128L;
+    const char* a = (p.a == NS_X ? v.x : v.sym(p.a)) + k0 * 128L;
+    const char* b = (p.a == NS_X ? v.x : v.sym(p.b)) + k0 * 128L;
     f32x16 acc[Core::TM][Core::TN] = {};
     Core::run(a + ti * T * ld, (unsigned)ld, v.mp - ti * T, b + tj * T * ld, (unsigned)ld, v.mp - tj * T, k1 - k0, smem, acc);
+    typedef NsQuads<Core> Quads;
     if (parts > 1) {
-        const int nt = (v.mp + T - 1) / T, cut = nt * (nt + 1) / 2 - sl.full;
-        float* d = v.part + (((long)blockIdx.y * cut + t - sl.full) * parts + sp) * NsQuads<Core>::FLOATS + threadIdx.x * 4;
-        NsQuads<Core>::each(acc, [&](int q, int, int, const float (&c)[4]) { *(f32x4*)(d + q * 1024) = f32x4{c[0], c[1], c[2], c[3]}; });
+        float* d = v.part() + (((long)blockIdx.y * cut + t - sl.full) * parts + sp) * Quads::FLOATS + threadIdx.x * 4;
+        Quads::each([&](int b, int, int) { float q[4]; Quads::quad(acc, b, q); *(f32x4*)(d + b * 1024) = f32x4{q[0], q[1], q[2], q[3]}; });
         return;
     }
-    NsQuads<Core>::each(acc, [&](int, int i, int j, const float (&c)[4]) { ns_prod_store(v, p, ti, tj, ti * T + i, tj * T + j, c); });
+    const long ls = (long)v.mp * 4;
+    float alpha = p.alpha;
+    if (p.e >= 0) { Quads::blend(acc, alpha, p.beta, v.sym(p.e), ls, ti * T, tj * T, v.mp, v.mp); alpha = 1.f; }
+    if (p.f >= 0) Quads::blend(acc, alpha, p.gamma, v.sym(p.f), ls, ti * T, tj * T, v.mp, v.mp);
+    char* d = v.sym(p.d);
+    Quads::each([&](int b, int i, int j) {
+        i += ti * T; j += tj * T;
+        if (i >= v.mp || j >= v.mp) return;                                // whole 32 x 32 blocks
+        float q[4];
+        Quads::quad(acc, b, q);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) q[r] *= alpha;
+        ns_write4_sym(d, ls, ti == tj, i, j, q);
+    });
 }
 // one accumulator quad of a cut tile a thread; blockIdx.x = tile * quads + quad
 template <class Core> __global__ __launch_bounds__(256) void ns_finish_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr)
@@ -307,16 +338,31 @@ template <class Core> __global__ __launch_bounds__(256) void ns_finish_kernel(co
     const NsSplit sl = it.split[kind];
     const int t = sl.full + id - sl.c;
     const NsView v(it);
-    int ti, tj, i, j;
-    ns_lower(t, ti, tj);
-    NsQuads<Core>::at(q, i, j);
     const int nt = (v.mp + T - 1) / T, cut = nt * (nt + 1) / 2 - sl.full;
-    const float* s = v.part + (((long)blockIdx.y * cut + t - sl.full) * sl.s) * NsQuads<Core>::FLOATS + q * 1024 + threadIdx.x * 4;
+    int ti, tj, i, j;
+    ns_lower(t, nt, ti, tj);
+    NsQuads<Core>::at(q, i, j);
+    const float* s = v.part() + (((long)blockIdx.y * cut + t - sl.full) * sl.s) * NsQuads<Core>::FLOATS + q * 1024 + threadIdx.x * 4;
     f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int sp = 0; sp < sl.s; ++sp) { const f32x4 w = *(const f32x4*)(s + (long)sp * NsQuads<Core>::FLOATS); for (int r = 0; r < 4; ++r) c[r] += w[r]; }
-    const float w[4] = {c[0], c[1], c[2], c[3]};
-    ns_prod_store(v, p, ti, tj, ti * T + i, tj * T + j, w);
+    i += ti * T; j += tj * T;
+    if (i >= v.mp || j >= v.mp) return;
+    const long ls = (long)v.mp * 4;
+    float w[4], x[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) w[r] = p.alpha * c[r];
+    if (p.e >= 0) {
+        ns_read4(v.sym(p.e), ls, j, i, x);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] = fmaf(p.beta, x[r], w[r]);
+    }
+    if (p.f >= 0) {
+        ns_read4(v.sym(p.f), ls, j, i, x);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] = fmaf(p.gamma, x[r], w[r]);
+    }
+    ns_write4_sym(v.sym(p.d), ls, ti == tj, i, j, w);
 }
 
 __device__ __forceinline__ void ns_rates(const float* hyper, int rows, int cols, int adjust, float& keep, float& rate)
@@ -327,38 +373,50 @@ __device__ __forceinline__ void ns_rates(const float* hyper, int rows, int cols,
 }
 
 // X <- alpha Q X + beta X.  MODE 0: back to X and the other X^T; 1: to the caller's matrix; 2: the Muon update of the caller's parameter
-template <class Core, typename T, int MODE> __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsItem* __restrict__ tab, int count, int q, int xt, float alpha, float beta, const float* __restrict__ hyper, int adjust)
+template <class Core, typename T, int MODE> __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsItem* __restrict__ tab, int count, int q, int xt, float alpha, float beta, const float* __restrict__ hyper, int adjust, NsDeal deal)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     constexpr int B = Core::BM;
-    const int id = count == 1 ? nt_xcd(blockIdx.x, gridDim.x) : blockIdx.x;
+    const int id = ns_dealt(deal, blockIdx.x);
+    if (id < 0) return;
     const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].p_app; })];
     const NsView v(it);
     int ti, tj;
     nt_band(id - it.p_app, (v.np + B - 1) / B, (v.mp + B - 1) / B, tj, ti);
     f32x16 acc[Core::TM][Core::TN] = {};
     const long ld = (long)v.mp * 4;
-    Core::run(v.sym[q] + ti * B * ld, (unsigned)ld, v.mp - ti * B, v.xt[xt] + tj * B * ld, (unsigned)ld, v.np - tj * B, v.mp / 32, smem, acc);
-    const char* x = v.xt[xt];
-    float keep = 0.f, rate = 0.f;
-    if (MODE == 2) ns_rates(hyper, it.rows, it.cols, adjust, keep, rate);
-    NsQuads<Core>::each(acc, [&](int, int i, int j, const float (&a)[4]) {
-        i += ti * B; j += tj * B;
-        if (i >= v.mp || j >= v.np) return;                                // whole 32 x 32 blocks
-        float w[4], o[4];
-        ns_read4(x, ld, j, i, o);
+    Core::run(v.sym(q) + ti * B * ld, (unsigned)ld, v.mp - ti * B, v.xt(xt) + tj * B * ld, (unsigned)ld, v.np - tj * B, v.mp / 32, smem, acc);
+    typedef NsQuads<Core> Quads;
+    Quads::blend(acc, alpha, beta, v.xt(xt), ld, ti * B, tj * B, v.mp, v.np);
+    if (MODE == 0) {
+        Quads::each([&](int b, int i, int j) {
+            i += ti * B; j += tj * B;
+            if (i >= v.mp || j >= v.np) return;                            // whole 32 x 32 blocks
+            float q[4];
+            Quads::quad(acc, b, q);
+            ns_write4(v.xt(xt ^ 1), ld, v.x, v.np * 4L, i, j, q);
+        });
+        return;
+    }
+    const long si = v.tall ? 1 : it.ld_dst, sj = v.tall ? it.ld_dst : 1;
+    T* d = (T*)it.dst + ti * B * si + tj * B * sj;
+    const int mi = v.m - ti * B, nj = v.n - tj * B;
+    if (MODE == 2) {
+        float keep, rate, old[Quads::N][4];
+        ns_rates(hyper, it.rows, it.cols, adjust, keep, rate);
+        Quads::each([&](int b, int i, int j) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) w[r] = fmaf(alpha, a[r], beta * o[r]);
-        if (MODE == 0) { ns_write4(v.xt[xt ^ 1], ld, v.x, v.np * 4L, i, j, w); return; }
-        if (j >= v.n) return;
-        T* d = (T*)it.dst + (v.tall ? (long)j * it.ld_dst + i : (long)i * it.ld_dst + j);
-        const long st = v.tall ? 1 : it.ld_dst;
+            for (int r = 0; r < 4; ++r) old[b][r] = i + r < mi && j < nj ? (float)d[(i + r) * si + j * sj] : 0.f;
+        });
+        Quads::each([&](int b, int i, int j) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (i + r >= v.m) break;
-            if (MODE == 1) ns_store(d + r * st, w[r]);
-            else d[r * st] = (T)fmaf(-rate, w[r], keep * (float)d[r * st]);
-        }
+            for (int r = 0; r < 4; ++r) if (i + r < mi && j < nj) d[(i + r) * si + j * sj] = (T)fmaf(-rate, acc[b / (4 * Core::TN)][b / 4 % Core::TN][(b & 3) * 4 + r], keep * old[b][r]);
+        });
+        return;
+    }
+    Quads::each([&](int b, int i, int j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) if (i + r < mi && j < nj) ns_store(d + (i + r) * si + j * sj, acc[b / (4 * Core::TN)][b / 4 % Core::TN][(b & 3) * 4 + r]);
     });
 }
 
@@ -555,7 +613,7 @@ static int ns_check(const saunet_ns_desc* d, const char* who)
 }
 
 // One call: the matrices with up to 32 rows go one way, the others the other way
-struct NsPlan { long small, large, norm, pack, tile, app, grid[NS_KINDS], cut[NS_KINDS], tab_at, part_at, bytes, shortest; int tile_m, tile_n; };
+struct NsPlan { long small, large, norm, pack, tile, app, grid[NS_KINDS], cut[NS_KINDS], tab_at, part_at, bytes, shortest; int tile_m, tile_n; NsDeal deal[NS_KINDS + 1]; };
 
 static bool ns_is_small(const saunet_ns_desc* d, const saunet_ns_item& t)
 {
@@ -564,42 +622,60 @@ static bool ns_is_small(const saunet_ns_desc* d, const saunet_ns_item& t)
     for (int i = 1; i < d->steps; ++i) grow *= (double)d->a * d->a;
     return (t.rows < t.cols ? t.rows : t.cols) <= 32 && grow <= 1e8;
 }
-// Cuts along the reduction, for one kind of launch (ny products a tile, steps(i) reduction steps of matrix i).  A launch that fills less than half of
-// the NS_SLOTS workgroups that run at once is cut until it fills them, eight steps a part and four parts at least (six 1000 x 1024 matrices in two
-// parts: 41 -> 33 us and 14 for the finishing launch); one of a few rounds whose last round is less than half full has that round's tiles cut.  4096 x 4096: 528 tiles on 512
-// slots were 262 us, with sixteen of them cut sixteen-fold 170 us.
+// Cuts along the reduction, for one kind of launch (ny products a tile, steps[i] reduction steps of matrix i).  A tile longer than an even share of the
+// launch's work is cut into shares (sixteen steps at least) where that saves 32 steps: they are 11 us, the finishing launch costs 8 (six 1000 x 1024
+// matrices in two parts of sixteen: 41 -> 33 us for the products, 14 more to finish).  A single matrix of a few rounds of NS_SLOTS workgroups whose last
+// round is less than half full has that round's tiles cut: 4096 x 4096, 528 tiles on 512 slots, 262 us -> 200 + 11.
 static void ns_cut(int kind, int ny, NsPlan& p, const int* tiles, const int* steps, int count, NsItem* out)
 {
-    long total = 0, at = 0;
-    int longest = 1;
-    for (int i = 0; i < count; ++i) { total += (long)tiles[i] * ny; if (steps[i] > longest) longest = steps[i]; }
-    int part = longest;                          // steps a part
+    long total = 0, at = 0, work = 0;
+    for (int i = 0; i < count; ++i) { total += (long)tiles[i] * ny; work += (long)tiles[i] * ny * steps[i]; }
+    const long share = work / NS_SLOTS > 16 ? work / NS_SLOTS : 16;
     long tail = 0, tail_s = 1;
-    if (total <= NS_SLOTS / 2) {
-        int lo = 8, hi = longest;
-        while (lo < hi) {                        // the smallest part for which the launch still fits
-            const int mid = (lo + hi) / 2;
-            long w = 0;
-            for (int i = 0; i < count; ++i) w += (long)tiles[i] * ny * ((steps[i] + mid - 1) / mid);
-            if (w <= NS_SLOTS) hi = mid; else lo = mid + 1;
-        }
-        part = lo;
-        if (part > longest / 4) part = longest;
-    } else if (total > NS_SLOTS && total < 4 * NS_SLOTS && total % NS_SLOTS && total % NS_SLOTS <= NS_SLOTS / 2) {
+    if (count == 1 && total > NS_SLOTS && total < 4 * NS_SLOTS && total % NS_SLOTS && total % NS_SLOTS <= NS_SLOTS / 2) {
         tail = (total % NS_SLOTS + ny - 1) / ny;
-        if (tail > tiles[count - 1]) tail = 0;
-        else { tail_s = NS_SLOTS / (tail * ny); if (tail_s > steps[count - 1] / 8) tail_s = steps[count - 1] / 8; if (tail_s < 2) { tail = 0; tail_s = 1; } }
+        tail_s = NS_SLOTS / (tail * ny);
+        if (tail_s > steps[0] / 8) tail_s = steps[0] / 8;
+        if (tail_s < 2) { tail = 0; tail_s = 1; }
     }
     p.cut[kind] = 0;
     for (int i = 0; i < count; ++i) {
         NsSplit s = {(int)at, tiles[i], 1, (int)p.cut[kind]};
-        if (i == count - 1 && tail) { s.full = tiles[i] - (int)tail; s.s = (int)tail_s; }
-        else if (steps[i] > part) { s.full = 0; s.s = (steps[i] + part - 1) / part; }
+        if (tail) { s.full = tiles[i] - (int)tail; s.s = (int)tail_s; }
+        else if (steps[i] >= share + 32) { s.full = 0; s.s = (int)((steps[i] + share - 1) / share); }
         p.cut[kind] += tiles[i] - s.full;
         at += s.full + (long)(tiles[i] - s.full) * s.s;
         out[i].split[kind] = s;
     }
     p.grid[kind] = at;
+}
+
+// Runs of equal cost for the XCDs: runs[r] = {workgroups, cost of one}, in launch order
+struct NsRun { long n; long cost; };
+constexpr int NS_FIXED = 8;                  // start and end of a tile, in reduction steps
+static NsDeal ns_deal(const NsRun* run, int runs)
+{
+    NsDeal d = {};
+    long total = 0, before = 0, at = 0;
+    for (int r = 0; r < runs; ++r) total += run[r].n * run[r].cost;
+    int x = 1;
+    for (int r = 0; r < runs; ++r) {
+        for (; x < 8; ++x) {
+            const long need = total * x / 8 - before;                     // border x falls into this run?
+            if (need > run[r].n * run[r].cost) break;
+            d.b[x] = (int)(at + (need + run[r].cost / 2) / run[r].cost);
+        }
+        before += run[r].n * run[r].cost; at += run[r].n;
+    }
+    for (; x < 9; ++x) d.b[x] = (int)at;
+    d.b[8] = (int)at;
+    return d;
+}
+static unsigned ns_deal_grid(const NsDeal& d)
+{
+    int most = 0;
+    for (int x = 0; x < 8; ++x) if (d.b[x + 1] - d.b[x] > most) most = d.b[x + 1] - d.b[x];
+    return 8u * most;
 }
 
 // `large` and `small`: the items of either way (capacity 4096), laid out against workspace `ws`.  Workspace: table | norm partials | matrices
@@ -625,6 +701,14 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
         a128 += (m + 127) / 128 * ((n + 127) / 128);
         if (p.large == 1 || m < p.shortest) p.shortest = m;
     }
+    // the longest reductions first: what starts last is short
+    for (long i = 1; i < p.large; ++i) {
+        const NsItem o = large[i];
+        long j = i;
+        auto side = [](const NsItem& t) { return t.rows < t.cols ? t.rows : t.cols; };
+        for (; j > 0 && side(large[j - 1]) < side(o); --j) large[j] = large[j - 1];
+        large[j] = o;
+    }
     p.tile_m = ab_env_int("SAUNET_NS_TILE", t128 <= 128 ? 64 : 128);
     p.tile_n = ab_env_int("SAUNET_NS_ATILE", a128 <= 128 ? 64 : 128);
     for (long i = 0; i < p.large; ++i) {
@@ -643,6 +727,19 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
         ns_cut(NS_GRAM, 1, p, tiles, gram, (int)p.large, large);
         ns_cut(NS_ONE, 1, p, tiles, sym, (int)p.large, large);
         ns_cut(NS_TWO, 2, p, tiles, sym, (int)p.large, large);
+        static thread_local NsRun run[2 * 4096];
+        for (int k = 0; k < NS_KINDS; ++k) {
+            int n = 0;
+            for (long i = 0; i < p.large; ++i) {
+                const NsSplit& sp = large[i].split[k];
+                const int steps = k == NS_GRAM ? gram[i] : sym[i];
+                if (sp.full) run[n++] = NsRun{sp.full, steps + NS_FIXED};
+                if (tiles[i] > sp.full && !sp.full) run[n++] = NsRun{(long)(tiles[i] - sp.full) * sp.s, steps / sp.s + NS_FIXED};
+            }
+            p.deal[k] = ns_deal(run, n);
+        }
+        for (long i = 0; i < p.large; ++i) run[i] = NsRun{(i + 1 < p.large ? large[i + 1].p_app : p.app) - large[i].p_app, sym[i] + NS_FIXED};
+        p.deal[NS_KINDS] = ns_deal(run, (int)p.large);
     }
     long at = 0;
     auto take = [&](long bytes) { const long r = at; at += (bytes + 255) / 256 * 256; return r; };
@@ -741,15 +838,19 @@ static bool ns_schedule(const saunet_ns_desc* d, bool compose, NsSchedule& w)
     return true;
 }
 
-template <class Core, typename T, bool MUON> static void ns_launch_apply(const saunet_ns_desc* d, const NsPlan& p, const NsItem* tab, const NsOp& o, const float* hyper, hipStream_t st)
+template <class Core, typename T, int MODE> static void ns_launch_apply(const saunet_ns_desc* d, const NsPlan& p, const NsItem* tab, const NsOp& o, const float* hyper, hipStream_t st)
 {
-    if (!o.last) hipLaunchKernelGGL((ns_apply_kernel<Core, T, 0>), dim3((unsigned)p.app), dim3(256), Core::LDS, st, tab, (int)p.large, o.q, o.xt, o.alpha, o.beta, hyper, 0);
-    else hipLaunchKernelGGL((ns_apply_kernel<Core, T, MUON ? 2 : 1>), dim3((unsigned)p.app), dim3(256), Core::LDS, st, tab, (int)p.large, o.q, o.xt, o.alpha, o.beta, hyper, d->adjust);
+    static DeviceOnce once;
+    if (once.first()) (void)hipFuncSetAttribute((const void*)ns_apply_kernel<Core, T, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
+    hipLaunchKernelGGL((ns_apply_kernel<Core, T, MODE>), dim3(ns_deal_grid(p.deal[NS_KINDS])), dim3(256), Core::LDS, st, tab, (int)p.large, o.q, o.xt, o.alpha, o.beta, hyper, d->adjust, p.deal[NS_KINDS]);
 }
 template <class Core> static void ns_launch_prod(const NsPlan& p, const NsItem* tab, const NsOp& o, hipStream_t st)
 {
     const int kind = o.gram ? NS_GRAM : o.ny == 2 ? NS_TWO : NS_ONE;
-    hipLaunchKernelGGL((ns_prod_kernel<Core>), dim3((unsigned)p.grid[kind], o.ny), dim3(256), Core::LDS, st, tab, (int)p.large, kind, o.pr);
+    static DeviceOnce once;
+    if (once.first()) (void)hipFuncSetAttribute((const void*)ns_prod_kernel<Core>, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
+    const unsigned dealt = ns_deal_grid(p.deal[kind]);
+    hipLaunchKernelGGL((ns_prod_kernel<Core>), dim3(dealt + (unsigned)(p.grid[kind] - p.deal[kind].b[8]), o.ny), dim3(256), Core::LDS, st, tab, (int)p.large, kind, o.pr, p.deal[kind], (int)dealt);
     if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(256), 0, st, tab, (int)p.large, kind, o.pr);
 }
 
@@ -790,8 +891,9 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, cons
     for (int i = 0; i < w.count; ++i) {
         const NsOp& o = w.op[i];
         if (o.apply) {
-            if (p.tile_n == 64) ns_launch_apply<NsCore64, T, MUON>(d, p, tab, o, hyper, st);
-            else ns_launch_apply<NsCore128, T, MUON>(d, p, tab, o, hyper, st);
+            constexpr int LAST = MUON ? 2 : 1;
+            if (p.tile_n == 64) o.last ? ns_launch_apply<NsCore64, T, LAST>(d, p, tab, o, hyper, st) : ns_launch_apply<NsCore64, T, 0>(d, p, tab, o, hyper, st);
+            else o.last ? ns_launch_apply<NsCore128, T, LAST>(d, p, tab, o, hyper, st) : ns_launch_apply<NsCore128, T, 0>(d, p, tab, o, hyper, st);
             SAUNET_CHECK_LAUNCH("ns_apply");
         } else {
             if (p.tile_m == 64) ns_launch_prod<NsCore64>(p, tab, o, st);

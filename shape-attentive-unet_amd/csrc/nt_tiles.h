@@ -52,7 +52,9 @@ __device__ __forceinline__ void nt_band(int t, int rows, int cols, int& r, int& 
 // float16 pairs: a row is a sequence of blocks of 32 elements, each 64 bytes of high parts followed by 64 bytes of low parts (x = hi + lo to 2^-24
 // of x).  hi hi + hi lo + lo hi in float32; what is dropped, lo lo, is below 2^-24 of |a| |b|.
 struct NtF16Pair {
-    static constexpr int RB = 128, KSUB = 2, PARTS = 2;
+    // the MFMA's adder cuts off instead of rounding, which over a long sum of one sign is a bias: 256 additions cost 6e-6 of the sum.  Every FLUSH stages the
+    // accumulators are added to a float32 total and start again.
+    static constexpr int RB = 128, KSUB = 2, PARTS = 2, FLUSH = 8;
     typedef f32x16 Acc;
     static __device__ __forceinline__ int chunk(int ks, int part, int half) { return part * 4 + ks * 2 + half; }
     static __device__ __forceinline__ void mma(const u32x4 (&a)[2], const u32x4 (&b)[2], Acc& c)
@@ -64,7 +66,7 @@ struct NtF16Pair {
 };
 // int8, 64 elements a stage
 struct NtI8 {
-    static constexpr int RB = 64, KSUB = 2, PARTS = 1;
+    static constexpr int RB = 64, KSUB = 2, PARTS = 1, FLUSH = 0;          // integer sums are exact
     typedef i32x16 Acc;
     static __device__ __forceinline__ int chunk(int ks, int, int half) { return ks * 2 + half; }
     static __device__ __forceinline__ void mma(const u32x4 (&a)[1], const u32x4 (&b)[1], Acc& c)
@@ -81,7 +83,7 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
     static constexpr int STAGE = (BM + BN) * RB, LDS = ST * STAGE, CPR = RB / 16, RPI = 1024 / RB;
     static constexpr int QA = BM * RB / 1024 / NW, QB = BN * RB / 1024 / NW, LPW = QA + QB;
     static_assert(QA * NW * 1024 == BM * RB && QB * NW * 1024 == BN * RB, "every wave requests whole instructions of one operand");
-    static_assert(ST >= 2 && ST <= 4 && (ST - 1) * LPW < 64 && Op::KSUB == 2, "vmcnt counts to 63");
+    static_assert(ST >= 2 && ST <= 8 && (ST - 1) * LPW < 64 && Op::KSUB == 2, "vmcnt counts to 63");
     typedef typename Op::Acc Acc;
 
     // 256 bytes of LDS answer at once: 2 (4) rows of the tile beside each other, so rows that agree modulo 2 (4) have to differ in their key
@@ -89,7 +91,7 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
 
     // a, b: first byte of the tile's first row at its first stage (uniform); arows, brows: rows that exist from there on (>= 1)
     static __device__ __forceinline__ void run(const char* a, unsigned lda, int arows, const char* b, unsigned ldb, int brows, int ksteps, unsigned char* smem,
-                                               Acc (&acc)[TM][TN])
+                                               Acc (&total)[TM][TN])
     {
         a = nt_uniform(a); b = nt_uniform(b);
         ksteps = __builtin_amdgcn_readfirstlane(ksteps);
@@ -114,6 +116,8 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
         };
         const int r0 = lane & 31, half = lane >> 5, k0 = key(r0);
         u32x4 fa[2][TM][Op::PARTS], fb[2][TN][Op::PARTS];
+        Acc part[TM][TN] = {};
+        Acc (&acc)[TM][TN] = Op::FLUSH ? part : total;
         auto read = [&](int s, int ks) {
             const unsigned char* st = smem + (s % ST) * STAGE;
             const unsigned char* sa = st + (wm * (BM / WGM) + r0) * RB;
@@ -135,10 +139,16 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
         };
         // this wave's LDS reads are in registers, its requests of all but the newest `young` stages have landed; then the workgroup's have
         auto settle = [&](int young) {
-            if (young >= 3 && ST > 3) nt_wait_barrier<(ST > 3 ? 3 : 0) * LPW>();
-            else if (young == 2 && ST > 2) nt_wait_barrier<(ST > 2 ? 2 : 0) * LPW>();
-            else if (young == 1) nt_wait_barrier<LPW>();
-            else nt_wait_barrier<0>();
+            switch (young) {
+            case 0: nt_wait_barrier<0>(); break;
+            case 1: nt_wait_barrier<LPW>(); break;
+            case 2: nt_wait_barrier<(ST > 2 ? 2 : 0) * LPW>(); break;
+            case 3: nt_wait_barrier<(ST > 3 ? 3 : 0) * LPW>(); break;
+            case 4: nt_wait_barrier<(ST > 4 ? 4 : 0) * LPW>(); break;
+            case 5: nt_wait_barrier<(ST > 5 ? 5 : 0) * LPW>(); break;
+            case 6: nt_wait_barrier<(ST > 6 ? 6 : 0) * LPW>(); break;
+            default: nt_wait_barrier<(ST > 7 ? 7 : 0) * LPW>(); break;
+            }
         };
         for (int s = 0; s < ST && s < ksteps; ++s) issue(s);
         settle((ksteps < ST ? ksteps : ST) - 1);
@@ -156,6 +166,12 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
             __builtin_amdgcn_sched_barrier(0);
             mma(1);
             __builtin_amdgcn_sched_barrier(0);
+            if (Op::FLUSH && ((s & (Op::FLUSH - 1)) == Op::FLUSH - 1 || s + 1 == ksteps)) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) { total[i][j] += part[i][j]; part[i][j] = Acc{}; }
+            }
         }
     }
 };

@@ -2247,12 +2247,8 @@ def ns_desc(rows, dtype, steps, coefficients, eps, adjust=0):
     """saunet_ns_desc over `rows`, a flat list of (src, dst, buf, ld_src, ld_dst, rows, cols) per matrix; keep the pair referenced until the call returns"""
     n = len(rows) // 7
     items = struct.pack("@" + "PPPqqii" * n, *rows)
-    d = L.NsDesc()
     buf = C.create_string_buffer(items, len(items))
-    d.item, d.count, d.dtype, d.steps, d.adjust = C.addressof(buf), n, dtype, steps, adjust
-    d.a, d.b, d.c = coefficients
-    d.eps = eps
-    return d, buf
+    return L.NsDesc(C.addressof(buf), n, dtype, steps, adjust, coefficients[0], coefficients[1], coefficients[2], eps), buf
 
 
 def ns_workspace(d, device):
@@ -2311,7 +2307,7 @@ def newton_schulz(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
         step = 0 if v.dim() == 2 else v.stride(0)
         for i in range(b):
             rows += (v.data_ptr() + i * step * size, out.data_ptr() + i * m * n * size, 0, ld, n, m, n)
-    with torch.cuda.device(ts[0].device):
+    with L.on(ts[0].device):
         for s0 in range(0, len(rows), 7 * L.NS_ITEMS_MAX):
             d, hold = ns_desc(rows[s0:s0 + 7 * L.NS_ITEMS_MAX], L.matrix_dtype_code(ts[0]), steps, coefficients, eps)
             ws = ns_workspace(d, ts[0].device)
@@ -2320,6 +2316,7 @@ def newton_schulz(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
 
 
 # ------------------------------------------------------------------------------------------------ int8 matrix products
+_MATRIX_CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 INT8_K_MAX = 131071          # 2^31 / 128^2: the integer sum of a product stays inside 32 bits
 
 
@@ -2378,13 +2375,15 @@ class Int8Rows:
 def _float_rows(x, who):
     """x [..., k] as (row view [rows, k] with unit column stride, k)"""
     _check_dev(x)
-    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    if x.dtype not in _MATRIX_CODES:
         raise RuntimeError("%s takes float32, bfloat16 or float16 rows, not %s" % (who, x.dtype))
     if x.dim() < 1 or not 1 <= x.shape[-1] <= INT8_K_MAX:
         raise RuntimeError("%s: rows of 1 to %d elements, got %s" % (who, INT8_K_MAX, tuple(x.shape)))
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError("%s serves inference: call it under torch.no_grad() or on a detached tensor" % who)
     k = x.shape[-1]
+    if x.dim() == 2 and x.is_contiguous():
+        return x, k
     v = x.detach().reshape(-1, k) if x.numel() else x.detach().new_empty(0, k)
     if v.shape[0] and ((k > 1 and v.stride(1) != 1) or (v.shape[0] > 1 and v.stride(0) < k)):
         v = v.contiguous()
@@ -2405,7 +2404,7 @@ def quantize_rows(x, affine=None, relu=False):
     data = torch.empty(rows, ld, dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     if rows:
-        with torch.cuda.device(x.device):
+        with L.on(x.device):
             L.call("saunet_quantize_rows", L.matrix_dtype_code(v), v.data_ptr(), v.stride(0) if rows > 1 else k, rows, k,
                    L.ptr(affine[0]) if affine is not None else None, L.ptr(affine[1]) if affine is not None else None, 1 if relu else 0,
                    data.data_ptr(), ld, scale.data_ptr(), L.stream())
@@ -2414,11 +2413,12 @@ def quantize_rows(x, affine=None, relu=False):
 
 def _int8_out(lead, rows, n, dtype, device, out):
     """-> (what the caller gets, its [rows, n] view)"""
-    if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    if dtype not in _MATRIX_CODES:
         raise RuntimeError("int8 products come as float32, bfloat16 or float16, not %s" % dtype)
+    lead = tuple(lead)
     if out is None:
         out = torch.empty(lead + (n,), dtype=dtype, device=device)
-        return out, out.view(rows, n)
+        return out, out if len(lead) == 1 else out.view(rows, n)
     if tuple(out.shape) != lead + (n,) or out.dtype != dtype or out.device != device:
         raise RuntimeError("out has to be %s of %s on %s" % (lead + (n,), dtype, device))
     v = out if out.dim() == 2 else out.view(rows, n)
@@ -2432,7 +2432,7 @@ def _int8_bias(bias, n, device):
         return None
     if bias.numel() != n or bias.device != device:
         raise RuntimeError("bias has to hold %d elements on %s" % (n, device))
-    return bias.detach().float().contiguous()
+    return bias if bias.dtype == torch.float32 and bias.is_contiguous() else bias.detach().float().contiguous()
 
 
 def matmul_int8(a, b, bias=None, relu=False, dtype=torch.bfloat16, out=None):
@@ -2449,17 +2449,30 @@ def matmul_int8(a, b, bias=None, relu=False, dtype=torch.bfloat16, out=None):
     y, yv = _int8_out(a.lead, rows, n, dtype, a.device, out)
     bias = _int8_bias(bias, n, a.device)
     if rows and n:
-        d = L.Int8Desc()
-        d.a, d.a_scale, d.lda, d.m = a.data.data_ptr(), a.scale.data_ptr(), a.data.shape[1], rows
-        d.b, d.b_scale, d.ldb, d.n, d.k = b.data.data_ptr(), b.scale.data_ptr(), b.data.shape[1], n, a.k
-        d.bias, d.y, d.ldy = L.ptr(bias), yv.data_ptr(), yv.stride(0) if rows > 1 else n
-        d.dtype, d.relu = L.matrix_dtype_code(yv), 1 if relu else 0
-        with torch.cuda.device(a.device):
+        d = L.Int8Desc(a.data.data_ptr(), a.scale.data_ptr(), a.data.shape[1], rows, b.data.data_ptr(), b.scale.data_ptr(), b.data.shape[1], n, a.k,
+                       L.ptr(bias), yv.data_ptr(), yv.stride(0) if rows > 1 else n, _MATRIX_CODES[dtype], 1 if relu else 0)
+        with L.on(a.device):
             L.call("saunet_matmul_int8", C.byref(d), L.stream())
     return y
 
 
 def linear_int8(x, w, bias=None, relu=False, dtype=None, out=None):
     """A linear layer over rows x [..., k] with an int8 weight ``w`` (Int8Rows [n, k]): the rows are quantised on the way (quantize_rows), the product is
-    matmul_int8's.  ``dtype``: the result's, x's by default."""
-    return matmul_int8(quantize_rows(x), w, bias, relu, x.dtype if dtype is None else dtype, out)
+    matmul_int8's -- the same result as the two calls, bit for bit.  ``dtype``: the result's, x's by default."""
+    v, k = _float_rows(x, "linear_int8")
+    if not isinstance(w, Int8Rows) or len(w.lead) != 1:
+        raise RuntimeError("linear_int8 takes an Int8Rows weight [n, k]")
+    if k != w.k or x.device != w.device:
+        raise RuntimeError("linear_int8: %s on %s does not meet %s on %s" % (tuple(x.shape), x.device, w.shape, w.device))
+    rows, n = v.shape[0], w.lead[0]
+    dtype = x.dtype if dtype is None else dtype
+    y, yv = _int8_out(x.shape[:-1], rows, n, dtype, x.device, out)
+    bias = _int8_bias(bias, n, x.device)
+    if rows and n:
+        d = L.Int8Desc(None, None, 0, rows, w.data.data_ptr(), w.scale.data_ptr(), w.data.shape[1], n, k,
+                       L.ptr(bias), yv.data_ptr(), yv.stride(0) if rows > 1 else n, _MATRIX_CODES[dtype], 1 if relu else 0)
+        need = rows * (_int8_stride(k) + 4)
+        with L.on(x.device):
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+            L.call("saunet_linear_int8", C.byref(d), _MATRIX_CODES[x.dtype], v.data_ptr(), v.stride(0) if rows > 1 else k, ws.data_ptr(), need, L.stream())
+    return y

@@ -206,6 +206,7 @@ _SIGS = {
     "saunet_muon_step": [C.POINTER(NsDesc), vp, vp, i64, vp],
     "saunet_quantize_rows": [i32, vp, i64, i64, i32, vp, vp, i32, vp, i64, vp, vp],
     "saunet_matmul_int8": [C.POINTER(Int8Desc), vp],
+    "saunet_linear_int8": [C.POINTER(Int8Desc), i32, vp, i64, vp, i64, vp],
     "saunet_bucket_copy": [C.POINTER(TensorList), i32, f32, vp],
 }
 ABI_VERSION = 4          # include/saunet_hip.h: SAUNET_ABI_VERSION (the struct layouts below mirror that header)
@@ -259,6 +260,24 @@ def stream():
     if _raw_stream is not None and _cur_device is not None:
         return _raw_stream(_cur_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE_CTX = _Here()
+
+
+def on(device):
+    """context that makes `device` the current one -- nothing to do, at no cost, where it already is"""
+    if _cur_device is not None and _cur_device() == device.index:
+        return _HERE_CTX
+    return torch.cuda.device(device)
 
 
 def ptr(t):

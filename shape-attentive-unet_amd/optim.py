@@ -297,7 +297,7 @@ class FusedMuon(_FusedBase):
                 rows += (p.grad.data_ptr(), p.data_ptr(), b.data_ptr(), n, n, m, n)
             if not rows:
                 continue
-            with torch.cuda.device(ps[0].device):
+            with L.on(ps[0].device):
                 for s0 in range(0, len(rows), 7 * L.NS_ITEMS_MAX):
                     d, hold = HF.ns_desc(rows[s0:s0 + 7 * L.NS_ITEMS_MAX], L.F32, g["ns_steps"], g["ns_coefficients"], g["eps"],
                                          1 if g["adjust_lr_fn"] == "match_rms_adamw" else 0)

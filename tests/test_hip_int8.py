@@ -87,6 +87,17 @@ def test_c_entries_refuse_before_any_launch():
     assert mm(k=131072, lda=131072, ldb=131072) == -1 and mm(a=None) == -1 and mm(y=None) == -1
     assert mm(dtype=9) == -2 and mm(a=4104) == -4 and mm(m=0) == 0
 
+    def lin(x_dtype=L.F32, x=4096, ldx=64, ws=4096, wsb=1 << 20, **kw):
+        d = L.Int8Desc()
+        v = dict(m=30, b=4096, b_scale=4096, ldb=64, n=5, k=33, bias=None, y=4096, ldy=5, dtype=L.F32, relu=0)
+        v.update(kw)
+        for name, val in v.items():
+            setattr(d, name, val)
+        return h.saunet_linear_int8(C.byref(d), x_dtype, x, ldx, ws, wsb, None)
+
+    assert lin(x_dtype=4) == -2 and lin(ldx=32) == -1 and lin(x=None) == -1 and lin(ws=None) == -1 and lin(wsb=30 * 68 - 1) == -1 and lin(ws=4104) == -1
+    assert lin(b=4100) == -4 and lin(y=None) == -1 and lin(m=0) == 0
+
 
 # ------------------------------------------------------------------------------------------------ quantisation
 @pytest.mark.gpu
@@ -206,7 +217,7 @@ def test_matmul_int8_into_slices_leaves_the_rest_alone(dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m", [1, 2, 5, 16, 17, 40, 300])
 def test_linear_int8(m, dtype):
-    for k, n in ((64, 48), (200, 130), (1024, 512), (2049, 77), (6000, 20)):
+    for k, n in ((1, 1), (3, 33), (4096, 20), (8191, 18), (20000, 17), (64, 48), (200, 130), (1024, 512), (2049, 77), (6000, 20)):
         x, w = rows(m, k, k + m, dtype), rows(n, k, 7)
         wr = HF.quantize_rows(w.cuda())
         bias = torch.randn(n, generator=torch.Generator().manual_seed(1))
@@ -217,6 +228,18 @@ def test_linear_int8(m, dtype):
             y = HF.linear_int8(x.cuda(), wr, bias=None if b is None else b.cuda(), relu=relu, dtype=od)
             ref, size = product64(q, s, wr.q.cpu(), wr.scale.cpu(), b, relu)
             check_product(y, ref, size, od or dtype)
+            two = HF.matmul_int8(HF.quantize_rows(x.cuda()), wr, bias=None if b is None else b.cuda(), relu=relu, dtype=od or dtype)
+            assert torch.equal(y, two)
+    x = rows(m, 72, 3, dtype)
+    x[0, 5] = float("nan")
+    x[m // 2, 7] = float("inf")
+    x[m - 1] = 0
+    y = HF.linear_int8(x.cuda(), HF.quantize_rows(rows(20, 72, 4).cuda()), dtype=torch.float32).cpu()
+    bad = ~torch.isfinite(x.float()).all(1)
+    assert y[bad].isnan().all() and not y[~bad].isnan().any() and (bad[m - 1] or not y[m - 1].any())
+    wide = rows(m, 300, 11, dtype).cuda()
+    wr = HF.quantize_rows(rows(24, 96, 6).cuda())
+    assert torch.equal(HF.linear_int8(wide[:, 101:197], wr, dtype=torch.float32), HF.linear_int8(wide[:, 101:197].contiguous(), wr, dtype=torch.float32))
     lead = rows(6 * m, 96, 5, dtype).view(2, 3, m, 96).cuda()
     wr = HF.quantize_rows(rows(24, 96, 6).cuda())
     assert torch.equal(HF.linear_int8(lead, wr, dtype=torch.float32), HF.linear_int8(lead.view(-1, 96), wr, dtype=torch.float32).view(2, 3, m, 24))
