@@ -177,6 +177,7 @@ typedef NtCore<NtF16Pair, 128, 128, 2, 2, 2> NsCore128;
 typedef NtCore<NtF16Pair, 64, 64, 2, 2, 4> NsCore64;
 constexpr int NS_SLOTS = 512;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4_t;
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 
 // Accumulator quad b of a thread: the four rows i .. i + 3 of column j, relative to the tile
 template <class Core> struct NsQuads {
@@ -192,28 +193,13 @@ template <class Core> struct NsQuads {
 #pragma unroll
         for (int b = 0; b < N; ++b) { int i, j; at(b, i, j); f(b, i, j); }
     }
-    // acc <- alpha acc + beta E over the tile at (i0, j0), E[j][i .. i + 3] a pair matrix of ld bytes a row.  All loads are under way before the first is
-    // used: a load behind another quad's stores would wait for them, sixteen memory latencies in a row (20 of the 50 us of such a launch).
-    static __device__ __forceinline__ void blend(f32x16 (&acc)[Core::TM][Core::TN], float alpha, float beta, const char* e, long ld, int i0, int j0, int mlim, int nlim)
-    {
-        f16x4_t h[N], l[N];
-        each([&](int b, int i, int j) {
-            i += i0; j += j0;
-            if (i < mlim && j < nlim) { const char* s = e + (long)j * ld + (i >> 5) * 128 + (i & 31) * 2; h[b] = *(const f16x4_t*)s; l[b] = *(const f16x4_t*)(s + 64); }
-        });
-        each([&](int b, int, int) {
-            f32x16& c = acc[b / (4 * Core::TN)][b / 4 % Core::TN];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) c[(b & 3) * 4 + r] = fmaf(alpha, c[(b & 3) * 4 + r], beta * ((float)h[b][r] + (float)l[b][r]));
-        });
-    }
     static __device__ __forceinline__ void quad(const f32x16 (&acc)[Core::TM][Core::TN], int b, float (&q)[4])
     {
 #pragma unroll
         for (int r = 0; r < 4; ++r) q[r] = acc[b / (4 * Core::TN)][b / 4 % Core::TN][(b & 3) * 4 + r];
     }
 };
-// four consecutive elements (row j, columns i .. i + 3) of a pair matrix with lda bytes a row
+// four consecutive elements (row j, columns i .. i + 3) of a pair matrix with ldb bytes a row
 __device__ __forceinline__ void ns_read4(const char* p, long ldb, int j, int i, float (&v)[4])
 {
     const char* s = p + (long)j * ldb + (i >> 5) * 128 + (i & 31) * 2;
@@ -221,34 +207,116 @@ __device__ __forceinline__ void ns_read4(const char* p, long ldb, int j, int i, 
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = (float)h[r] + (float)l[r];
 }
-// value (i .. i + 3, j) to row j of dt and to the rows i .. i + 3 of d
-__device__ __forceinline__ void ns_write4(char* dt, long ldt, char* d, long ldd, int i, int j, const float (&v)[4])
+__device__ __forceinline__ void ns_split4(const float (&v)[4], f16x4_t& h, f16x4_t& l)
 {
-    f16x4_t h, l;
 #pragma unroll
     for (int r = 0; r < 4; ++r) { const Pair s = ns_split(v[r]); h[r] = s.h; l[r] = s.l; }
-    char* p = dt + (long)j * ldt + (i >> 5) * 128 + (i & 31) * 2;
-    *(f16x4_t*)p = h; *(f16x4_t*)(p + 64) = l;
-    char* q = d + (long)i * ldd + (j >> 5) * 128 + (j & 31) * 2;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) { *(_Float16*)(q + r * ldd) = h[r]; *(_Float16*)(q + r * ldd + 64) = l[r]; }
 }
-// the same into a symmetric matrix: of a tile on the diagonal the upper part is dropped, so that the stored matrix is symmetric to the last bit.  An
-// antisymmetric rounding error would not shrink with a I + P as the error of S does: it grew six-fold a product (2e-5 of |X| after five steps).
-__device__ __forceinline__ void ns_write4_sym(char* d, long ld, bool diag, int i, int j, const float (&v)[4])
+// (i .. i + 3, j) of a tile of a symmetric matrix that lies on the diagonal: the part above it is dropped and the part below written to both halves, so
+// that the stored matrix is symmetric to the last bit.  An antisymmetric rounding error would not shrink with a I + P as the error of S does: it grew
+// six-fold a product (2e-5 of |X| after five steps).  put(row, col, pair)
+template <typename F> __device__ __forceinline__ void ns_both_halves(int i, int j, const float (&v)[4], F put)
 {
-    if (!diag || i >= j) { ns_write4(d, ld, d, ld, i, j, v); return; }
-    if (i + 3 < j) return;
 #pragma unroll
-    for (int r = 1; r < 4; ++r) {
+    for (int r = 0; r < 4; ++r) {
         if (i + r < j) continue;
         const Pair s = ns_split(v[r]);
-        char* p = d + (long)j * ld + ((i + r) >> 5) * 128 + ((i + r) & 31) * 2;
-        char* q = d + (long)(i + r) * ld + (j >> 5) * 128 + (j & 31) * 2;
-        *(_Float16*)p = s.h; *(_Float16*)(p + 64) = s.l;
-        *(_Float16*)q = s.h; *(_Float16*)(q + 64) = s.l;
+        put(j, i + r, s);
+        put(i + r, j, s);
     }
 }
+
+// A tile of pairs in LDS, between the accumulators and memory: rows of BM pairs, the 16-byte chunks of row r swapped by XOR with r so that a column of
+// them is spread over the banks.  Straight from the accumulators a store is 8 bytes in each of 32 rows, or 2 bytes in a row: such an epilogue was 20 000
+// of the 79 000 cycles of a 128 x 128 tile with a reduction of 1000.
+template <class Core> struct NsTile {
+    static constexpr int B = Core::BM, ROW = B * 4, CH = ROW / 16, RPI = 1024 / ROW, INSTR = B * ROW / 1024 / Core::NW;
+    static_assert(Core::BM == Core::BN && B * ROW <= Core::LDS, "the tile fits");
+    typedef NsQuads<Core> Quads;
+    static __device__ __forceinline__ unsigned char* at(unsigned char* smem, int row, int col)        // high part; the low part is 4 chunks on
+    {
+        return smem + row * ROW + ((((col >> 5) * 8 + ((col & 31) >> 3)) ^ (row & (CH - 1))) * 16) + (col & 7) * 2;
+    }
+    static __device__ __forceinline__ unsigned char* lo(unsigned char* smem, int row, int col)
+    {
+        return smem + row * ROW + ((((col >> 5) * 8 + 4 + ((col & 31) >> 3)) ^ (row & (CH - 1))) * 16) + (col & 7) * 2;
+    }
+    // acc <- alpha acc + beta E;  e: the tile of E^T, `rows` of its rows and `cols` of its columns (a multiple of 32) exist.  Ends with LDS in use.
+    static __device__ __forceinline__ void blend(f32x16 (&acc)[Core::TM][Core::TN], float alpha, float beta, const char* e, long ld, int rows, int cols, unsigned char* smem)
+    {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int last = cols >= B ? CH - 1 : cols / 4 - 1;
+        e = nt_uniform(e);
+        nt_wait_barrier<0>();                                              // everybody is done with what LDS held
+#pragma unroll
+        for (int q = 0; q < INSTR; ++q) {
+            const int k = q * Core::NW + wave, row = k * RPI + lane / CH, c = (lane % CH) ^ (row & (CH - 1));
+            nt_dma16(e, (unsigned)((row < rows ? row : rows - 1) * ld + (c < last ? c : last) * 16), (unsigned)(uintptr_t)smem + k * 1024);
+        }
+        nt_wait_barrier<0>();
+        Quads::each([&](int b, int i, int j) {
+            const f16x4_t h = *(const f16x4_t*)at(smem, j, i), l = *(const f16x4_t*)lo(smem, j, i);
+            f32x16& c = acc[b / (4 * Core::TN)][b / 4 % Core::TN];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) c[(b & 3) * 4 + r] = fmaf(alpha, c[(b & 3) * 4 + r], beta * ((float)h[r] + (float)l[r]));
+        });
+    }
+    static __device__ __forceinline__ void copy_out(char* d, long ld, int rows, int cols, unsigned char* smem)
+    {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < B * CH / Core::NT; ++k) {
+            const int id = k * Core::NT + threadIdx.x, row = id / CH, c = id % CH;
+            if (row < rows && (c >> 3) * 32 < cols) *(u32x4*)(d + row * ld + c * 16) = *(const u32x4*)(smem + row * ROW + (c ^ (row & (CH - 1))) * 16);
+        }
+    }
+    // the tile transposed, rows j of the accumulators' columns, to dt
+    static __device__ __forceinline__ void store_t(const f32x16 (&acc)[Core::TM][Core::TN], float alpha, char* dt, long ld, int rows, int cols, bool diag, unsigned char* smem)
+    {
+        nt_wait_barrier<0>();
+        Quads::each([&](int b, int i, int j) {
+            float q[4];
+            Quads::quad(acc, b, q);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) q[r] *= alpha;
+            if (diag) {
+                ns_both_halves(i, j, q, [&](int r, int c, const Pair& s) { *(_Float16*)at(smem, r, c) = s.h; *(_Float16*)lo(smem, r, c) = s.l; });
+            } else {
+                f16x4_t h, l;
+                ns_split4(q, h, l);
+                *(f16x4_t*)at(smem, j, i) = h; *(f16x4_t*)lo(smem, j, i) = l;
+            }
+        });
+        copy_out(dt, ld, rows, cols, smem);
+    }
+    // the tile itself to d: four lanes swap their 4 x 4 elements first, so that each holds four consecutive columns of one row
+    static __device__ __forceinline__ u32x2 swap4(u32x2 v)
+    {
+        const bool s = threadIdx.x & 1, t = threadIdx.x & 2;
+        const unsigned p0 = __builtin_amdgcn_update_dpp(0, v[0], 0xB1, 0xf, 0xf, true), p1 = __builtin_amdgcn_update_dpp(0, v[1], 0xB1, 0xf, 0xf, true);
+        const unsigned e0 = s ? __builtin_amdgcn_perm(v[0], p0, 0x07060302u) : __builtin_amdgcn_perm(p0, v[0], 0x05040100u);
+        const unsigned e1 = s ? __builtin_amdgcn_perm(v[1], p1, 0x07060302u) : __builtin_amdgcn_perm(p1, v[1], 0x05040100u);
+        const unsigned y = __builtin_amdgcn_update_dpp(0, t ? e0 : e1, 0x4E, 0xf, 0xf, true);
+        return t ? u32x2{y, e1} : u32x2{e0, y};
+    }
+    static __device__ __forceinline__ void store(const f32x16 (&acc)[Core::TM][Core::TN], float alpha, char* d, long ld, int rows, int cols, unsigned char* smem)
+    {
+        nt_wait_barrier<0>();
+        Quads::each([&](int b, int i, int j) {
+            float q[4];
+            Quads::quad(acc, b, q);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) q[r] *= alpha;
+            f16x4_t h, l;
+            ns_split4(q, h, l);
+            const int row = i + (j & 3), col = j & ~3;
+            *(u32x2*)at(smem, row, col) = swap4(__builtin_bit_cast(u32x2, h));
+            *(u32x2*)lo(smem, row, col) = swap4(__builtin_bit_cast(u32x2, l));
+        });
+        copy_out(d, ld, rows, cols, smem);
+    }
+};
+
 // tile t of the lower triangle of nt x nt tiles: (ti, tj), tj <= ti.  Walked in blocks of 8 x 8 tiles, so that the tiles in flight on one XCD share
 // eight row panels of either operand.
 __device__ __forceinline__ int ns_row(int t)          // row of t in a triangle walked row by row
@@ -293,7 +361,7 @@ template <class Core> __global__ __launch_bounds__(256, 2) void ns_prod_kernel(c
     // (deal ends at the first cut tile of a single matrix: its parts follow in launch order, behind a whole number of rounds)
     const int id = (int)blockIdx.x < tail ? ns_dealt(deal, blockIdx.x) : deal.b[8] + (int)blockIdx.x - tail;
     if (id < 0) return;
-    const NsProd p = pr.p[blockIdx.y];
+    const NsProd p = blockIdx.y ? pr.p[1] : pr.p[0];
     const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].split[kind].p; })];
     const NsView v(it);
     const NsSplit sl = it.split[kind];
@@ -313,27 +381,21 @@ template <class Core> __global__ __launch_bounds__(256, 2) void ns_prod_kernel(c
         Quads::each([&](int b, int, int) { float q[4]; Quads::quad(acc, b, q); *(f32x4*)(d + b * 1024) = f32x4{q[0], q[1], q[2], q[3]}; });
         return;
     }
-    const long ls = (long)v.mp * 4;
+    typedef NsTile<Core> Tile;
+    const long ls = (long)v.mp * 4, oij = (long)ti * T * ls + tj * T * 4, oji = (long)tj * T * ls + ti * T * 4;       // tile (ti, tj) and its mirror image
+    const int ri = v.mp - ti * T, rj = v.mp - tj * T;
     float alpha = p.alpha;
-    if (p.e >= 0) { Quads::blend(acc, alpha, p.beta, v.sym(p.e), ls, ti * T, tj * T, v.mp, v.mp); alpha = 1.f; }
-    if (p.f >= 0) Quads::blend(acc, alpha, p.gamma, v.sym(p.f), ls, ti * T, tj * T, v.mp, v.mp);
-    char* d = v.sym(p.d);
-    Quads::each([&](int b, int i, int j) {
-        i += ti * T; j += tj * T;
-        if (i >= v.mp || j >= v.mp) return;                                // whole 32 x 32 blocks
-        float q[4];
-        Quads::quad(acc, b, q);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) q[r] *= alpha;
-        ns_write4_sym(d, ls, ti == tj, i, j, q);
-    });
+    if (p.e >= 0) { Tile::blend(acc, alpha, p.beta, v.sym(p.e) + oji, ls, rj, ri, smem); alpha = 1.f; }
+    if (p.f >= 0) Tile::blend(acc, alpha, p.gamma, v.sym(p.f) + oji, ls, rj, ri, smem);
+    Tile::store_t(acc, alpha, v.sym(p.d) + oji, ls, rj, ri, ti == tj, smem);
+    if (ti != tj) Tile::store(acc, alpha, v.sym(p.d) + oij, ls, ri, rj, smem);
 }
 // one accumulator quad of a cut tile a thread; blockIdx.x = tile * quads + quad
 template <class Core> __global__ __launch_bounds__(256) void ns_finish_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr)
 {
     constexpr int T = Core::BM, N = NsQuads<Core>::N;
     const int id = blockIdx.x / N, q = blockIdx.x % N;
-    const NsProd p = pr.p[blockIdx.y];
+    const NsProd p = blockIdx.y ? pr.p[1] : pr.p[0];
     const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].split[kind].c; })];
     const NsSplit sl = it.split[kind];
     const int t = sl.full + id - sl.c;
@@ -362,7 +424,17 @@ template <class Core> __global__ __launch_bounds__(256) void ns_finish_kernel(co
 #pragma unroll
         for (int r = 0; r < 4; ++r) w[r] = fmaf(p.gamma, x[r], w[r]);
     }
-    ns_write4_sym(v.sym(p.d), ls, ti == tj, i, j, w);
+    char* d = v.sym(p.d);
+    if (ti == tj) {
+        ns_both_halves(i, j, w, [&](int r, int c, const Pair& e) { char* o = d + r * ls + (c >> 5) * 128 + (c & 31) * 2; *(_Float16*)o = e.h; *(_Float16*)(o + 64) = e.l; });
+        return;
+    }
+    f16x4_t h, l;
+    ns_split4(w, h, l);
+    char* o = d + j * ls + (i >> 5) * 128 + (i & 31) * 2;
+    *(f16x4_t*)o = h; *(f16x4_t*)(o + 64) = l;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) { char* m = d + (i + r) * ls + (j >> 5) * 128 + (j & 31) * 2; *(_Float16*)m = h[r]; *(_Float16*)(m + 64) = l[r]; }
 }
 
 __device__ __forceinline__ void ns_rates(const float* hyper, int rows, int cols, int adjust, float& keep, float& rate)
@@ -387,15 +459,13 @@ template <class Core, typename T, int MODE> __global__ __launch_bounds__(256, 2)
     const long ld = (long)v.mp * 4;
     Core::run(v.sym(q) + ti * B * ld, (unsigned)ld, v.mp - ti * B, v.xt(xt) + tj * B * ld, (unsigned)ld, v.np - tj * B, v.mp / 32, smem, acc);
     typedef NsQuads<Core> Quads;
-    Quads::blend(acc, alpha, beta, v.xt(xt), ld, ti * B, tj * B, v.mp, v.np);
+    typedef NsTile<Core> Tile;
+    const long oji = (long)tj * B * ld + ti * B * 4;
+    const int ri = v.mp - ti * B, rj = v.np - tj * B;
+    Tile::blend(acc, alpha, beta, v.xt(xt) + oji, ld, rj, ri, smem);
     if (MODE == 0) {
-        Quads::each([&](int b, int i, int j) {
-            i += ti * B; j += tj * B;
-            if (i >= v.mp || j >= v.np) return;                            // whole 32 x 32 blocks
-            float q[4];
-            Quads::quad(acc, b, q);
-            ns_write4(v.xt(xt ^ 1), ld, v.x, v.np * 4L, i, j, q);
-        });
+        Tile::store_t(acc, 1.f, v.xt(xt ^ 1) + oji, ld, rj, ri, false, smem);
+        Tile::store(acc, 1.f, v.x + (long)ti * B * v.np * 4 + tj * B * 4, v.np * 4L, ri, rj, smem);
         return;
     }
     const long si = v.tall ? 1 : it.ld_dst, sj = v.tall ? it.ld_dst : 1;
@@ -425,9 +495,10 @@ template <class Core, typename T, int MODE> __global__ __launch_bounds__(256, 2)
 // sound (an error grows by a^2 = 12 a step from 2^-53): one pass over the matrix for S, whose trace is the norm, one workgroup for W, one pass
 // for W X0.  The float64 rate of the vector units equals the float32 one, and both passes move little else than the matrix.
 constexpr int NSS_COLS = 64;                   // columns of the long side a workgroup stages at once
-struct NssItem { const void* src; void* dst; float* buf; double* ws; int ld_src, ld_dst, rows, cols, p, tiles; };       // tiles: of NSS_COLS, a workgroup
-constexpr int NSS_CHUNK = 64;
-struct NssItems { NssItem it[NSS_CHUNK]; };
+struct NssItem { const void* src; void* dst; float* buf; int ld_src, ld_dst, rows, cols, p, tiles; };       // tiles: of NSS_COLS, a workgroup
+constexpr int NSS_CHUNK = 80;
+struct NssItems { double* ws; NssItem it[NSS_CHUNK]; };       // ws: 1024 numbers for every workgroup and for every matrix
+__device__ __forceinline__ double* nss_ws(const NssItems& items, int i) { return items.ws + (long)(items.it[i].p + i) * 1024; }
 static_assert(sizeof(NssItems) <= 4032, "kernel arguments end at 4 KB");
 
 // columns c0 .. c0 + 63 of the matrix (long side) into s[32][68], zeros outside
@@ -459,7 +530,8 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void nss_gram
     __shared__ __attribute__((aligned(16))) float s_x[32][68];
     __shared__ double s_g[4][32][33];
     const int id = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, a0 = (tid >> 3 & 7) * 4, b0 = (tid & 7) * 4;
-    const NssItem it = items.it[ns_find(count, id, [&](int i) { return items.it[i].p; })];
+    const int which = ns_find(count, id, [&](int i) { return items.it[i].p; });
+    const NssItem it = items.it[which];
     double acc[4][4] = {};
     const int n = it.rows > it.cols ? it.rows : it.cols, first = (id - it.p) * it.tiles;
     for (int t = 0; t < it.tiles && (first + t) * NSS_COLS < n; ++t) {
@@ -485,7 +557,7 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void nss_gram
 #pragma unroll
         for (int j = 0; j < 4; ++j) s_g[wave][a0 + i][b0 + j] = acc[i][j];
     __syncthreads();
-    double* g = it.ws + (long)(1 + id - it.p) * 1024;
+    double* g = nss_ws(items, which) + (long)(1 + id - it.p) * 1024;
     for (int k = tid; k < 1024; k += 256) g[k] = (s_g[0][k >> 5][k & 31] + s_g[1][k >> 5][k & 31]) + (s_g[2][k >> 5][k & 31] + s_g[3][k >> 5][k & 31]);
 }
 
@@ -509,11 +581,12 @@ __global__ __launch_bounds__(512) void nss_poly_kernel(NssItems items, int steps
     __shared__ NssMat S, P, R, W;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = wave & 3;
     const NssItem it = items.it[blockIdx.x];
+    double* ws = nss_ws(items, blockIdx.x);
     const int n = it.rows > it.cols ? it.rows : it.cols, parts = (n + it.tiles * NSS_COLS - 1) / (it.tiles * NSS_COLS);
     for (int k = tid; k < 1024; k += 512) {
         double sum = 0.0;
 #pragma unroll 8
-        for (int p = 0; p < parts; ++p) sum += it.ws[(long)(1 + p) * 1024 + k];
+        for (int p = 0; p < parts; ++p) sum += ws[(long)(1 + p) * 1024 + k];
         S[k >> 5][k & 31] = sum;
     }
     __syncthreads();
@@ -547,15 +620,16 @@ __global__ __launch_bounds__(512) void nss_poly_kernel(NssItems items, int steps
         }
         __syncthreads();
     }
-    for (int k = tid; k < 1024; k += 512) it.ws[k] = W[k >> 5][k & 31];
+    for (int k = tid; k < 1024; k += 512) ws[k] = W[k >> 5][k & 31];
 }
 template <typename T, bool MUON> __global__ __launch_bounds__(256) void nss_apply_kernel(NssItems items, int count, const float* __restrict__ hyper, int adjust)
 {
     __shared__ __attribute__((aligned(16))) float s_x[32][68];
     __shared__ __attribute__((aligned(16))) double s_w[32][34];
     const int id = blockIdx.x, tid = threadIdx.x;
-    const NssItem it = items.it[ns_find(count, id, [&](int i) { return items.it[i].p; })];
-    for (int k = tid; k < 1024; k += 256) s_w[k >> 5][k & 31] = it.ws[k];
+    const int which = ns_find(count, id, [&](int i) { return items.it[i].p; });
+    const NssItem it = items.it[which];
+    for (int k = tid; k < 1024; k += 256) s_w[k >> 5][k & 31] = nss_ws(items, which)[k];
     const bool tall = it.rows > it.cols;
     const int m = tall ? it.cols : it.rows, n = tall ? it.rows : it.cols, first = (id - it.p) * it.tiles;
     float keep = 0.f, rate = 0.f;
@@ -613,7 +687,7 @@ static int ns_check(const saunet_ns_desc* d, const char* who)
 }
 
 // One call: the matrices with up to 32 rows go one way, the others the other way
-struct NsPlan { long small, large, norm, pack, tile, app, grid[NS_KINDS], cut[NS_KINDS], tab_at, part_at, bytes, shortest; int tile_m, tile_n; NsDeal deal[NS_KINDS + 1]; };
+struct NsPlan { long small, large, small_at, norm, pack, tile, app, grid[NS_KINDS], cut[NS_KINDS], tab_at, part_at, bytes, shortest; int tile_g, tile_m, tile_n; NsDeal deal[NS_KINDS + 1]; };
 
 static bool ns_is_small(const saunet_ns_desc* d, const saunet_ns_item& t)
 {
@@ -681,9 +755,9 @@ static unsigned ns_deal_grid(const NsDeal& d)
 // `large` and `small`: the items of either way (capacity 4096), laid out against workspace `ws`.  Workspace: table | norm partials | matrices
 static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* small, char* ws)
 {
-    static thread_local int tiles[4096], gram[4096], sym[4096];
+    static thread_local int tiles[2][4096], gram[4096], sym[4096];
     p = NsPlan();
-    long t128 = 0, a128 = 0;
+    long w128 = 0, a128 = 0, g128 = 0;
     for (int i = 0; i < d->count; ++i) {
         const saunet_ns_item& t = d->item[i];
         const long m = t.rows < t.cols ? t.rows : t.cols, n = t.rows < t.cols ? t.cols : t.rows;
@@ -697,8 +771,9 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
         }
         NsItem& o = large[p.large++];
         o.src = t.src; o.dst = t.dst; o.buf = (float*)t.buf; o.ld_src = (int)t.ld_src; o.ld_dst = (int)t.ld_dst; o.rows = t.rows; o.cols = t.cols;
-        t128 += (m + 127) / 128 * ((m + 127) / 128 + 1) / 2;
+        w128 += (m + 127) / 128 * ((m + 127) / 128 + 1) / 2 * ((m + 31) / 32);
         a128 += (m + 127) / 128 * ((n + 127) / 128);
+        g128 += (m + 127) / 128 * ((m + 127) / 128 + 1) / 2 * ((n + 31) / 32);
         if (p.large == 1 || m < p.shortest) p.shortest = m;
     }
     // the longest reductions first: what starts last is short
@@ -709,32 +784,33 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
         for (; j > 0 && side(large[j - 1]) < side(o); --j) large[j] = large[j - 1];
         large[j] = o;
     }
-    p.tile_m = ab_env_int("SAUNET_NS_TILE", t128 <= 128 ? 64 : 128);
+    p.tile_g = ab_env_int("SAUNET_NS_GTILE", g128 <= 1024 ? 64 : 128);
+    p.tile_m = ab_env_int("SAUNET_NS_TILE", w128 <= 2048 ? 64 : 128);
     p.tile_n = ab_env_int("SAUNET_NS_ATILE", a128 <= 128 ? 64 : 128);
     for (long i = 0; i < p.large; ++i) {
         NsItem& o = large[i];
         const long m = o.rows < o.cols ? o.rows : o.cols, n = o.rows < o.cols ? o.cols : o.rows, mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
-        const long tm = (m + p.tile_m - 1) / p.tile_m;
+        const long tm = (m + p.tile_m - 1) / p.tile_m, tg = (m + p.tile_g - 1) / p.tile_g;
         o.p_norm = (int)p.norm; o.p_pack = (int)p.pack; o.p_app = (int)p.app;
-        tiles[i] = (int)(tm * (tm + 1) / 2); gram[i] = (int)(np / 32); sym[i] = (int)(mp / 32);
+        tiles[0][i] = (int)(tg * (tg + 1) / 2); tiles[1][i] = (int)(tm * (tm + 1) / 2); gram[i] = (int)(np / 32); sym[i] = (int)(mp / 32);
         p.norm += (m * n + NS_NORM - 1) / NS_NORM;
         p.pack += ((mp + 63) / 64) * ((np + 63) / 64);
         p.app += ((m + p.tile_n - 1) / p.tile_n) * ((n + p.tile_n - 1) / p.tile_n);
-        p.tile += tiles[i];
+        p.tile += tiles[1][i] + tiles[0][i];
         if (p.norm > 0x3fffffff || p.pack > 0x3fffffff || p.app > 0x3fffffff || p.tile > 0x3ffffff) return set_error(SAUNET_BAD_SHAPE, "newton_schulz: the list is too large for one call");
     }
     if (p.large) {
-        ns_cut(NS_GRAM, 1, p, tiles, gram, (int)p.large, large);
-        ns_cut(NS_ONE, 1, p, tiles, sym, (int)p.large, large);
-        ns_cut(NS_TWO, 2, p, tiles, sym, (int)p.large, large);
+        ns_cut(NS_GRAM, 1, p, tiles[0], gram, (int)p.large, large);
+        ns_cut(NS_ONE, 1, p, tiles[1], sym, (int)p.large, large);
+        ns_cut(NS_TWO, 2, p, tiles[1], sym, (int)p.large, large);
         static thread_local NsRun run[2 * 4096];
         for (int k = 0; k < NS_KINDS; ++k) {
             int n = 0;
             for (long i = 0; i < p.large; ++i) {
                 const NsSplit& sp = large[i].split[k];
-                const int steps = k == NS_GRAM ? gram[i] : sym[i];
+                const int steps = k == NS_GRAM ? gram[i] : sym[i], all = tiles[k != NS_GRAM][i];
                 if (sp.full) run[n++] = NsRun{sp.full, steps + NS_FIXED};
-                if (tiles[i] > sp.full && !sp.full) run[n++] = NsRun{(long)(tiles[i] - sp.full) * sp.s, steps / sp.s + NS_FIXED};
+                if (all > sp.full && !sp.full) run[n++] = NsRun{(long)(all - sp.full) * sp.s, steps / sp.s + NS_FIXED};
             }
             p.deal[k] = ns_deal(run, n);
         }
@@ -749,12 +825,14 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
         long cut = 0;
         for (int k = 0; k < NS_KINDS; ++k) {
             const NsSplit& s = large[i].split[k];
-            const long c = s.s > 1 ? (long)(tiles[i] - s.full) * s.s * (k == NS_TWO ? 2 : 1) : 0;
+            const long side = k == NS_GRAM ? p.tile_g : p.tile_m;
+            const long c = s.s > 1 ? (long)(tiles[k != NS_GRAM][i] - s.full) * s.s * (k == NS_TWO ? 2 : 1) * side * side * 4 : 0;
             if (c > cut) cut = c;
         }
-        large[i].ws = ws + take(NsView::bytes(large[i].rows, large[i].cols) + cut * p.tile_m * p.tile_m * 4);
+        large[i].ws = ws + take(NsView::bytes(large[i].rows, large[i].cols) + cut);
     }
-    for (long i = 0; i < p.small; ++i) small[i].ws = (double*)(ws + take((long)(small[i].p + 1) * 1024 * 8));
+    p.small_at = at;
+    for (long i = 0; i < p.small; ++i) take((long)(small[i].p + 1) * 1024 * 8);
     p.bytes = at + 256;
     return SAUNET_OK;
 }
@@ -869,7 +947,9 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, cons
         NssItems ch;
         const int k = (int)(p.small - i < NSS_CHUNK ? p.small - i : NSS_CHUNK);
         int grid = 0;
+        ch.ws = (double*)(ws + p.small_at);
         for (int j = 0; j < k; ++j) { ch.it[j] = small[i + j]; ch.it[j].p = grid; grid += small[i + j].p; }
+        p.small_at += (long)(grid + k) * 1024 * 8;
         hipLaunchKernelGGL((nss_gram_kernel<T, MUON>), dim3(grid), dim3(256), 0, st, ch, k, hyper);
         hipLaunchKernelGGL(nss_poly_kernel, dim3(k), dim3(512), 0, st, ch, d->steps, (double)d->a, (double)d->b, (double)d->c, d->eps);
         hipLaunchKernelGGL((nss_apply_kernel<T, MUON>), dim3(grid), dim3(256), 0, st, ch, k, hyper, d->adjust);
@@ -896,7 +976,7 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, cons
             else o.last ? ns_launch_apply<NsCore128, T, LAST>(d, p, tab, o, hyper, st) : ns_launch_apply<NsCore128, T, 0>(d, p, tab, o, hyper, st);
             SAUNET_CHECK_LAUNCH("ns_apply");
         } else {
-            if (p.tile_m == 64) ns_launch_prod<NsCore64>(p, tab, o, st);
+            if ((o.gram ? p.tile_g : p.tile_m) == 64) ns_launch_prod<NsCore64>(p, tab, o, st);
             else ns_launch_prod<NsCore128>(p, tab, o, st);
             SAUNET_CHECK_LAUNCH("ns_prod");
         }
