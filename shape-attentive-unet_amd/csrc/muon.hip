@@ -175,6 +175,7 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_
 // 64 KB of LDS, two workgroups a CU.  (Twice the stages in one workgroup a CU brought nothing, also where a launch has fewer workgroups than CUs.)
 typedef NtCore<NtF16Pair, 128, 128, 2, 2, 2> NsCore128;
 typedef NtCore<NtF16Pair, 64, 64, 2, 2, 4> NsCore64;
+typedef NtCore<NtF16Pair, 128, 128, 4, 2, 2> NsCore128W;         // eight waves, for launches without a second workgroup for every CU (six 1000 x 1024 matrices 755 -> 701 us; 4096 x 4096 with it throughout 4219 -> 4699)
 constexpr int NS_SLOTS = 512;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4_t;
 typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
@@ -354,7 +355,7 @@ __device__ __forceinline__ int ns_dealt(const NsDeal& d, int id)
 struct NsProd { int a, b, e, f, d; float alpha, beta, gamma; };
 struct NsProds { NsProd p[2]; };
 
-template <class Core> __global__ __launch_bounds__(256, 2) void ns_prod_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr, NsDeal deal, int tail)
+template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) void ns_prod_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr, NsDeal deal, int tail)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     constexpr int T = Core::BM;
@@ -378,7 +379,7 @@ template <class Core> __global__ __launch_bounds__(256, 2) void ns_prod_kernel(c
     typedef NsQuads<Core> Quads;
     if (parts > 1) {
         float* d = v.part() + (((long)blockIdx.y * cut + t - sl.full) * parts + sp) * Quads::FLOATS + threadIdx.x * 4;
-        Quads::each([&](int b, int, int) { float q[4]; Quads::quad(acc, b, q); *(f32x4*)(d + b * 1024) = f32x4{q[0], q[1], q[2], q[3]}; });
+        Quads::each([&](int b, int, int) { float q[4]; Quads::quad(acc, b, q); *(f32x4*)(d + b * Core::NT * 4) = f32x4{q[0], q[1], q[2], q[3]}; });
         return;
     }
     typedef NsTile<Core> Tile;
@@ -391,7 +392,7 @@ template <class Core> __global__ __launch_bounds__(256, 2) void ns_prod_kernel(c
     if (ti != tj) Tile::store(acc, alpha, v.sym(p.d) + oij, ls, ri, rj, smem);
 }
 // one accumulator quad of a cut tile a thread; blockIdx.x = tile * quads + quad
-template <class Core> __global__ __launch_bounds__(256) void ns_finish_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr)
+template <class Core> __global__ __launch_bounds__(Core::NT) void ns_finish_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr)
 {
     constexpr int T = Core::BM, N = NsQuads<Core>::N;
     const int id = blockIdx.x / N, q = blockIdx.x % N;
@@ -404,7 +405,7 @@ template <class Core> __global__ __launch_bounds__(256) void ns_finish_kernel(co
     int ti, tj, i, j;
     ns_lower(t, nt, ti, tj);
     NsQuads<Core>::at(q, i, j);
-    const float* s = v.part() + (((long)blockIdx.y * cut + t - sl.full) * sl.s) * NsQuads<Core>::FLOATS + q * 1024 + threadIdx.x * 4;
+    const float* s = v.part() + (((long)blockIdx.y * cut + t - sl.full) * sl.s) * NsQuads<Core>::FLOATS + q * Core::NT * 4 + threadIdx.x * 4;
     f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int sp = 0; sp < sl.s; ++sp) { const f32x4 w = *(const f32x4*)(s + (long)sp * NsQuads<Core>::FLOATS); for (int r = 0; r < 4; ++r) c[r] += w[r]; }
@@ -445,7 +446,7 @@ __device__ __forceinline__ void ns_rates(const float* hyper, int rows, int cols,
 }
 
 // X <- alpha Q X + beta X.  MODE 0: back to X and the other X^T; 1: to the caller's matrix; 2: the Muon update of the caller's parameter
-template <class Core, typename T, int MODE> __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsItem* __restrict__ tab, int count, int q, int xt, float alpha, float beta, const float* __restrict__ hyper, int adjust, NsDeal deal)
+template <class Core, typename T, int MODE> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) void ns_apply_kernel(const NsItem* __restrict__ tab, int count, int q, int xt, float alpha, float beta, const float* __restrict__ hyper, int adjust, NsDeal deal)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     constexpr int B = Core::BM;
@@ -920,7 +921,7 @@ template <class Core, typename T, int MODE> static void ns_launch_apply(const sa
 {
     static DeviceOnce once;
     if (once.first()) (void)hipFuncSetAttribute((const void*)ns_apply_kernel<Core, T, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
-    hipLaunchKernelGGL((ns_apply_kernel<Core, T, MODE>), dim3(ns_deal_grid(p.deal[NS_KINDS])), dim3(256), Core::LDS, st, tab, (int)p.large, o.q, o.xt, o.alpha, o.beta, hyper, d->adjust, p.deal[NS_KINDS]);
+    hipLaunchKernelGGL((ns_apply_kernel<Core, T, MODE>), dim3(ns_deal_grid(p.deal[NS_KINDS])), dim3(Core::NT), Core::LDS, st, tab, (int)p.large, o.q, o.xt, o.alpha, o.beta, hyper, d->adjust, p.deal[NS_KINDS]);
 }
 template <class Core> static void ns_launch_prod(const NsPlan& p, const NsItem* tab, const NsOp& o, hipStream_t st)
 {
@@ -928,8 +929,8 @@ template <class Core> static void ns_launch_prod(const NsPlan& p, const NsItem* 
     static DeviceOnce once;
     if (once.first()) (void)hipFuncSetAttribute((const void*)ns_prod_kernel<Core>, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
     const unsigned dealt = ns_deal_grid(p.deal[kind]);
-    hipLaunchKernelGGL((ns_prod_kernel<Core>), dim3(dealt + (unsigned)(p.grid[kind] - p.deal[kind].b[8]), o.ny), dim3(256), Core::LDS, st, tab, (int)p.large, kind, o.pr, p.deal[kind], (int)dealt);
-    if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(256), 0, st, tab, (int)p.large, kind, o.pr);
+    hipLaunchKernelGGL((ns_prod_kernel<Core>), dim3(dealt + (unsigned)(p.grid[kind] - p.deal[kind].b[8]), o.ny), dim3(Core::NT), Core::LDS, st, tab, (int)p.large, kind, o.pr, p.deal[kind], (int)dealt);
+    if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(Core::NT), 0, st, tab, (int)p.large, kind, o.pr);
 }
 
 template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
@@ -976,7 +977,9 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, cons
             else o.last ? ns_launch_apply<NsCore128, T, LAST>(d, p, tab, o, hyper, st) : ns_launch_apply<NsCore128, T, 0>(d, p, tab, o, hyper, st);
             SAUNET_CHECK_LAUNCH("ns_apply");
         } else {
+            const int kind = o.gram ? NS_GRAM : o.ny == 2 ? NS_TWO : NS_ONE;
             if ((o.gram ? p.tile_g : p.tile_m) == 64) ns_launch_prod<NsCore64>(p, tab, o, st);
+            else if (p.grid[kind] * o.ny <= NS_SLOTS / 2) ns_launch_prod<NsCore128W>(p, tab, o, st);
             else ns_launch_prod<NsCore128>(p, tab, o, st);
             SAUNET_CHECK_LAUNCH("ns_prod");
         }
