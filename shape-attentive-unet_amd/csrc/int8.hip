@@ -93,7 +93,8 @@ template <int G> __device__ __forceinline__ unsigned q_top(unsigned top)
 }
 
 // G lanes a row, NV vectors a lane kept in registers (k <= G * NV * V, 16-byte aligned rows); NV == 0: any k and alignment, the row is read twice
-template <typename T, int G, int NV> __global__ __launch_bounds__(256) void quantize_rows_kernel(QArgs a)
+// PRO: scale / shift / relu in front (16-byte aligned vectors where NV > 0)
+template <typename T, int G, int NV, bool PRO> __global__ __launch_bounds__(256) void quantize_rows_kernel(QArgs a)
 {
     constexpr int V = QElem<T>::V;
     const int lane = threadIdx.x % G;
@@ -117,9 +118,20 @@ template <typename T, int G, int NV> __global__ __launch_bounds__(256) void quan
             const int c = (i * G + lane) * V;
             QElem<T>::unpack(v[i], f[i]);
             if (c < a.k && c + V > a.k) for (int j = 0; j < V; ++j) f[i][j] = c + j < a.k ? QElem<T>::load(x + c + j) : 0.f;
-            if (a.scale || a.relu)
+            if (PRO && c + V <= a.k) {
+                if (a.scale)
 #pragma unroll
+                    for (int h = 0; h < V; h += 4) {
+                        const f32x4 sc = *(const f32x4*)(a.scale + c + h), sh = *(const f32x4*)(a.shift + c + h);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) f[i][h + j] = fmaf(f[i][h + j], sc[j], sh[j]);
+                    }
+                if (a.relu)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) f[i][j] = f[i][j] < 0.f ? 0.f : f[i][j];
+            } else if (PRO) {
                 for (int j = 0; j < V; ++j) if (c + j < a.k) f[i][j] = pro(f[i][j], c + j);
+            }
 #pragma unroll
             for (int j = 0; j < V; ++j) { const unsigned b = __float_as_uint(f[i][j]) & 0x7fffffffu; top = b > top ? b : top; }
         }
@@ -151,10 +163,10 @@ template <typename T, int G, int NV> __global__ __launch_bounds__(256) void quan
 
 // Lanes a row: as few as hold it in one or two vectors each, so that a wave keeps several short rows in flight; a workgroup to a row where there are
 // fewer rows than would fill the card with a wave each
-template <typename T> static void q_launch(const QArgs& a, hipStream_t st)
+template <typename T, bool PRO> static void q_launch(const QArgs& a, hipStream_t st)
 {
     constexpr int V = QElem<T>::V;
-#define Q_GO(G, NV) hipLaunchKernelGGL((quantize_rows_kernel<T, G, NV>), dim3((unsigned)((a.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, st, a)
+#define Q_GO(G, NV) hipLaunchKernelGGL((quantize_rows_kernel<T, G, NV, PRO>), dim3((unsigned)((a.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, st, a)
     const bool few = a.rows <= 1024 && a.k > 128 * V;
     if (!a.vec || a.k > 2048 * V) { if (a.rows <= 4096 && a.k > 256) Q_GO(256, 0); else Q_GO(64, 0); }
     else if (a.k <= 16 * V) Q_GO(16, 1);
@@ -449,11 +461,10 @@ int saunet_quantize_rows(int dtype, const void* x, int64_t ldx, int64_t rows, in
     if ((uintptr_t)q & 15) return set_error(SAUNET_BAD_ALIGN, "quantize_rows: q has to lie on a 16-byte border");
     if (rows > 0x7fffffffL * 4) return set_error(SAUNET_BAD_SHAPE, "quantize_rows: %lld rows", (long long)rows);
     const int size = dtype == SAUNET_F32 ? 4 : 2;
-    QArgs a = {x, ldx, rows, k, scale, shift, relu, (signed char*)q, ldq, s, !((uintptr_t)x & 15) && !(ldx * size & 15)};
+    QArgs a = {x, ldx, rows, k, scale, shift, relu, (signed char*)q, ldq, s, !(((uintptr_t)x | (uintptr_t)scale | (uintptr_t)shift) & 15) && !(ldx * size & 15)};
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == SAUNET_F32) q_launch<float>(a, st);
-    else if (dtype == SAUNET_BF16) q_launch<u16>(a, st);
-    else q_launch<_Float16>(a, st);
+    if (scale || relu) dtype == SAUNET_F32 ? q_launch<float, true>(a, st) : dtype == SAUNET_BF16 ? q_launch<u16, true>(a, st) : q_launch<_Float16, true>(a, st);
+    else dtype == SAUNET_F32 ? q_launch<float, false>(a, st) : dtype == SAUNET_BF16 ? q_launch<u16, false>(a, st) : q_launch<_Float16, false>(a, st);
     SAUNET_CHECK_LAUNCH("quantize_rows");
     return SAUNET_OK;
 }

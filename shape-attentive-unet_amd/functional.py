@@ -291,6 +291,16 @@ def folded_conv_bn(weight, bias, bn, transposed, dtype):
     return INFER.get(srcs + [_DTYPE_TOKEN[dtype]], build)
 
 
+def folded_conv_bn_int8(weight, bn):
+    """Inference: (w' as Int8Rows, b') of a 1x1 convolution with the BatchNorm behind it folded in, cached like folded_conv_bn"""
+    def build():
+        p = bn_finalize(None, 1, bn.weight, bn.bias, bn.running_mean, bn.running_var, bn.momentum, bn.eps, False)
+        return quantize_rows(weight.detach().flatten(1).float() * p.scale.view(-1, 1)), p.shift.clone()
+
+    return INFER.get([weight, bn.weight, bn.bias, bn.running_mean, bn.running_var, _INT8_TOKEN], build)
+
+
+_INT8_TOKEN = torch.zeros(0)
 _DTYPE_TOKEN = {torch.float32: torch.zeros(0), torch.bfloat16: torch.zeros(0)}    # distinct key objects per storage dtype
 
 
@@ -2088,11 +2098,18 @@ class _DenseBlock(torch.autograd.Function):
         return (dx0, None, None) + tuple(grads) + (None,) * (4 * nl)
 
 
-def dense_block_infer(x0, layers):
+# int8 conv1 of a dense layer (dense_block_infer): on maps of at most so many pixels, from so many input channels.  The products win everywhere, but the
+# pass that quantises the activations reads and writes them once more.  us, bf16 against int8 (128 output channels):
+#   pixels   256: 512 channels  9.0 / 7.6, 992 15.1 / 10.1      1024: 256 channels 6.1 / 7.5, 992 15.3 / 10.8
+#   pixels  4096: 256 channels  6.2 / 7.8, 512 9.2 / 9.1, 992 15.3 / 12.4      8192: 512 channels 9.5 / 11.2      32768: 1024 channels 28 / 34
+INT8_PIXELS_MAX, INT8_CHANNELS_MIN = 4096, 448
+
+
+def dense_block_infer(x0, layers, int8=False):
     """Inference form of a DenseNet block: per layer ONE prologue'd 1x1 conv whose weights carry norm2 (w' = w * s2, bias = t2, ReLU in the
     epilogue -> the 3x3 conv needs no prologue) and one plain 3x3 conv writing its 32 channels into the concat buffer.  norm1 cannot be
     folded (a ReLU sits between it and conv1 and every layer has its own gamma/beta over the shared concat channels): it stays the operand
-    prologue, with its eval-mode coefficients cached (bn_finalize)."""
+    prologue, with its eval-mode coefficients cached (bn_finalize).  int8: conv1 as an int8 product (pointwise_int8) where that is faster."""
     x0 = nhwc(x0)
     n, c0, h, w = x0.shape
     growth = layers[0].conv2.weight.shape[0]
@@ -2102,17 +2119,21 @@ def dense_block_infer(x0, layers):
     cin = c0
     for m in layers:
         p1 = bn_finalize(None, 1, m.norm1.weight, m.norm1.bias, m.norm1.running_mean, m.norm1.running_var, m.norm1.momentum, m.norm1.eps, False)
-        w1p, b1 = folded_conv_bn(m.conv1.weight, None, m.norm2, False, x0.dtype)
-        a2 = conv_forward_raw(buf[:, :cin], m.conv1.weight, b1, 1, 0, pro=(p1.scale, p1.shift, True), act_relu=True, packed=w1p)
+        if int8 and n * h * w <= INT8_PIXELS_MAX and cin >= INT8_CHANNELS_MIN:
+            w1q, b1 = folded_conv_bn_int8(m.conv1.weight, m.norm2)
+            a2 = pointwise_int8(buf[:, :cin], w1q, b1, relu=True, affine=(p1.scale, p1.shift), affine_relu=True)
+        else:
+            w1p, b1 = folded_conv_bn(m.conv1.weight, None, m.norm2, False, x0.dtype)
+            a2 = conv_forward_raw(buf[:, :cin], m.conv1.weight, b1, 1, 0, pro=(p1.scale, p1.shift, True), act_relu=True, packed=w1p)
         conv_forward_raw(a2, m.conv2.weight, None, 1, 1, out=buf[:, cin:cin + growth])
         cin += growth
     return buf
 
 
-def dense_block(x0, layers, training):
-    """layers: list of modules with norm1, conv1, norm2, conv2.  Returns (concat buffer, its channel statistics)."""
+def dense_block(x0, layers, training, int8=False):
+    """layers: list of modules with norm1, conv1, norm2, conv2.  Returns (concat buffer, its channel statistics).  int8: see dense_block_infer."""
     if not training and not torch.is_grad_enabled() and x0.is_cuda:
-        return dense_block_infer(x0, layers), None
+        return dense_block_infer(x0, layers, int8), None
     eps = {float(m.norm1.eps) for m in layers}       # (norm2 of a layer normalises its own 128 channels: its eps / momentum travel per layer)
     if len(eps) > 1:
         # the block shares one set of normalised-input rows (invstd computed once per concat channel) between all its norm1 layers, forward and
@@ -2471,8 +2492,26 @@ def linear_int8(x, w, bias=None, relu=False, dtype=None, out=None):
     if rows and n:
         d = L.Int8Desc(None, None, 0, rows, w.data.data_ptr(), w.scale.data_ptr(), w.data.shape[1], n, k,
                        L.ptr(bias), yv.data_ptr(), yv.stride(0) if rows > 1 else n, _MATRIX_CODES[dtype], 1 if relu else 0)
-        need = rows * (_int8_stride(k) + 4)
+        need = rows * (_int8_stride(k) + 4) if rows > 1 or k > 16384 else 0              # one row needs none
         with L.on(x.device):
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-            L.call("saunet_linear_int8", C.byref(d), _MATRIX_CODES[x.dtype], v.data_ptr(), v.stride(0) if rows > 1 else k, ws.data_ptr(), need, L.stream())
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+            L.call("saunet_linear_int8", C.byref(d), _MATRIX_CODES[x.dtype], v.data_ptr(), v.stride(0) if rows > 1 else k, L.ptr(ws), need, L.stream())
+    return y
+
+
+def pointwise_int8(x, w, bias=None, relu=False, affine=None, affine_relu=False, out=None):
+    """A 1x1 convolution in int8: x [N, C, H, W] (channels_last, channel slices too; anything else is converted), ``w`` Int8Rows [Cout, C].  Every pixel
+    is a row of quantize_rows (``affine``, ``affine_relu``: a BatchNorm + ReLU in front), the product is matmul_int8's.  Returns x's dtype in
+    channels_last memory, or fills ``out``, a channel slice of a channels_last buffer."""
+    x = nhwc(x)
+    n, c, h, wd = x.shape
+    if not isinstance(w, Int8Rows) or len(w.lead) != 1 or w.k != c:
+        raise RuntimeError("pointwise_int8: the weight is Int8Rows [Cout, %d]" % c)
+    ld = ld_of(x) if c > 1 or n * h * wd > 1 else 1
+    rows = quantize_rows(x.detach().as_strided((n * h * wd, c), (ld, 1)) if not (torch.is_grad_enabled() and x.requires_grad) else x, affine, affine_relu)
+    cout = w.lead[0]
+    y = new_act(n, cout, h, wd, x.dtype, x.device) if out is None else out
+    if out is not None and (tuple(out.shape) != (n, cout, h, wd) or out.dtype != x.dtype or nhwc(out) is not out):
+        raise RuntimeError("pointwise_int8: out has to be a channels_last [%d, %d, %d, %d] of %s" % (n, cout, h, wd, x.dtype))
+    matmul_int8(rows, w, bias, relu, x.dtype, out=y.as_strided((n * h * wd, cout), (ld_of(y) if n * h * wd > 1 else cout, 1)))
     return y

@@ -285,13 +285,15 @@ class _DenseLayer(nn.Module):
 
 
 class _DenseBlock(nn.ModuleDict):
+    int8 = False             # SAUNet.int8_inference
+
     def __init__(self, num_layers, cin, growth=32, bn_size=4):
         super().__init__()
         for i in range(num_layers):
             self["denselayer%d" % (i + 1)] = _DenseLayer(cin + i * growth, growth, bn_size)
 
     def forward(self, x, with_stats=False):
-        buf, stats = HF.dense_block(x, list(self.values()), self.training)
+        buf, stats = HF.dense_block(x, list(self.values()), self.training, self.int8)
         return (buf, stats) if with_stats else buf
 
     def total_channels(self):
@@ -421,6 +423,15 @@ class SAUNet(nn.Module):
         if mode != self.training:
             HF._EVAL_BN.clear()       # eval-mode BatchNorm coefficients are cached per module: drop them on every mode switch
         return super().train(mode)
+
+    def int8_inference(self, enabled=True):
+        """Run the 1x1 convolutions of the dense layers as int8 products (weights by output channel, activations by pixel, quantised on the way) in
+        eval mode without gradients, where that is faster (HF.INT8_PIXELS_MAX, HF.INT8_CHANNELS_MIN: at batch size 1 most of the third and all of the
+        fourth dense block).  Off by default; training and gradients are never affected.  Returns self."""
+        for m in self.modules():
+            if isinstance(m, _DenseBlock):
+                m.int8 = bool(enabled)
+        return self
 
     def _prep_input(self, x):
         """float image [B,3,H,W] (any layout) -> NHWC, 8 channels (5 zero), compute dtype."""

@@ -212,6 +212,7 @@ def build_parser():
     p.add_argument("--synthetic", type=int, default=64, help="number of synthetic training slices (no ACDC data mounted)")
     p.add_argument("--size", type=int, default=256)
     p.add_argument("--val_slices", type=int, default=8)
+    p.add_argument("--val_int8", action="store_true", help="validate with the dense layers' 1x1 convolutions in int8 (SAUNet.int8_inference)")
     p.add_argument("--augment", action="store_true", help="train on raw ragged slices augmented on the GPU (augment.DeviceAugmenter: the loader's "
                    "crop/flip/rotate/gamma/z-score/elastic chain, train.py:236 + data/ac17_dataloader.py)")
     return p
@@ -227,6 +228,7 @@ def main(argv=None):
     unet = SAUNet(num_classes=args.num_class).to(device)
     if args.weights_unet:
         unet.load_state_dict(torch.load(args.weights_unet, map_location="cpu"), strict=False)
+    unet.int8_inference(args.val_int8)
     dp.broadcast_parameters(unet)
     sm = SegmentationModule(DualLoss(mode="train"), unet, args.num_class)
     optimizers = optim.create_optimizers(unet, args.optimizer, args.lr_encoder, args.beta1, args.weight_decay)
