@@ -348,7 +348,7 @@ def test_dense_block_int8_follows_its_definition(monkeypatch):
 
 
 @pytest.mark.gpu
-def test_saunet_int8_inference_switch():
+def test_saunet_int8_inference_switch(monkeypatch):
     import saunet_amd
     from saunet_amd import data
     saunet_amd.set_compute_dtype(torch.bfloat16)
@@ -367,14 +367,15 @@ def test_saunet_int8_inference_switch():
         out = net(img)[0]
         return seen[0], out
 
-    L.load().saunet_launch_log()
+    calls, inner = [], HF.pointwise_int8
+    monkeypatch.setattr(HF, "pointwise_int8", lambda *a, **k: calls.append(1) or inner(*a, **k))
     with torch.no_grad():
         plain = run()[0].clone()
-        assert b"quantize_rows" not in L.load().saunet_launch_log()
+        assert not calls
         net.int8_inference()
         y, out = run()
         y = y.clone()
-        assert b"quantize_rows" in L.load().saunet_launch_log()
+        assert len(calls) == 2 + 18 + 16                # layers of the second (128 + 32 i), third (256 + 32 i) and fourth (512 + 32 i) block with 448 channels or more
         assert torch.isfinite(out).all() and not torch.equal(y, plain)
         assert torch.equal(run()[0], y)
         net.int8_inference(False)
