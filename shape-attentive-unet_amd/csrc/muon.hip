@@ -31,7 +31,7 @@ struct NsItem {            // one matrix, as the host lays it out
 constexpr int NS_CHUNK = 36;                 // of them are kernel arguments
 struct NsItems { NsItem it[NS_CHUNK]; };
 static_assert(sizeof(NsItems) <= 4064, "kernel arguments end at 4 KB");
-constexpr int NS_NORM = 8192;                // elements a workgroup of the norm pass takes
+constexpr int NS_NORM = 4096;                // elements a workgroup of the norm pass takes
 
 enum { NS_X = -1, NS_A = 0, NS_P, NS_R, NS_Q0, NS_Q1, NS_NSYM };
 struct NsView {
@@ -102,18 +102,22 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_norm_
     float h[5] = {0.f, 0.f, 0.f, 0.f, 1.f};
     if (MUON) for (int i = 0; i < 5; ++i) h[i] = hyper[i];
     double sum = 0.0;
-    auto one = [&](long e, float g) {
-        float u = g;
-        if (MUON) { const float b = ns_momentum(g, it.buf[e], h); it.buf[e] = b; u = ns_update(g, b, h); }
+    constexpr int EACH = NS_NORM / 256;
+    float g[EACH], old[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        const long e = e0 + k * 256 + threadIdx.x;
+        const long r = it.ld_src == it.cols ? 0 : e / it.cols;
+        g[k] = old[k] = 0.f;
+        if (e < total) { g[k] = ns_load((const T*)it.src + (r * (it.ld_src - it.cols) + e)); if (MUON) old[k] = it.buf[e]; }
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        const long e = e0 + k * 256 + threadIdx.x;
+        if (e >= total) break;
+        float u = g[k];
+        if (MUON) { const float b = ns_momentum(g[k], old[k], h); it.buf[e] = b; u = ns_update(g[k], b, h); }
         sum += (double)u * (double)u;
-    };
-    if (it.ld_src == it.cols) {
-        for (int k = threadIdx.x; k < NS_NORM; k += 256) { const long e = e0 + k; if (e < total) one(e, ns_load((const T*)it.src + e)); }
-    } else {
-        for (int k = threadIdx.x; k < NS_NORM; k += 256) {
-            const long e = e0 + k;
-            if (e < total) { const long r = e / it.cols; one(e, ns_load((const T*)it.src + r * it.ld_src + (e - r * it.cols))); }
-        }
     }
     sum = wave_sum(sum);
     if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
@@ -129,6 +133,18 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_
     const int tid = threadIdx.x, id = blockIdx.x;
     const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].p_pack; })];
     const NsView v(it);
+    float h[5] = {0.f, 0.f, 0.f, 0.f, 1.f};
+    if (MUON) for (int i = 0; i < 5; ++i) h[i] = hyper[i];
+    // tiles in the caller's orientation: r along its rows, c along its columns; the elements are on their way while the norm is summed
+    const int rp = v.tall ? v.np : v.mp, cp = v.tall ? v.mp : v.np, tc = (cp + 63) / 64, t = id - it.p_pack;
+    const int r0 = t / tc * 64, c0 = t % tc * 64;
+    float g[16], buf[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const int r = r0 + k * 4 + (tid >> 6), c = c0 + (tid & 63);
+        g[k] = buf[k] = 0.f;
+        if (r < it.rows && c < it.cols) { g[k] = ns_load((const T*)it.src + (long)r * it.ld_src + c); if (MUON) buf[k] = it.buf[(long)r * it.cols + c]; }
+    }
     const int nblk = (int)(((long)it.rows * it.cols + NS_NORM - 1) / NS_NORM);
     double sum = 0.0;
     for (int i = tid; i < nblk; i += 256) sum += part[it.p_norm + i];
@@ -137,20 +153,11 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_
     __syncthreads();
     const double norm = sqrt(((s_sum[0] + s_sum[1]) + s_sum[2]) + s_sum[3]);
     const double inv = (double)sx / (norm <= (double)eps ? (double)eps : norm);      // a NaN norm stays NaN
-    float h[5] = {0.f, 0.f, 0.f, 0.f, 1.f};
-    if (MUON) for (int i = 0; i < 5; ++i) h[i] = hyper[i];
-    // tiles in the caller's orientation: r along its rows, c along its columns
-    const int rp = v.tall ? v.np : v.mp, cp = v.tall ? v.mp : v.np, tc = (cp + 63) / 64, t = id - it.p_pack;
-    const int r0 = t / tc * 64, c0 = t % tc * 64;
-    for (int k = tid; k < 64 * 64; k += 256) {
-        const int r = r0 + (k >> 6), c = c0 + (k & 63);
-        float u = 0.f;
-        if (r < it.rows && c < it.cols) {
-            u = ns_load((const T*)it.src + (long)r * it.ld_src + c);
-            if (MUON) u = ns_update(u, it.buf[(long)r * it.cols + c], h);
-            u = (float)((double)u * inv);
-        }
-        s_t[k >> 6][k & 63] = u;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        // (a padding element is zero, not zero times a scale that may be NaN)
+        const int r = r0 + k * 4 + (tid >> 6), c = c0 + (tid & 63);
+        s_t[k * 4 + (tid >> 6)][tid & 63] = r < it.rows && c < it.cols ? (float)((double)(MUON ? ns_update(g[k], buf[k], h) : g[k]) * inv) : 0.f;
     }
     __syncthreads();
     // 8 consecutive elements a thread: 16 bytes of high and of low parts; along[] runs along the caller's rows, across[] along its columns
@@ -271,26 +278,7 @@ template <class Core> struct NsTile {
             if (row < rows && (c >> 3) * 32 < cols) *(u32x4*)(d + row * ld + c * 16) = *(const u32x4*)(smem + row * ROW + (c ^ (row & (CH - 1))) * 16);
         }
     }
-    // the tile transposed, rows j of the accumulators' columns, to dt
-    static __device__ __forceinline__ void store_t(const f32x16 (&acc)[Core::TM][Core::TN], float alpha, char* dt, long ld, int rows, int cols, bool diag, unsigned char* smem)
-    {
-        nt_wait_barrier<0>();
-        Quads::each([&](int b, int i, int j) {
-            float q[4];
-            Quads::quad(acc, b, q);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) q[r] *= alpha;
-            if (diag) {
-                ns_both_halves(i, j, q, [&](int r, int c, const Pair& s) { *(_Float16*)at(smem, r, c) = s.h; *(_Float16*)lo(smem, r, c) = s.l; });
-            } else {
-                f16x4_t h, l;
-                ns_split4(q, h, l);
-                *(f16x4_t*)at(smem, j, i) = h; *(f16x4_t*)lo(smem, j, i) = l;
-            }
-        });
-        copy_out(dt, ld, rows, cols, smem);
-    }
-    // the tile itself to d: four lanes swap their 4 x 4 elements first, so that each holds four consecutive columns of one row
+    // four lanes (columns j & ~3 ..) transpose their 4 x 4 elements: lane t gets row t, four consecutive columns
     static __device__ __forceinline__ u32x2 swap4(u32x2 v)
     {
         const bool s = threadIdx.x & 1, t = threadIdx.x & 2;
@@ -300,6 +288,31 @@ template <class Core> struct NsTile {
         const unsigned y = __builtin_amdgcn_update_dpp(0, t ? e0 : e1, 0x4E, 0xf, 0xf, true);
         return t ? u32x2{y, e1} : u32x2{e0, y};
     }
+    // the tile transposed, rows j of the accumulators' columns, to dt; diag: a symmetric tile on the diagonal, see ns_both_halves
+    static __device__ __forceinline__ void store_t(const f32x16 (&acc)[Core::TM][Core::TN], float alpha, char* dt, long ld, int rows, int cols, bool diag, unsigned char* smem)
+    {
+        nt_wait_barrier<0>();
+        Quads::each([&](int b, int i, int j) {
+            float q[4];
+            Quads::quad(acc, b, q);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) q[r] *= alpha;
+            f16x4_t h, l;
+            ns_split4(q, h, l);
+            if (!diag || i > j) { *(f16x4_t*)at(smem, j, i) = h; *(f16x4_t*)lo(smem, j, i) = l; }
+            if (diag) {       // the lower part in its own place too; of a 4 x 4 block on the diagonal the row's part up to it, the mirrored part behind it
+                const int t = j & 3, j0 = j & ~3;
+                const f16x4_t uh = __builtin_bit_cast(f16x4_t, swap4(__builtin_bit_cast(u32x2, h))), ul = __builtin_bit_cast(f16x4_t, swap4(__builtin_bit_cast(u32x2, l)));
+                if (i == j0) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) { h[r] = r <= t ? uh[r] : h[r]; l[r] = r <= t ? ul[r] : l[r]; }
+                    *(f16x4_t*)at(smem, j, j0) = h; *(f16x4_t*)lo(smem, j, j0) = l;
+                } else if (i > j0) { *(f16x4_t*)at(smem, i + t, j0) = uh; *(f16x4_t*)lo(smem, i + t, j0) = ul; }
+            }
+        });
+        copy_out(dt, ld, rows, cols, smem);
+    }
+    // the tile itself to d
     static __device__ __forceinline__ void store(const f32x16 (&acc)[Core::TM][Core::TN], float alpha, char* d, long ld, int rows, int cols, unsigned char* smem)
     {
         nt_wait_barrier<0>();
@@ -355,6 +368,19 @@ __device__ __forceinline__ int ns_dealt(const NsDeal& d, int id)
 struct NsProd { int a, b, e, f, d; float alpha, beta, gamma; };
 struct NsProds { NsProd p[2]; };
 
+// blends E and F into a whole tile and stores it with its mirror image
+template <class Core> __device__ __forceinline__ void ns_prod_end(const NsView& v, const NsProd& p, int ti, int tj, f32x16 (&acc)[Core::TM][Core::TN], unsigned char* smem)
+{
+    typedef NsTile<Core> Tile;
+    constexpr int T = Core::BM;
+    const long ls = (long)v.mp * 4, oij = (long)ti * T * ls + tj * T * 4, oji = (long)tj * T * ls + ti * T * 4;       // tile (ti, tj) and its mirror image
+    const int ri = v.mp - ti * T, rj = v.mp - tj * T;
+    float alpha = p.alpha;
+    if (p.e >= 0) { Tile::blend(acc, alpha, p.beta, v.sym(p.e) + oji, ls, rj, ri, smem); alpha = 1.f; }
+    if (p.f >= 0) Tile::blend(acc, alpha, p.gamma, v.sym(p.f) + oji, ls, rj, ri, smem);
+    Tile::store_t(acc, alpha, v.sym(p.d) + oji, ls, rj, ri, ti == tj, smem);
+    if (ti != tj) Tile::store(acc, alpha, v.sym(p.d) + oij, ls, ri, rj, smem);
+}
 template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) void ns_prod_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr, NsDeal deal, int tail)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -382,14 +408,25 @@ template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) voi
         Quads::each([&](int b, int, int) { float q[4]; Quads::quad(acc, b, q); *(f32x4*)(d + b * Core::NT * 4) = f32x4{q[0], q[1], q[2], q[3]}; });
         return;
     }
-    typedef NsTile<Core> Tile;
-    const long ls = (long)v.mp * 4, oij = (long)ti * T * ls + tj * T * 4, oji = (long)tj * T * ls + ti * T * 4;       // tile (ti, tj) and its mirror image
-    const int ri = v.mp - ti * T, rj = v.mp - tj * T;
-    float alpha = p.alpha;
-    if (p.e >= 0) { Tile::blend(acc, alpha, p.beta, v.sym(p.e) + oji, ls, rj, ri, smem); alpha = 1.f; }
-    if (p.f >= 0) Tile::blend(acc, alpha, p.gamma, v.sym(p.f) + oji, ls, rj, ri, smem);
-    Tile::store_t(acc, alpha, v.sym(p.d) + oji, ls, rj, ri, ti == tj, smem);
-    if (ti != tj) Tile::store(acc, alpha, v.sym(p.d) + oij, ls, ri, rj, smem);
+    ns_prod_end<Core>(v, p, ti, tj, acc, smem);
+}
+// The m x m products between a Gram matrix and the product with X, one workgroup a matrix of up to 128 rows: each is a single tile, and a launch of its own
+// would cost it 8 us, most of them the launch and the walk through the table.  What the workgroup stored it reads back through the same L1.
+constexpr int NS_CHAIN = 10;
+struct NsChain { int n; NsProd p[NS_CHAIN]; };
+template <class Core> __global__ __launch_bounds__(Core::NT) void ns_chain_kernel(const NsItem* __restrict__ tab, NsChain ch)
+{
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+    const NsItem it = tab[blockIdx.x];
+    const NsView v(it);
+    const int ld = v.mp * 4;
+    for (int i = 0; i < ch.n; ++i) {
+        const NsProd p = ch.p[i];
+        f32x16 acc[Core::TM][Core::TN] = {};
+        Core::run(v.sym(p.a), ld, v.mp, v.sym(p.b), ld, v.mp, v.mp / 32, smem, acc);
+        ns_prod_end<Core>(v, p, 0, 0, acc, smem);
+        nt_wait_barrier<0>();                                              // every wave's stores have arrived
+    }
 }
 // one accumulator quad of a cut tile a thread; blockIdx.x = tile * quads + quad
 template <class Core> __global__ __launch_bounds__(Core::NT) void ns_finish_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr)
@@ -969,8 +1006,20 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, cons
     hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)p.norm), dim3(256), 0, st, tab, n, hyper, part);
     hipLaunchKernelGGL((ns_pack_kernel<T, MUON>), dim3((unsigned)p.pack), dim3(256), 0, st, tab, n, hyper, part, d->eps, w.sx);
     SAUNET_CHECK_LAUNCH("ns_pack");
+    const bool chain = (large[0].rows < large[0].cols ? large[0].rows : large[0].cols) <= 128;        // (the longest is first)
     for (int i = 0; i < w.count; ++i) {
         const NsOp& o = w.op[i];
+        if (chain && !o.apply && !o.gram) {
+            NsChain ch = {};
+            for (; !w.op[i].apply; ++i)
+                for (int y = 0; y < w.op[i].ny; ++y) ch.p[ch.n++] = w.op[i].pr.p[y];
+            --i;
+            static DeviceOnce once;
+            if (once.first()) (void)hipFuncSetAttribute((const void*)ns_chain_kernel<NsCore128W>, hipFuncAttributeMaxDynamicSharedMemorySize, NsCore128W::LDS);
+            hipLaunchKernelGGL((ns_chain_kernel<NsCore128W>), dim3(n), dim3(NsCore128W::NT), NsCore128W::LDS, st, tab, ch);
+            SAUNET_CHECK_LAUNCH("ns_chain");
+            continue;
+        }
         if (o.apply) {
             constexpr int LAST = MUON ? 2 : 1;
             if (p.tile_n == 64) o.last ? ns_launch_apply<NsCore64, T, LAST>(d, p, tab, o, hyper, st) : ns_launch_apply<NsCore64, T, 0>(d, p, tab, o, hyper, st);
