@@ -241,14 +241,32 @@ template <class Core> struct NsTile {
     static constexpr int B = Core::BM, ROW = B * 4, CH = ROW / 16, RPI = 1024 / ROW, INSTR = B * ROW / 1024 / Core::NW;
     static_assert(Core::BM == Core::BN && B * ROW <= Core::LDS, "the tile fits");
     typedef NsQuads<Core> Quads;
-    static __device__ __forceinline__ unsigned char* at(unsigned char* smem, int row, int col)        // high part; the low part is 4 chunks on
-    {
-        return smem + row * ROW + ((((col >> 5) * 8 + ((col & 31) >> 3)) ^ (row & (CH - 1))) * 16) + (col & 7) * 2;
-    }
-    static __device__ __forceinline__ unsigned char* lo(unsigned char* smem, int row, int col)
-    {
-        return smem + row * ROW + ((((col >> 5) * 8 + 4 + ((col & 31) >> 3)) ^ (row & (CH - 1))) * 16) + (col & 7) * 2;
-    }
+    // Where the accumulator quads of a thread lie: rows j of the transposed tile (four consecutive columns i), or, after swap4, row i + t of the tile itself
+    // (four consecutive columns).  The wave's, the lane's and the quad's share of a chunk number have no bit in common, so the XOR is one
+    // instruction a quad; the low part is four chunks on, which is address bit 6.
+    struct Where {
+        unsigned t0, tx, u0, ux;                       // row start and chunk swap of either
+        __device__ __forceinline__ Where()
+        {
+            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31, t = l & 3;
+            const int wi = (wave / Core::WGN) * (B / Core::WGM), wj = (wave % Core::WGN) * (B / Core::WGN);
+            t0 = (wj + l) * ROW + half * 8;
+            tx = ((wi / 32 * 8) ^ (l & (CH - 1))) * 16;
+            u0 = (wi + half * 4 + t) * ROW + (l & 4) * 2;
+            ux = ((wj / 32 * 8 + (l >> 3)) ^ (half * 4 + t)) * 16;
+        }
+        __device__ __forceinline__ unsigned tile_t(int b) const          // quad b of tile (ti, tj), group g
+        {
+            const int ti = b / (4 * Core::TN), tj = b / 4 % Core::TN, g = b & 3;
+            return t0 + tj * 32 * ROW + (tx ^ ((ti * 8 + g) * 16));
+        }
+        __device__ __forceinline__ unsigned tile(int b) const
+        {
+            const int ti = b / (4 * Core::TN), tj = b / 4 % Core::TN, g = b & 3;
+            return u0 + (ti * 32 + g * 8) * ROW + (ux ^ (((tj * 8) ^ ((g * 8) & (CH - 1))) * 16));
+        }
+    };
+    static_assert((Core::TN & (Core::TN - 1)) == 0 && (Core::TM & (Core::TM - 1)) == 0, "chunk numbers add without a carry");
     // acc <- alpha acc + beta E;  e: the tile of E^T, `rows` of its rows and `cols` of its columns (a multiple of 32) exist.  Ends with LDS in use.
     static __device__ __forceinline__ void blend(f32x16 (&acc)[Core::TM][Core::TN], float alpha, float beta, const char* e, long ld, int rows, int cols, unsigned char* smem)
     {
@@ -262,8 +280,10 @@ template <class Core> struct NsTile {
             nt_dma16(e, (unsigned)((row < rows ? row : rows - 1) * ld + (c < last ? c : last) * 16), (unsigned)(uintptr_t)smem + k * 1024);
         }
         nt_wait_barrier<0>();
-        Quads::each([&](int b, int i, int j) {
-            const f16x4_t h = *(const f16x4_t*)at(smem, j, i), l = *(const f16x4_t*)lo(smem, j, i);
+        const Where w;
+        Quads::each([&](int b, int, int) {
+            const unsigned o = w.tile_t(b);
+            const f16x4_t h = *(const f16x4_t*)(smem + o), l = *(const f16x4_t*)(smem + (o ^ 64));
             f32x16& c = acc[b / (4 * Core::TN)][b / 4 % Core::TN];
 #pragma unroll
             for (int r = 0; r < 4; ++r) c[(b & 3) * 4 + r] = fmaf(alpha, c[(b & 3) * 4 + r], beta * ((float)h[r] + (float)l[r]));
@@ -292,6 +312,7 @@ template <class Core> struct NsTile {
     static __device__ __forceinline__ void store_t(const f32x16 (&acc)[Core::TM][Core::TN], float alpha, char* dt, long ld, int rows, int cols, bool diag, unsigned char* smem)
     {
         nt_wait_barrier<0>();
+        const Where w;
         Quads::each([&](int b, int i, int j) {
             float q[4];
             Quads::quad(acc, b, q);
@@ -299,15 +320,20 @@ template <class Core> struct NsTile {
             for (int r = 0; r < 4; ++r) q[r] *= alpha;
             f16x4_t h, l;
             ns_split4(q, h, l);
-            if (!diag || i > j) { *(f16x4_t*)at(smem, j, i) = h; *(f16x4_t*)lo(smem, j, i) = l; }
-            if (diag) {       // the lower part in its own place too; of a 4 x 4 block on the diagonal the row's part up to it, the mirrored part behind it
-                const int t = j & 3, j0 = j & ~3;
-                const f16x4_t uh = __builtin_bit_cast(f16x4_t, swap4(__builtin_bit_cast(u32x2, h))), ul = __builtin_bit_cast(f16x4_t, swap4(__builtin_bit_cast(u32x2, l)));
-                if (i == j0) {
+            const unsigned o = w.tile_t(b);
+            if (!diag) { *(f16x4_t*)(smem + o) = h; *(f16x4_t*)(smem + (o ^ 64)) = l; return; }
+            // the lower part twice, mirrored and in its own place; of a 4 x 4 block on the diagonal the row's part up to it, the mirrored part behind it
+            const int t = j & 3, j0 = j & ~3;
+            if (i < j0) return;                                            // (the four lanes of a swap agree)
+            const f16x4_t uh = __builtin_bit_cast(f16x4_t, swap4(__builtin_bit_cast(u32x2, h))), ul = __builtin_bit_cast(f16x4_t, swap4(__builtin_bit_cast(u32x2, l)));
+            const unsigned u = w.tile(b);
+            if (i == j0) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) { h[r] = r <= t ? uh[r] : h[r]; l[r] = r <= t ? ul[r] : l[r]; }
-                    *(f16x4_t*)at(smem, j, j0) = h; *(f16x4_t*)lo(smem, j, j0) = l;
-                } else if (i > j0) { *(f16x4_t*)at(smem, i + t, j0) = uh; *(f16x4_t*)lo(smem, i + t, j0) = ul; }
+                for (int r = 0; r < 4; ++r) { h[r] = r <= t ? uh[r] : h[r]; l[r] = r <= t ? ul[r] : l[r]; }
+                *(f16x4_t*)(smem + o) = h; *(f16x4_t*)(smem + (o ^ 64)) = l;
+            } else {
+                *(f16x4_t*)(smem + o) = h; *(f16x4_t*)(smem + (o ^ 64)) = l;
+                *(f16x4_t*)(smem + u) = uh; *(f16x4_t*)(smem + (u ^ 64)) = ul;
             }
         });
         copy_out(dt, ld, rows, cols, smem);
@@ -316,16 +342,17 @@ template <class Core> struct NsTile {
     static __device__ __forceinline__ void store(const f32x16 (&acc)[Core::TM][Core::TN], float alpha, char* d, long ld, int rows, int cols, unsigned char* smem)
     {
         nt_wait_barrier<0>();
-        Quads::each([&](int b, int i, int j) {
+        const Where w;
+        Quads::each([&](int b, int, int) {
             float q[4];
             Quads::quad(acc, b, q);
 #pragma unroll
             for (int r = 0; r < 4; ++r) q[r] *= alpha;
             f16x4_t h, l;
             ns_split4(q, h, l);
-            const int row = i + (j & 3), col = j & ~3;
-            *(u32x2*)at(smem, row, col) = swap4(__builtin_bit_cast(u32x2, h));
-            *(u32x2*)lo(smem, row, col) = swap4(__builtin_bit_cast(u32x2, l));
+            const unsigned u = w.tile(b);
+            *(u32x2*)(smem + u) = swap4(__builtin_bit_cast(u32x2, h));
+            *(u32x2*)(smem + (u ^ 64)) = swap4(__builtin_bit_cast(u32x2, l));
         });
         copy_out(d, ld, rows, cols, smem);
     }
