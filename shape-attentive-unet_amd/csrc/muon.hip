@@ -5,12 +5,13 @@
 // One call takes any number of matrices of any shapes: every launch below covers one phase of ALL of them, a workgroup finds its matrix in a
 // table of tile prefixes.  The whole chain is some twenty launches whatever the list is.
 //
-// Composition.  S_k+1 = P_k S_k P_k with P_k = a I + b S_k + c S_k^2, and all of them commute, so up to three steps run on the m x m matrices alone
-// (S and the product Q = P_2 P_1 P_0) before X is touched: 6 m^2 n + 14 m^3 operations for five steps (3 + 2) against 5 (3 m^2 n + m^3).  Equal for a
-// square, 2.4x less at n = 27 m.  An error of S grows by a^2 = 12 with every step it is carried through, so S is formed anew from X after three:
-// composing all five loses four digits, composing three + two none (1.0e-6 against 0.5e-6 of |X|; the same chain in float32: 2e-6 .. 1e-5).
-// What is composed is (P_2 P_1 P_0 - a^3 I): up to 41 in size where s is near 1, for a result near 1.  Since the s^2 add up to 1, that costs
-// 41 / sqrt(m) roundings of the result's norm -- nothing from m = 32 on, two digits at m = 1, so a list with a shorter matrix goes step by step.
+// Composition.  S_k+1 = P_k S_k P_k with P_k = a I + b S_k + c S_k^2, and all of them commute, so some steps run on the m x m matrices alone (S and
+// the product of the P_k) before X is touched: three, then two at a time; 6 m^2 n + 14 m^3 operations for five steps against 5 (3 m^2 n + m^3).  Equal for
+// a square, 2.4x less at n = 27 m.  What it costs in digits: an error of S grows by a^2 = 12 with every step it is carried through, and the product is
+// kept as (P_2 P_1 P_0 - a^3 I), up to 41 in size where s is near 1, for a result near 1.  In the first block the s^2 add up to 1, so the 41 are divided by
+// sqrt(m): nothing from m = 32 on (a list with a shorter matrix that is not handled below goes step by step).  Later most s are near 1: two steps at a
+// time, 11 roundings.  Distance from float64 for 48 x 120 and 300 x 500 normal matrices, five steps: 2.1e-6 and 3.1e-6, step by step 1.6e-6 and 1.6e-6,
+// float32 matrices 1.3e-6 and 1.6e-6; all five steps at once lose four digits.
 //
 // Number format.  Every matrix between the first and the last pass is a pair of float16 planes, x = hi + lo to 2^-24 (nt_tiles.h: 128-byte blocks of 32
 // elements), scaled by a power of two that the host derives from the singular values' range.  A product is then three float16 MFMAs with float32
@@ -849,9 +850,12 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
         for (; j > 0 && side(large[j - 1]) < side(o); --j) large[j] = large[j - 1];
         large[j] = o;
     }
-    p.tile_g = ab_env_int("SAUNET_NS_GTILE", g128 <= 1024 ? 64 : 128);
-    p.tile_m = ab_env_int("SAUNET_NS_TILE", w128 <= 2048 ? 64 : 128);
-    p.tile_n = ab_env_int("SAUNET_NS_ATILE", a128 <= 128 ? 64 : 128);
+    // 64 x 64 tiles where the work would leave CUs idle: Gram products by their steps (512 x 13824, 4320 of them: 398 us a call with 64, 380 with 128;
+    // 128 x 256, 8: 217 against 228), the m x m products likewise (SAUNet's list, 1100: 1090 against 1173; six 1000 x 1024, 6900: 942 against 803), the
+    // products with X by their tiles (128 x 256, 2: 196 against 217; 512 x 13824, 432: 423 against 398)
+    p.tile_g = g128 <= 1024 ? 64 : 128;
+    p.tile_m = w128 <= 2048 ? 64 : 128;
+    p.tile_n = a128 <= 128 ? 64 : 128;
     for (long i = 0; i < p.large; ++i) {
         NsItem& o = large[i];
         const long m = o.rows < o.cols ? o.rows : o.cols, n = o.rows < o.cols ? o.cols : o.rows, mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
@@ -929,8 +933,8 @@ static bool ns_schedule(const saunet_ns_desc* d, bool compose, NsSchedule& w)
     int xt = 0;
     auto push = [&](int ny, const NsProds& pr, bool gram) { w.op[w.count++] = NsOp{0, ny, pr, 0, 0, 0.f, 0.f, gram, false}; };
     for (int done = 0; done < d->steps;) {
-        // three steps at a time on the Gram matrix while a^2 each keeps its rounding error below 2^8 of itself, else one
-        const int left = d->steps - done, nb = compose ? (left == 4 ? 2 : left < 3 ? left : 3) : 1;
+        // up to three steps at once on the first Gram matrix, up to two on a later one (see the head of this file)
+        const int left = d->steps - done, most = !compose ? 1 : done ? 2 : 3, nb = left < most ? left : most;
         for (int i = 0; i <= NS_GRID; ++i) S[i] = x[i] * x[i];
         float sa = ns_scale(S), sp, sq = 0;
         if (sa == 0.f) return false;

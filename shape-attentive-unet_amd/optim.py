@@ -322,6 +322,6 @@ def create_optimizers(unet, optimizer="sgd", lr=5e-4, momentum=0.9, weight_decay
         mats = [p for p in groups[0]["params"] if p.shape[0] > 1 and p.numel() > p.shape[0]]
         ids = {id(p) for p in mats}
         rest = [p for g in groups for p in g["params"] if id(p) not in ids]
-        return [FusedMuon(mats, lr=lr, weight_decay=weight_decay, momentum=momentum, adjust_lr_fn="match_rms_adamw"),
-                FusedAdam(rest, lr=lr, betas=(0.9, 0.999))]
+        opts = [FusedMuon(mats, lr=lr, weight_decay=weight_decay, momentum=momentum, adjust_lr_fn="match_rms_adamw")] if mats else []
+        return opts + ([FusedAdam(rest, lr=lr, betas=(0.9, 0.999))] if rest else [])
     raise ValueError("optimizer %s: sgd, adam and radam (train.py:187-207) or muon" % optimizer)

@@ -244,6 +244,9 @@ def test_linear_int8(m, dtype):
     wr = HF.quantize_rows(rows(24, 96, 6).cuda())
     assert torch.equal(HF.linear_int8(lead, wr, dtype=torch.float32), HF.linear_int8(lead.view(-1, 96), wr, dtype=torch.float32).view(2, 3, m, 24))
     assert HF.linear_int8(lead[:0], wr).shape == (0, 3, m, 24)
+    one = HF.linear_int8(lead[0, 0, 0], wr, dtype=torch.float32)                      # a single vector
+    assert one.shape == (24,) and torch.equal(one, HF.linear_int8(lead[0, 0, :1], wr, dtype=torch.float32)[0])
+    assert HF.matmul_int8(HF.quantize_rows(lead[0, 0, 0]), wr, out=torch.empty(24, dtype=torch.bfloat16, device="cuda")).shape == (24,)
 
 
 @pytest.mark.gpu
