@@ -9,9 +9,9 @@
 // the product of the P_k) before X is touched: three, then two at a time; 6 m^2 n + 14 m^3 operations for five steps against 5 (3 m^2 n + m^3).  Equal for
 // a square, 2.4x less at n = 27 m.  What it costs in digits: an error of S grows by a^2 = 12 with every step it is carried through, and the product is
 // kept as (P_2 P_1 P_0 - a^3 I), up to 41 in size where s is near 1, for a result near 1.  In the first block the s^2 add up to 1, so the 41 are divided by
-// sqrt(m): nothing from m = 32 on (a list with a shorter matrix that is not handled below goes step by step).  Later most s are near 1: two steps at a
-// time, 11 roundings.  Distance from float64 for 48 x 120 and 300 x 500 normal matrices, five steps: 2.1e-6 and 3.1e-6, step by step 1.6e-6 and 1.6e-6,
-// float32 matrices 1.3e-6 and 1.6e-6; all five steps at once lose four digits.
+// sqrt(m): three from m = 256 on, two before.  Later most s are near 1, so there P is kept as (a - 1) I + b S + c S^2, near zero, and two steps are composed.
+// Matrices of up to 128 rows go step by step.  Distance from float64 over that of the same chain in float32 matrices, gradient-like input, five steps:
+// 0.6 - 1.2 for 33 .. 128 rows (three + two: 1.4 - 4.6), 0.9 - 1.1 for 129 .. 255 (three + two: 1.2 - 3.8), 1.2 at 300, 0.8 at 512, 0.4 at 1000 and above.
 //
 // Number format.  Every matrix between the first and the last pass is a pair of float16 planes, x = hi + lo to 2^-24 (nt_tiles.h: 128-byte blocks of 32
 // elements), scaled by a power of two that the host derives from the singular values' range.  A product is then three float16 MFMAs with float32
@@ -390,10 +390,10 @@ __device__ __forceinline__ int ns_dealt(const NsDeal& d, int id)
     return t < d.b[x + 1] ? t : -1;
 }
 
-// D = alpha A B^T (+ beta E + gamma F) for a symmetric D -- X X^T, or a product of symmetric matrices that commute: lower tiles, both halves
+// D = alpha A B^T (+ beta E + gamma F + diag I) for a symmetric D -- X X^T, or a product of symmetric matrices that commute: lower tiles, both halves
 // written.  blockIdx.y picks the product: the two of one phase are independent.  The tiles behind the first split.full are cut along the reduction into
 // split.s parts, whose float32 sums go to memory in accumulator order for ns_finish_kernel.
-struct NsProd { int a, b, e, f, d; float alpha, beta, gamma; };
+struct NsProd { int a, b, e, f, d; float alpha, beta, gamma, diag; };          // diag: added to the diagonal of a product with an E
 struct NsProds { NsProd p[2]; };
 
 // blends E and F into a whole tile and stores it with its mirror image
@@ -406,6 +406,11 @@ template <class Core> __device__ __forceinline__ void ns_prod_end(const NsView& 
     float alpha = p.alpha;
     if (p.e >= 0) { Tile::blend(acc, alpha, p.beta, v.sym(p.e) + oji, ls, rj, ri, smem); alpha = 1.f; }
     if (p.f >= 0) Tile::blend(acc, alpha, p.gamma, v.sym(p.f) + oji, ls, rj, ri, smem);
+    if (p.diag != 0.f && ti == tj)
+        NsQuads<Core>::each([&](int b, int i, int j) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[b / (4 * Core::TN)][b / 4 % Core::TN][(b & 3) * 4 + r] += i + r == j ? p.diag : 0.f;
+        });
     Tile::store_t(acc, alpha, v.sym(p.d) + oji, ls, rj, ri, ti == tj, smem);
     if (ti != tj) Tile::store(acc, alpha, v.sym(p.d) + oij, ls, ri, rj, smem);
 }
@@ -492,6 +497,8 @@ template <class Core> __global__ __launch_bounds__(Core::NT) void ns_finish_kern
     }
     char* d = v.sym(p.d);
     if (ti == tj) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] += i + r == j ? p.diag : 0.f;
         ns_both_halves(i, j, w, [&](int r, int c, const Pair& e) { char* o = d + r * ls + (c >> 5) * 128 + (c & 31) * 2; *(_Float16*)o = e.h; *(_Float16*)(o + 64) = e.l; });
         return;
     }
@@ -923,18 +930,21 @@ static float ns_scale(const double* v)
 struct NsOp { int apply, ny; NsProds pr; int q, xt; float alpha, beta; bool gram, last; };
 struct NsSchedule { int count; float sx; NsOp op[32 * 4]; };
 
-static bool ns_schedule(const saunet_ns_desc* d, bool compose, NsSchedule& w)
+// first, later: steps composed at once in the first block and in the others (see the head of this file)
+static bool ns_schedule(const saunet_ns_desc* d, int first, int later, NsSchedule& w)
 {
     double x[NS_GRID + 1], S[NS_GRID + 1], P[NS_GRID + 1], Q[NS_GRID + 1], R[NS_GRID + 1];
-    const double a = d->a, b = d->b, c = d->c;
+    const double b = d->b, c = d->c;
     for (int i = 0; i <= NS_GRID; ++i) { const double u = (double)i / NS_GRID; x[i] = u * u * u * u * (1.0 + 1e-6); }
     float sx = w.sx = ns_scale(x);
     w.count = 0;
     int xt = 0;
     auto push = [&](int ny, const NsProds& pr, bool gram) { w.op[w.count++] = NsOp{0, ny, pr, 0, 0, 0.f, 0.f, gram, false}; };
     for (int done = 0; done < d->steps;) {
-        // up to three steps at once on the first Gram matrix, up to two on a later one (see the head of this file)
-        const int left = d->steps - done, most = !compose ? 1 : done ? 2 : 3, nb = left < most ? left : most;
+        const int left = d->steps - done, most = done ? later : first, nb = left < most ? left : most;
+        // P is kept as b S + c S^2 in the first block, where most s are small, and as that + (a - 1) I, near zero where s is near 1, later: its rounding
+        // counts in units of what is kept (300 x 500, five steps: 3.1e-6 of |X| without the shift, 1.6e-6 with it)
+        const double a = done ? 1.0 : (double)d->a, shift = (double)d->a - a;
         for (int i = 0; i <= NS_GRID; ++i) S[i] = x[i] * x[i];
         float sa = ns_scale(S), sp, sq = 0;
         if (sa == 0.f) return false;
@@ -942,11 +952,11 @@ static bool ns_schedule(const saunet_ns_desc* d, bool compose, NsSchedule& w)
         double q = 0;
         int Qb = NS_Q0;
         for (int j = 0; j < nb; ++j) {
-            for (int i = 0; i <= NS_GRID; ++i) P[i] = b * S[i] + c * S[i] * S[i];
+            for (int i = 0; i <= NS_GRID; ++i) P[i] = b * S[i] + c * S[i] * S[i] + shift;
             sp = ns_scale(P);
             if (sp == 0.f) return false;
             const int Pb = j ? NS_P : NS_Q0;
-            push(1, NsProds{{{NS_A, NS_A, NS_A, -1, Pb, (float)(c * sp / ((double)sa * sa)), (float)(b * sp / sa), 0.f}, {}}}, false);
+            push(1, NsProds{{{NS_A, NS_A, NS_A, -1, Pb, (float)(c * sp / ((double)sa * sa)), (float)(b * sp / sa), 0.f, (float)(shift * sp)}, {}}}, false);
             NsProds pr = {};
             int ny = 0;
             if (j == 0) { for (int i = 0; i <= NS_GRID; ++i) Q[i] = P[i]; sq = sp; q = a; }
@@ -1001,7 +1011,22 @@ template <class Core> static void ns_launch_prod(const NsPlan& p, const NsItem* 
     if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(Core::NT), 0, st, tab, (int)p.large, kind, o.pr);
 }
 
-template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
+// The matrices with up to NS_MID rows and the others are two chains of launches: the short ones have their products between Gram matrix and X in one launch
+// and go step by step, which costs them nothing and keeps their digits.  k: 0 the short ones, 1 the others
+constexpr int NS_MID = 128;
+static saunet_ns_desc ns_part(const saunet_ns_desc* d, int k, saunet_ns_item* item)
+{
+    saunet_ns_desc r = *d;
+    r.item = item; r.count = 0;
+    for (int i = 0; i < d->count; ++i) {
+        const saunet_ns_item& t = d->item[i];
+        if (((t.rows < t.cols ? t.rows : t.cols) > NS_MID) == (k == 1)) item[r.count++] = t;
+    }
+    return r;
+}
+
+// go: false looks only whether the call can be made
+template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool go, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
 {
     static thread_local NsItem large[4096];
     static thread_local NssItem small[4096];
@@ -1011,7 +1036,10 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, cons
     if (rc) return rc;
     if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255)) return set_error(SAUNET_BAD_SHAPE, "%s: the workspace has to hold %ld bytes on a 256-byte border", who, p.bytes);
     NsSchedule w;
-    if (!ns_schedule(d, (double)d->a * d->a <= 16.0 && p.shortest >= 32, w)) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
+    const bool chain = p.large && (large[0].rows < large[0].cols ? large[0].rows : large[0].cols) <= NS_MID;        // (the longest is first)
+    const bool compose = p.large && !chain && (double)d->a * d->a <= 16.0;
+    if (!ns_schedule(d, !compose ? 1 : p.shortest < 256 ? 2 : 3, compose ? 2 : 1, w)) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
+    if (!go) return SAUNET_OK;
     for (long i = 0; i < p.small; i += NSS_CHUNK) {
         NssItems ch;
         const int k = (int)(p.small - i < NSS_CHUNK ? p.small - i : NSS_CHUNK);
@@ -1037,7 +1065,6 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, cons
     hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)p.norm), dim3(256), 0, st, tab, n, hyper, part);
     hipLaunchKernelGGL((ns_pack_kernel<T, MUON>), dim3((unsigned)p.pack), dim3(256), 0, st, tab, n, hyper, part, d->eps, w.sx);
     SAUNET_CHECK_LAUNCH("ns_pack");
-    const bool chain = (large[0].rows < large[0].cols ? large[0].rows : large[0].cols) <= 128;        // (the longest is first)
     for (int i = 0; i < w.count; ++i) {
         const NsOp& o = w.op[i];
         if (chain && !o.apply && !o.gram) {
@@ -1067,6 +1094,18 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, cons
     return SAUNET_OK;
 }
 
+template <typename T, bool MUON> static int ns_run_all(const saunet_ns_desc* d, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
+{
+    static thread_local saunet_ns_item item[4096];
+    for (int pass = 0; pass < 2; ++pass)
+        for (int k = 0; k < 2; ++k) {
+            const saunet_ns_desc part = ns_part(d, k, item);
+            const int rc = part.count ? ns_run<T, MUON>(&part, pass == 1, hyper, workspace, workspace_bytes, st, who) : SAUNET_OK;
+            if (rc) return rc;
+        }
+    return SAUNET_OK;
+}
+
 }  // namespace saunet
 
 using namespace saunet;
@@ -1077,10 +1116,17 @@ int64_t saunet_newton_schulz_workspace(const saunet_ns_desc* d)
 {
     static thread_local NsItem large[4096];
     static thread_local NssItem small[4096];
+    static thread_local saunet_ns_item item[4096];
     NsPlan p;
     int rc = ns_check(d, "newton_schulz");
-    if (!rc) rc = ns_plan(d, p, large, small, nullptr);
-    return rc ? rc : p.bytes;
+    int64_t most = 0;
+    for (int k = 0; k < 2 && !rc; ++k) {          // one chain behind the other, in the same memory
+        const saunet_ns_desc part = ns_part(d, k, item);
+        if (!part.count) continue;
+        rc = ns_plan(&part, p, large, small, nullptr);
+        if (p.bytes > most) most = p.bytes;
+    }
+    return rc ? rc : most;
 }
 
 int saunet_newton_schulz(const saunet_ns_desc* d, void* workspace, int64_t workspace_bytes, void* stream)
@@ -1089,9 +1135,9 @@ int saunet_newton_schulz(const saunet_ns_desc* d, void* workspace, int64_t works
     if (rc) return rc;
     for (int i = 0; i < d->count; ++i) if (!d->item[i].src || !d->item[i].dst) return set_error(SAUNET_BAD_SHAPE, "newton_schulz: matrix %d has no memory", i);
     hipStream_t st = (hipStream_t)stream;
-    if (d->dtype == SAUNET_F32) return ns_run<float, false>(d, nullptr, workspace, workspace_bytes, st, "newton_schulz");
-    if (d->dtype == SAUNET_BF16) return ns_run<u16, false>(d, nullptr, workspace, workspace_bytes, st, "newton_schulz");
-    return ns_run<_Float16, false>(d, nullptr, workspace, workspace_bytes, st, "newton_schulz");
+    if (d->dtype == SAUNET_F32) return ns_run_all<float, false>(d, nullptr, workspace, workspace_bytes, st, "newton_schulz");
+    if (d->dtype == SAUNET_BF16) return ns_run_all<u16, false>(d, nullptr, workspace, workspace_bytes, st, "newton_schulz");
+    return ns_run_all<_Float16, false>(d, nullptr, workspace, workspace_bytes, st, "newton_schulz");
 }
 
 int saunet_muon_step(const saunet_ns_desc* d, const float* hyper, void* workspace, int64_t workspace_bytes, void* stream)
@@ -1105,7 +1151,7 @@ int saunet_muon_step(const saunet_ns_desc* d, const float* hyper, void* workspac
         if (!t.src || !t.dst || !t.buf) return set_error(SAUNET_BAD_SHAPE, "muon: matrix %d has no memory", i);
         if (t.ld_src != t.cols || t.ld_dst != t.cols) return set_error(SAUNET_BAD_SHAPE, "muon: matrix %d is not contiguous", i);
     }
-    return ns_run<float, true>(d, hyper, workspace, workspace_bytes, (hipStream_t)stream, "muon");
+    return ns_run_all<float, true>(d, hyper, workspace, workspace_bytes, (hipStream_t)stream, "muon");
 }
 
 }  // extern "C"
