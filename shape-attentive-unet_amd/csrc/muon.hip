@@ -18,6 +18,7 @@
 // accumulation, at a sixth of the cost of the float32 MFMA and with no more error.  Products of symmetric matrices compute the lower tiles only and
 // write both halves.  X and X^T are both kept: each is the operand with the contiguous reduction index in one of the two rectangular products.
 #include "nt_tiles.h"
+#include <algorithm>
 
 namespace saunet {
 
@@ -850,13 +851,7 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
         if (p.large == 1 || m < p.shortest) p.shortest = m;
     }
     // the longest reductions first: what starts last is short
-    for (long i = 1; i < p.large; ++i) {
-        const NsItem o = large[i];
-        long j = i;
-        auto side = [](const NsItem& t) { return t.rows < t.cols ? t.rows : t.cols; };
-        for (; j > 0 && side(large[j - 1]) < side(o); --j) large[j] = large[j - 1];
-        large[j] = o;
-    }
+    std::sort(large, large + p.large, [](const NsItem& x, const NsItem& y) { return (x.rows < x.cols ? x.rows : x.cols) > (y.rows < y.cols ? y.rows : y.cols); });
     // 64 x 64 tiles where the work would leave CUs idle: Gram products by their steps (512 x 13824, 4320 of them: 398 us a call with 64, 380 with 128;
     // 128 x 256, 8: 217 against 228), the m x m products likewise (SAUNet's list, 1100: 1090 against 1173; six 1000 x 1024, 6900: 942 against 803), the
     // products with X by their tiles (128 x 256, 2: 196 against 217; 512 x 13824, 432: 423 against 398)
@@ -1012,12 +1007,16 @@ template <class Core> static void ns_launch_prod(const NsPlan& p, const NsItem* 
 }
 
 // The matrices with up to NS_MID rows and the others are two chains of launches: the short ones have their products between Gram matrix and X in one launch
-// and go step by step, which costs them nothing and keeps their digits.  k: 0 the short ones, 1 the others
+// and keep the digits that composing would cost them.  A Muon step does not need those -- its result is multiplied by the learning rate and added to a
+// rounded parameter -- so there a list with both goes through one chain (SAUNet's matrices: 971 us, in two chains 1136).  k: 0 the short ones, 1 the others
 constexpr int NS_MID = 128;
-static saunet_ns_desc ns_part(const saunet_ns_desc* d, int k, saunet_ns_item* item)
+static saunet_ns_desc ns_part(const saunet_ns_desc* d, bool muon, int k, saunet_ns_item* item)
 {
     saunet_ns_desc r = *d;
     r.item = item; r.count = 0;
+    if (muon)
+        for (int i = 0; i < d->count; ++i)
+            if ((d->item[i].rows < d->item[i].cols ? d->item[i].rows : d->item[i].cols) > NS_MID) { r.item = d->item; r.count = k == 1 ? d->count : 0; return r; }
     for (int i = 0; i < d->count; ++i) {
         const saunet_ns_item& t = d->item[i];
         if (((t.rows < t.cols ? t.rows : t.cols) > NS_MID) == (k == 1)) item[r.count++] = t;
@@ -1037,8 +1036,11 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
     if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255)) return set_error(SAUNET_BAD_SHAPE, "%s: the workspace has to hold %ld bytes on a 256-byte border", who, p.bytes);
     NsSchedule w;
     const bool chain = p.large && (large[0].rows < large[0].cols ? large[0].rows : large[0].cols) <= NS_MID;        // (the longest is first)
-    const bool compose = p.large && !chain && (double)d->a * d->a <= 16.0;
-    if (!ns_schedule(d, !compose ? 1 : p.shortest < 256 ? 2 : 3, compose ? 2 : 1, w)) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
+    // Steps composed at once: see the head of this file.  (A chain of short matrices in twos would gain little: one of 128 x 256 183 us, step by step 171; sixty of
+    // 128 x 64 .. 992 299 us against 324.)
+    const bool compose = p.large && !chain && p.shortest > 32 && (double)d->a * d->a <= 16.0;
+    const int first = !compose ? 1 : !MUON && p.shortest < 256 ? 2 : 3, later = compose ? 2 : 1;
+    if (!ns_schedule(d, first, later, w)) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
     if (!go) return SAUNET_OK;
     for (long i = 0; i < p.small; i += NSS_CHUNK) {
         NssItems ch;
@@ -1099,7 +1101,7 @@ template <typename T, bool MUON> static int ns_run_all(const saunet_ns_desc* d, 
     static thread_local saunet_ns_item item[4096];
     for (int pass = 0; pass < 2; ++pass)
         for (int k = 0; k < 2; ++k) {
-            const saunet_ns_desc part = ns_part(d, k, item);
+            const saunet_ns_desc part = ns_part(d, MUON, k, item);
             const int rc = part.count ? ns_run<T, MUON>(&part, pass == 1, hyper, workspace, workspace_bytes, st, who) : SAUNET_OK;
             if (rc) return rc;
         }
@@ -1120,8 +1122,8 @@ int64_t saunet_newton_schulz_workspace(const saunet_ns_desc* d)
     NsPlan p;
     int rc = ns_check(d, "newton_schulz");
     int64_t most = 0;
-    for (int k = 0; k < 2 && !rc; ++k) {          // one chain behind the other, in the same memory
-        const saunet_ns_desc part = ns_part(d, k, item);
+    for (int k = 0; k < 4 && !rc; ++k) {          // one chain behind the other, in the same memory; for either use
+        const saunet_ns_desc part = ns_part(d, k & 2, k & 1, item);
         if (!part.count) continue;
         rc = ns_plan(&part, p, large, small, nullptr);
         if (p.bytes > most) most = p.bytes;
