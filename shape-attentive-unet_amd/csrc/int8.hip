@@ -249,17 +249,18 @@ template <typename T, class Core> __global__ __launch_bounds__(Core::NT) void ma
     }
 }
 
-// Tile by the amount of work, counted in 64 x 64 tiles (bf16 out; us for channels x tokens of a tile, K the reduction):
-//                                    64x64  128x64  128x128  128x256  256x256
-//   8192 x 4096, K 4096  (8192 tiles)   276     234      178      156      148      a long reduction and work for every CU: operand traffic is the bound
-//   131072 x 128, K 256  (4096 tiles)  21.1    18.2     18.9     16.5     27.9      a short one: memory is, two workgroups a CU overlap loads and stores
-//   2048 x 2048, K 2048  (1024 tiles)  22.4    19.7     18.3     24.9     33.5
-//   8192 x 256, K 8192    (512 tiles)  42.6    36.3     47.6     75.6      101      too few large tiles to fill the card: the smallest that do
-//   512 x 512, K 512       (64 tiles)   4.4     5.4      7.6      8.5     14.1
+// Tile by the amount of work, counted in 64 x 64 tiles (bf16 out; us for channels x tokens of a tile, K the reduction; L: four stages instead of two):
+//                                    64x64  128x64  128x128  128x128L  256x256
+//   8192 x 4096, K 4096  (8192 tiles)   276     234      178       179      142      a long reduction and work for every CU: operand traffic is the bound
+//   131072 x 128, K 256  (4096 tiles)  21.1    18.2     16.3      18.9     27.9      a short one: memory is, several workgroups a CU overlap loads and stores
+//   4096 x 1024, K 8192  (1024 tiles)    80      65       55        50      101
+//   2048 x 2048, K 2048  (1024 tiles)  22.4    19.7     15.5      15.8     33.5
+//   8192 x 256, K 8192    (512 tiles)  42.6    33.2     49.8      40.8      101      too few large tiles to fill the card: the smallest that do
+//   512 x 512, K 512       (64 tiles)   4.4     5.4      5.7       6.2     14.1
 typedef NtCore<NtI8, 64, 64, 2, 2, 4> I8Core64;
 typedef NtCore<NtI8, 128, 64, 2, 2, 4> I8CoreTall;
-typedef NtCore<NtI8, 128, 128, 2, 2, 3> I8Core128;
-typedef NtCore<NtI8, 128, 256, 2, 4, 2> I8CoreWide;
+typedef NtCore<NtI8, 128, 128, 2, 4, 2> I8Core128;
+typedef NtCore<NtI8, 128, 128, 4, 2, 4> I8Core128L;
 typedef NtCore<NtI8, 256, 256, 2, 4, 4> I8Core256;
 
 template <typename T, class Core> static int mm8_tiles(I8Args g, hipStream_t st)
@@ -415,10 +416,9 @@ template <typename T> static int mm8_launch(const I8Args& g, hipStream_t st)
     }
     const long t64 = ((g.m + 63) / 64) * ((g.n + 63) / 64);
     if (t64 >= 192 * 16 && g.ksteps >= 8) return mm8_tiles<T, I8Core256>(g, st);
-    if (t64 >= 512 * 8 && g.ksteps < 8) return mm8_tiles<T, I8CoreWide>(g, st);
     if (t64 <= 384) return mm8_tiles<T, I8Core64>(g, st);
-    if (t64 <= 768 || g.ksteps < 8) return mm8_tiles<T, I8CoreTall>(g, st);
-    return mm8_tiles<T, I8Core128>(g, st);
+    if (t64 <= 768) return mm8_tiles<T, I8CoreTall>(g, st);
+    return g.ksteps >= 64 ? mm8_tiles<T, I8Core128L>(g, st) : mm8_tiles<T, I8Core128>(g, st);
 }
 
 static int int8_check(const saunet_int8_desc* d, const char* who)
