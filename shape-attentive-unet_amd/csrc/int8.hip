@@ -277,9 +277,9 @@ template <typename T, class Core> static int mm8_tiles(I8Args g, hipStream_t st)
     return SAUNET_OK;
 }
 
-// ---- few tokens: the weight is read once, straight into registers -------------------------------------------------------------------------
-// A workgroup owns 16 channels; its 8 waves take the 64-byte steps of the reduction in turn, mfma_i32_16x16x64_i8 with 16 weight rows against MT x 16
-// tokens, and add their sums through LDS. 
+// ---- few tokens or channels: the operands go straight into registers -------------------------------------------------------------------------
+// A workgroup owns 16 channels and MT x 16 tokens; its 8 waves take the 64-byte steps of the reduction in turn, mfma_i32_16x16x64_i8 with 16 weight rows
+// against the tokens, and add their sums through LDS. 
 constexpr int FEW_WAVES = 8, FEW_UNROLL = 8;
 
 template <typename T, int MT> __global__ __launch_bounds__(FEW_WAVES * 64) void matmul_int8_few_kernel(I8Args g)
@@ -287,10 +287,11 @@ template <typename T, int MT> __global__ __launch_bounds__(FEW_WAVES * 64) void 
     __shared__ int s_red[FEW_WAVES][MT][16][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kq = (lane >> 4) * 16;
     const int n0 = blockIdx.x * 16;
+    const long m0 = (long)blockIdx.y * MT * 16;
     const char* b = g.b + (long)(n0 + r < g.n ? n0 + r : g.n - 1) * g.ldb + kq;
     const char* a[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) { const long m = t * 16 + r; a[t] = g.a + (m < g.m ? m : g.m - 1) * g.lda + kq; }
+    for (int t = 0; t < MT; ++t) { const long m = m0 + t * 16 + r; a[t] = g.a + (m < g.m ? m : g.m - 1) * g.lda + kq; }
     i32x4 acc[MT] = {};
     for (int s0 = wave; s0 < g.ksteps; s0 += FEW_WAVES * FEW_UNROLL) {
         i32x4 fb[FEW_UNROLL];
@@ -310,11 +311,12 @@ template <typename T, int MT> __global__ __launch_bounds__(FEW_WAVES * 64) void 
         for (int i = 0; i < 4; ++i) s_red[wave][t][r][(lane >> 4) * 4 + i] = acc[t][i];
     __syncthreads();
     for (int k = threadIdx.x; k < MT * 256; k += FEW_WAVES * 64) {
-        const int c = k & 15, m = k >> 4, n = n0 + c;
+        const int c = k & 15, t = k >> 4, n = n0 + c;
+        const long m = m0 + t;
         if (m >= g.m || n >= g.n) continue;
         int sum = 0;
 #pragma unroll
-        for (int w = 0; w < FEW_WAVES; ++w) sum += s_red[w][m >> 4][m & 15][c];
+        for (int w = 0; w < FEW_WAVES; ++w) sum += s_red[w][t >> 4][t & 15][c];
         float v = fmaf((float)sum * g.sa[m], g.sb[n], g.bias ? g.bias[n] : 0.f);
         if (g.relu && v < 0.f) v = 0.f;
         ((T*)g.y)[m * g.ldy + n] = YElem<T>::cvt(v);
@@ -405,10 +407,13 @@ template <typename X> static void linear_few(const I8Args& g, const QArgs& q, in
 
 template <typename T> static int mm8_launch(const I8Args& g, hipStream_t st)
 {
-    // a workgroup of the streaming kernel reads all tokens again: above 16 x 16384 of them times channels the tiles win (us: 24 tokens of 4096 through
-    // 4096 channels 12.9 against 17.6, 64 tokens through 16384 channels 53 against 24)
-    if (g.m <= 32 && (long)g.n * ((g.m + 15) / 16) <= 16384) {
-        const dim3 grid((unsigned)cdiv(g.n, 16)), block(FEW_WAVES * 64);
+    // Little work: eight waves share the reduction of 16 channels x 32 (16) tokens.  Every such workgroup reads its operands for itself, so the tiles win from
+    // some 512 workgroups on; us against the 64 x 64 tile, tokens x K x channels: 64 x 8075 x 1 7.6 / 28, 256 x 512 x 256 (128 workgroups) 2.8 / 4.5, 512 x 1024 x
+    // 512 (512) 5.1 / 6.1, 64 x 4096 x 4096 (512) 13.7 / 15.5; 777 x 1001 x 515 (825) 7.8 / 7.4, 128 x 4096 x 4096 (1024) 24 / 16.  With 16 tokens or less the
+    // weight is read once either way: to 16384 channels (1024 workgroups), 23.3 / 23.8.
+    const long few = (g.m + 31) / 32 * ((g.n + 15) / 16);
+    if (few <= (g.m <= 16 ? 1024 : 512)) {
+        const dim3 grid((unsigned)cdiv(g.n, 16), g.m <= 16 ? 1 : (unsigned)((g.m + 31) / 32)), block(FEW_WAVES * 64);
         if (g.m <= 16) hipLaunchKernelGGL((matmul_int8_few_kernel<T, 1>), grid, block, 0, st, g);
         else hipLaunchKernelGGL((matmul_int8_few_kernel<T, 2>), grid, block, 0, st, g);
         SAUNET_CHECK_LAUNCH("matmul_int8_few");

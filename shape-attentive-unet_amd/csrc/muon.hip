@@ -3,7 +3,7 @@
 //   X0 = G / max(|G|_F, eps);   S = X X^T,  X <- (a I + b S + c S^2) X,  `steps` times          (rows <= columns; the transpose otherwise)
 //
 // One call takes any number of matrices of any shapes: every launch below covers one phase of ALL of them, a workgroup finds its matrix in a
-// table of tile prefixes.  The whole chain is some twenty launches whatever the list is.
+// table of tile prefixes.  The whole chain is some twenty launches whatever the list is (two chains where it holds both short and long matrices).
 //
 // Composition.  S_k+1 = P_k S_k P_k with P_k = a I + b S_k + c S_k^2, and all of them commute, so some steps run on the m x m matrices alone (S and
 // the product of the P_k) before X is touched: three, then two at a time; 6 m^2 n + 14 m^3 operations for five steps against 5 (3 m^2 n + m^3).  Equal for
@@ -443,24 +443,6 @@ template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) voi
         return;
     }
     ns_prod_end<Core>(v, p, ti, tj, acc, smem);
-}
-// The m x m products between a Gram matrix and the product with X, one workgroup a matrix of up to 128 rows: each is a single tile, and a launch of its own
-// would cost it 8 us, most of them the launch and the walk through the table.  What the workgroup stored it reads back through the same L1.
-constexpr int NS_CHAIN = 10;
-struct NsChain { int n; NsProd p[NS_CHAIN]; };
-template <class Core> __global__ __launch_bounds__(Core::NT) void ns_chain_kernel(const NsItem* __restrict__ tab, NsChain ch)
-{
-    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-    const NsItem it = tab[blockIdx.x];
-    const NsView v(it);
-    const int ld = v.mp * 4;
-    for (int i = 0; i < ch.n; ++i) {
-        const NsProd p = ch.p[i];
-        f32x16 acc[Core::TM][Core::TN] = {};
-        Core::run(v.sym(p.a), ld, v.mp, v.sym(p.b), ld, v.mp, v.mp / 32, smem, acc);
-        ns_prod_end<Core>(v, p, 0, 0, acc, smem);
-        nt_wait_barrier<0>();                                              // every wave's stores have arrived
-    }
 }
 // one accumulator quad of a cut tile a thread; blockIdx.x = tile * quads + quad
 template <class Core> __global__ __launch_bounds__(Core::NT) void ns_finish_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr)
@@ -1006,9 +988,9 @@ template <class Core> static void ns_launch_prod(const NsPlan& p, const NsItem* 
     if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(Core::NT), 0, st, tab, (int)p.large, kind, o.pr);
 }
 
-// The matrices with up to NS_MID rows and the others are two chains of launches: the short ones have their products between Gram matrix and X in one launch
-// and keep the digits that composing would cost them.  A Muon step does not need those -- its result is multiplied by the learning rate and added to a
-// rounded parameter -- so there a list with both goes through one chain (SAUNet's matrices: 971 us, in two chains 1136).  k: 0 the short ones, 1 the others
+// The matrices with up to NS_MID rows and the others are two chains of launches: the short ones go step by step and keep the digits that composing would cost
+// them.  A Muon step does not need those -- its result is multiplied by the learning rate and added to a rounded parameter -- so there a list with both
+// goes through one chain (SAUNet's matrices: 956 us, in two chains 1136).  k: 0 the short ones, 1 the others
 constexpr int NS_MID = 128;
 static saunet_ns_desc ns_part(const saunet_ns_desc* d, bool muon, int k, saunet_ns_item* item)
 {
@@ -1035,10 +1017,9 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
     if (rc) return rc;
     if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255)) return set_error(SAUNET_BAD_SHAPE, "%s: the workspace has to hold %ld bytes on a 256-byte border", who, p.bytes);
     NsSchedule w;
-    const bool chain = p.large && (large[0].rows < large[0].cols ? large[0].rows : large[0].cols) <= NS_MID;        // (the longest is first)
-    // Steps composed at once: see the head of this file.  (A chain of short matrices in twos would gain little: one of 128 x 256 183 us, step by step 171; sixty of
-    // 128 x 64 .. 992 299 us against 324.)
-    const bool compose = p.large && !chain && p.shortest > 32 && (double)d->a * d->a <= 16.0;
+    // Steps composed at once: see the head of this file.  The longest matrix is the first.  (Short ones in twos would gain little: one of 128 x 256 183 us,
+    // step by step 171; sixty of 128 x 64 .. 992 299 us against 324.)
+    const bool compose = p.large && (large[0].rows < large[0].cols ? large[0].rows : large[0].cols) > NS_MID && p.shortest > 32 && (double)d->a * d->a <= 16.0;
     const int first = !compose ? 1 : !MUON && p.shortest < 256 ? 2 : 3, later = compose ? 2 : 1;
     if (!ns_schedule(d, first, later, w)) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
     if (!go) return SAUNET_OK;
@@ -1069,17 +1050,6 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
     SAUNET_CHECK_LAUNCH("ns_pack");
     for (int i = 0; i < w.count; ++i) {
         const NsOp& o = w.op[i];
-        if (chain && !o.apply && !o.gram) {
-            NsChain ch = {};
-            for (; !w.op[i].apply; ++i)
-                for (int y = 0; y < w.op[i].ny; ++y) ch.p[ch.n++] = w.op[i].pr.p[y];
-            --i;
-            static DeviceOnce once;
-            if (once.first()) (void)hipFuncSetAttribute((const void*)ns_chain_kernel<NsCore128W>, hipFuncAttributeMaxDynamicSharedMemorySize, NsCore128W::LDS);
-            hipLaunchKernelGGL((ns_chain_kernel<NsCore128W>), dim3(n), dim3(NsCore128W::NT), NsCore128W::LDS, st, tab, ch);
-            SAUNET_CHECK_LAUNCH("ns_chain");
-            continue;
-        }
         if (o.apply) {
             constexpr int LAST = MUON ? 2 : 1;
             if (p.tile_n == 64) o.last ? ns_launch_apply<NsCore64, T, LAST>(d, p, tab, o, hyper, st) : ns_launch_apply<NsCore64, T, 0>(d, p, tab, o, hyper, st);

@@ -170,7 +170,7 @@ def test_quantize_rows_affine_relu_and_strides(dtype):
 
 # ------------------------------------------------------------------------------------------------ the product
 SHAPES = [(1, 1, 1), (1, 64, 16), (2, 65, 17), (3, 1000, 130), (16, 4096, 64), (17, 200, 515), (31, 64, 128), (33, 63, 129), (64, 512, 512), (127, 130, 255), (129, 257, 257),
-          (200, 128, 1000), (513, 320, 96), (1000, 1001, 33), (2049, 256, 128), (70, 8192, 40)]
+          (200, 128, 1000), (513, 320, 96), (1000, 1001, 33), (2049, 256, 128), (70, 8192, 40), (64, 8075, 1), (500, 64, 17), (33, 1000, 8200), (16, 70, 16400), (900, 130, 600)]
 
 
 @pytest.mark.gpu
