@@ -618,23 +618,28 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void nss_gram
 }
 
 typedef __attribute__((ext_vector_type(4))) double f64x4;
-typedef double NssMat[32][36];          // rows 32 bytes apart in the banks
-// quadrant `quad` of A B for symmetric A, B: element r of lane l is (row l / 16 + 4 r, column l % 16) of it
+typedef __attribute__((ext_vector_type(2))) double f64x2;
+typedef double NssMat[32][34];          // rows 16 bytes apart in the banks: the 16-byte reads of 16 rows meet in none
+// quadrant `quad` of A B for symmetric A, B: element r of lane l is (row l / 16 + 4 r, column l % 16) of it.  A lane group takes eight neighbouring indices of
+// the sum, two a read; two chains, because the MFMAs of one wait for each other.
 __device__ __forceinline__ f64x4 nss_product(const NssMat& a, const NssMat& b, int quad)
 {
-    const int lane = threadIdx.x & 63, i = (quad >> 1) * 16 + (lane & 15), j = (quad & 1) * 16 + (lane & 15), k = lane >> 4;
-    f64x4 c = {0.0, 0.0, 0.0, 0.0}, d = c;                                 // two chains: the MFMAs of one wait for each other
+    const int lane = threadIdx.x & 63, i = (quad >> 1) * 16 + (lane & 15), j = (quad & 1) * 16 + (lane & 15), k = (lane >> 4) * 8;
+    f64x2 x[4], y[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) { x[s] = *(const f64x2*)&a[i][k + 2 * s]; y[s] = *(const f64x2*)&b[j][k + 2 * s]; }
+    f64x4 c = {0.0, 0.0, 0.0, 0.0}, d = c;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        c = __builtin_amdgcn_mfma_f64_16x16x4f64(a[i][s * 4 + k], b[j][s * 4 + k], c, 0, 0, 0);
-        d = __builtin_amdgcn_mfma_f64_16x16x4f64(a[i][16 + s * 4 + k], b[j][16 + s * 4 + k], d, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f64_16x16x4f64(x[s][0], y[s][0], c, 0, 0, 0);
+        d = __builtin_amdgcn_mfma_f64_16x16x4f64(x[s][1], y[s][1], d, 0, 0, 0);
     }
     return c + d;
 }
 // W / norm from the sums of nss_gram_kernel: a workgroup a matrix, waves 0 - 3 and 4 - 7 a product each.  S' = (a I + P)^2 S, W' = (a I + P) W.
 __global__ __launch_bounds__(512) void nss_poly_kernel(NssItems items, int steps, double a, double b, double c, float eps)
 {
-    __shared__ NssMat S, P, R, W;
+    __shared__ __attribute__((aligned(16))) NssMat S, P, R, W;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = wave & 3;
     const NssItem it = items.it[blockIdx.x];
     double* ws = nss_ws(items, blockIdx.x);
