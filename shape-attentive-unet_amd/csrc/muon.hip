@@ -897,7 +897,7 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
 
 // Largest magnitude that a matrix with eigenvalue f(s), s in [0, 1] the first singular values, can hold: its power-of-two scale leaves a factor of two
 // below the largest float16.  The grid is even in s^(1/4): small singular values grow fastest.  0: out of range.
-constexpr int NS_GRID = 256;
+constexpr int NS_GRID = 96;
 static float ns_scale(const double* v)
 {
     double top = 1e-3;
@@ -1011,8 +1011,8 @@ static saunet_ns_desc ns_part(const saunet_ns_desc* d, bool muon, int k, saunet_
     return r;
 }
 
-// go: false looks only whether the call can be made
-template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool go, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
+// go: false looks only whether the call can be made, and leaves its schedule in w
+template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool go, NsSchedule& w, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
 {
     static thread_local NsItem large[4096];
     static thread_local NssItem small[4096];
@@ -1021,12 +1021,11 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
     int rc = ns_plan(d, p, large, small, ws);
     if (rc) return rc;
     if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255)) return set_error(SAUNET_BAD_SHAPE, "%s: the workspace has to hold %ld bytes on a 256-byte border", who, p.bytes);
-    NsSchedule w;
     // Steps composed at once: see the head of this file.  The longest matrix is the first.  (Short ones in twos would gain little: one of 128 x 256 183 us,
     // step by step 171; sixty of 128 x 64 .. 992 299 us against 324.)
     const bool compose = p.large && (large[0].rows < large[0].cols ? large[0].rows : large[0].cols) > NS_MID && p.shortest > 32 && (double)d->a * d->a <= 16.0;
     const int first = !compose ? 1 : !MUON && p.shortest < 256 ? 2 : 3, later = compose ? 2 : 1;
-    if (!ns_schedule(d, first, later, w)) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
+    if (!go && !ns_schedule(d, first, later, w)) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
     if (!go) return SAUNET_OK;
     for (long i = 0; i < p.small; i += NSS_CHUNK) {
         NssItems ch;
@@ -1074,10 +1073,11 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
 template <typename T, bool MUON> static int ns_run_all(const saunet_ns_desc* d, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
 {
     static thread_local saunet_ns_item item[4096];
+    static thread_local NsSchedule w[2];
     for (int pass = 0; pass < 2; ++pass)
         for (int k = 0; k < 2; ++k) {
             const saunet_ns_desc part = ns_part(d, MUON, k, item);
-            const int rc = part.count ? ns_run<T, MUON>(&part, pass == 1, hyper, workspace, workspace_bytes, st, who) : SAUNET_OK;
+            const int rc = part.count ? ns_run<T, MUON>(&part, pass == 1, w[k], hyper, workspace, workspace_bytes, st, who) : SAUNET_OK;
             if (rc) return rc;
         }
     return SAUNET_OK;

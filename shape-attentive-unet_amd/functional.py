@@ -2282,7 +2282,7 @@ def ns_workspace(d, device):
 def ns_check_hyper(steps, coefficients, eps):
     if int(steps) != steps or not 1 <= steps <= 32:
         raise ValueError("Newton-Schulz takes 1 to 32 whole steps, got %r" % (steps,))
-    if len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients):
+    if len(coefficients) != 3 or not math.isfinite(coefficients[0] + coefficients[1] + coefficients[2]):
         raise ValueError("Newton-Schulz coefficients are three finite numbers, got %r" % (coefficients,))
     if not eps >= 1e-30 or not math.isfinite(eps):
         raise ValueError("Newton-Schulz eps has to be a positive number, got %r" % (eps,))
