@@ -41,14 +41,14 @@ struct NsView {
     char *x, *s0; long bx, bs;
     static long bytes(int rows, int cols)
     {
-        const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows, mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
+        const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows, mp = (m + 63) / 64 * 64, np = (n + 63) / 64 * 64;
         return 3 * mp * np * 4 + NS_NSYM * mp * mp * 4;
     }
     __device__ explicit NsView(const NsItem& it)
     {
         tall = it.rows > it.cols;
         m = tall ? it.cols : it.rows; n = tall ? it.rows : it.cols;
-        mp = (m + 31) / 32 * 32; np = (n + 31) / 32 * 32;
+        mp = (m + 63) / 64 * 64; np = (n + 63) / 64 * 64;
         bx = (long)mp * np * 4; bs = (long)mp * mp * 4;
         x = it.ws; s0 = x + 3 * bx;
     }
@@ -181,9 +181,11 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_
 }
 
 // ---- products -----------------------------------------------------------------------------------------------------------------------
-// 64 KB of LDS, two workgroups a CU.  (Twice the stages in one workgroup a CU brought nothing, also where a launch has fewer workgroups than CUs.)
+// 64 KB of LDS, two workgroups a CU.  (Twice the stages in one workgroup a CU brought nothing, also where a launch has fewer workgroups than CUs.)  The
+// small tile takes 64 elements a stage: half the barriers, 13.6 -> 11.5 us a launch at 512 rows, 19.2 -> 18.1 over SAUNet's list; matrices are padded to
+// 64 for it.
 typedef NtCore<NtF16Pair, 128, 128, 2, 2, 2> NsCore128;
-typedef NtCore<NtF16Pair, 64, 64, 2, 2, 4> NsCore64;
+typedef NtCore<NtF16Pair2, 64, 64, 2, 2, 2> NsCore64;
 typedef NtCore<NtF16Pair, 128, 128, 4, 2, 2> NsCore128W;         // eight waves, for launches without a second workgroup for every CU (six 1000 x 1024 matrices 755 -> 701 us; 4096 x 4096 with it throughout 4219 -> 4699)
 constexpr int NS_SLOTS = 512;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4_t;
@@ -430,10 +432,10 @@ template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) voi
     int t = id - sl.p, sp = 0, parts = 1, ti, tj;
     if (t >= sl.full) { sp = (t - sl.full) / cut; t = sl.full + (t - sl.full) % cut; parts = sl.s; }       // neighbours work on one stretch of the reduction
     ns_lower(t, nt, ti, tj);
-    const int steps = (p.a == NS_X ? v.np : v.mp) / 32, k0 = (int)((long)steps * sp / parts), k1 = (int)((long)steps * (sp + 1) / parts);
-    const long ld = steps * 128L;
-    const char* a = (p.a == NS_X ? v.x : v.sym(p.a)) + k0 * 128L;
-    const char* b = (p.a == NS_X ? v.x : v.sym(p.b)) + k0 * 128L;
+    const int steps = (p.a == NS_X ? v.np : v.mp) * 4 / Core::RB, k0 = (int)((long)steps * sp / parts), k1 = (int)((long)steps * (sp + 1) / parts);
+    const long ld = (long)steps * Core::RB;
+    const char* a = (p.a == NS_X ? v.x : v.sym(p.a)) + (long)k0 * Core::RB;
+    const char* b = (p.a == NS_X ? v.x : v.sym(p.b)) + (long)k0 * Core::RB;
     f32x16 acc[Core::TM][Core::TN] = {};
     Core::run(a + ti * T * ld, (unsigned)ld, v.mp - ti * T, b + tj * T * ld, (unsigned)ld, v.mp - tj * T, k1 - k0, smem, acc);
     typedef NsQuads<Core> Quads;
@@ -513,7 +515,7 @@ template <class Core, typename T, int MODE> __global__ __launch_bounds__(Core::N
     nt_band(id - it.p_app, (v.np + B - 1) / B, (v.mp + B - 1) / B, tj, ti);
     f32x16 acc[Core::TM][Core::TN] = {};
     const long ld = (long)v.mp * 4;
-    Core::run(v.sym(q) + ti * B * ld, (unsigned)ld, v.mp - ti * B, v.xt(xt) + tj * B * ld, (unsigned)ld, v.np - tj * B, v.mp / 32, smem, acc);
+    Core::run(v.sym(q) + ti * B * ld, (unsigned)ld, v.mp - ti * B, v.xt(xt) + tj * B * ld, (unsigned)ld, v.np - tj * B, v.mp * 4 / Core::RB, smem, acc);
     typedef NsQuads<Core> Quads;
     typedef NsTile<Core> Tile;
     const long oji = (long)tj * B * ld + ti * B * 4;
@@ -847,7 +849,7 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
     p.tile_n = a128 <= 128 ? 64 : 128;
     for (long i = 0; i < p.large; ++i) {
         NsItem& o = large[i];
-        const long m = o.rows < o.cols ? o.rows : o.cols, n = o.rows < o.cols ? o.cols : o.rows, mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
+        const long m = o.rows < o.cols ? o.rows : o.cols, n = o.rows < o.cols ? o.cols : o.rows, mp = (m + 63) / 64 * 64, np = (n + 63) / 64 * 64;
         const long tm = (m + p.tile_m - 1) / p.tile_m, tg = (m + p.tile_g - 1) / p.tile_g;
         o.p_norm = (int)p.norm; o.p_pack = (int)p.pack; o.p_app = (int)p.app;
         tiles[0][i] = (int)(tg * (tg + 1) / 2); tiles[1][i] = (int)(tm * (tm + 1) / 2); gram[i] = (int)(np / 32); sym[i] = (int)(mp / 32);

@@ -2,8 +2,8 @@
 //
 // A stage holds RB bytes of every row of the tile (BM rows of A, BN rows of B).  One DMA instruction of a wave lands 1 KB lane-linear in LDS, so the
 // 16-byte XOR swizzle that spreads a fragment read over all banks is applied to the per-lane SOURCE address and again on the read: LDS row r
-// holds source chunk (slot ^ key(r)).  ST buffers form a ring.  A stage is two half steps; the fragments of each are read while the MFMAs of the one before
-// run.  The one barrier of a stage stands between its halves, when its last fragments are in registers: behind it the buffer takes the requests of stage
+// holds source chunk (slot ^ key(r)).  ST buffers form a ring.  A stage is two (four) steps; the fragments of each are read while the MFMAs of the one before
+// run.  The one barrier of a stage stands in front of its last step, when its last fragments are in registers: behind it the buffer takes the requests of stage
 // s + ST, and stage s + 1, whose requests every wave has waited for with a counted vmcnt, is read.
 //
 // Operand rows beyond the matrix are clamped to its last row: they are read, multiplied and never stored.  The reduction length is a whole number of
@@ -64,6 +64,11 @@ struct NtF16Pair {
         c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a[0]), __builtin_bit_cast(f16x8_t, b[0]), c, 0, 0, 0);
     }
 };
+// two such blocks a stage: half the barriers, for tiles that do not need two workgroups a CU
+struct NtF16Pair2 : NtF16Pair {
+    static constexpr int RB = 256, KSUB = 4, FLUSH = 4;
+    static __device__ __forceinline__ int chunk(int ks, int part, int half) { return (ks >> 1) * 8 + part * 4 + (ks & 1) * 2 + half; }
+};
 // int8, 64 elements a stage
 struct NtI8 {
     static constexpr int RB = 64, KSUB = 2, PARTS = 1, FLUSH = 0;          // integer sums are exact
@@ -83,11 +88,11 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
     static constexpr int STAGE = (BM + BN) * RB, LDS = ST * STAGE, CPR = RB / 16, RPI = 1024 / RB;
     static constexpr int QA = BM * RB / 1024 / NW, QB = BN * RB / 1024 / NW, LPW = QA + QB;
     static_assert(QA * NW * 1024 == BM * RB && QB * NW * 1024 == BN * RB, "every wave requests whole instructions of one operand");
-    static_assert(ST >= 2 && ST <= 8 && (ST - 1) * LPW < 64 && Op::KSUB == 2, "vmcnt counts to 63");
+    static_assert(ST >= 2 && ST <= 8 && (ST - 1) * LPW < 64 && (Op::KSUB == 2 || Op::KSUB == 4), "vmcnt counts to 63");
     typedef typename Op::Acc Acc;
 
-    // 256 bytes of LDS answer at once: 2 (4) rows of the tile beside each other, so rows that agree modulo 2 (4) have to differ in their key
-    static __device__ __forceinline__ int key(int row) { return CPR == 8 ? ((row >> 1) & 7) : ((row >> 2) & 3); }
+    // 256 bytes of LDS answer at once: 1 (2, 4) rows of the tile beside each other, so rows that agree modulo 1 (2, 4) have to differ in their key
+    static __device__ __forceinline__ int key(int row) { return CPR == 16 ? (row & 15) : CPR == 8 ? ((row >> 1) & 7) : ((row >> 2) & 3); }
 
     // a, b: first byte of the tile's first row at its first stage (uniform); arows, brows: rows that exist from there on (>= 1)
     static __device__ __forceinline__ void run(const char* a, unsigned lda, int arows, const char* b, unsigned ldb, int brows, int ksteps, unsigned char* smem,
@@ -126,16 +131,16 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
             for (int p = 0; p < Op::PARTS; ++p) {
                 const int at = (Op::chunk(ks, p, half) ^ k0) * 16;
 #pragma unroll
-                for (int i = 0; i < TM; ++i) fa[ks][i][p] = *(const u32x4*)(sa + i * 32 * RB + at);
+                for (int i = 0; i < TM; ++i) fa[ks & 1][i][p] = *(const u32x4*)(sa + i * 32 * RB + at);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) fb[ks][j][p] = *(const u32x4*)(sb + j * 32 * RB + at);
+                for (int j = 0; j < TN; ++j) fb[ks & 1][j][p] = *(const u32x4*)(sb + j * 32 * RB + at);
             }
         };
         auto mma = [&](int ks) {
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) Op::mma(fa[ks][i], fb[ks][j], acc[i][j]);
+                for (int j = 0; j < TN; ++j) Op::mma(fa[ks & 1][i], fb[ks & 1][j], acc[i][j]);
         };
         // this wave's LDS reads are in registers, its requests of all but the newest `young` stages have landed; then the workgroup's have
         auto settle = [&](int young) {
@@ -154,17 +159,20 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
         settle((ksteps < ST ? ksteps : ST) - 1);
         read(0, 0);
         for (int s = 0; s < ksteps; ++s) {
-            read(s, 1);
-            __builtin_amdgcn_sched_barrier(0);
-            mma(0);
-            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks + 1 < Op::KSUB; ++ks) {
+                read(s, ks + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                mma(ks);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if (s + 1 < ksteps) {
                 settle(ksteps - 2 - s < ST - 2 ? ksteps - 2 - s : ST - 2);          // stage s + 1 is there; nobody reads stage s any more
                 if (s + ST < ksteps) issue(s + ST);
                 read(s + 1, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
-            mma(1);
+            mma(Op::KSUB - 1);
             __builtin_amdgcn_sched_barrier(0);
             if (Op::FLUSH && ((s & (Op::FLUSH - 1)) == Op::FLUSH - 1 || s + 1 == ksteps)) {
 #pragma unroll
