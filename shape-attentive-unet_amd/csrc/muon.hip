@@ -29,6 +29,13 @@ struct NsItem {            // one matrix, as the host lays it out
     int ld_src, ld_dst, rows, cols;
     int p_norm, p_pack, p_app;       // index of the matrix's first workgroup in the launches of each kind
     NsSplit split[NS_KINDS];
+    // (number by number: an index that the compiler does not know, or a choice between whole structures, puts them into scratch memory: 2 - 3 us a launch)
+    __device__ __forceinline__ NsSplit of(int kind) const
+    {
+        const bool g = kind == NS_GRAM, o = kind == NS_ONE;
+        const NsSplit x = split[NS_GRAM], y = split[NS_ONE], z = split[NS_TWO];
+        return NsSplit{g ? x.p : o ? y.p : z.p, g ? x.full : o ? y.full : z.full, g ? x.s : o ? y.s : z.s, g ? x.c : o ? y.c : z.c};
+    }
 };
 constexpr int NS_CHUNK = 36;                 // of them are kernel arguments
 struct NsItems { NsItem it[NS_CHUNK]; };
@@ -70,6 +77,15 @@ template <typename F> __device__ __forceinline__ int ns_find(int count, int id, 
     return __builtin_amdgcn_readfirstlane(base + __popcll(__ballot((step == 1 || lane < step) && i < count && first(i < count ? i : 0) <= id)) - 1);
 }
 
+// A single matrix is a kernel argument (the table of others is two loads one after the other in front of every tile) and needs no set-up launch:
+// 512 x 13824 310 -> 303 us a call
+struct NsTable { const NsItem* all; int count; NsItem one; };
+template <typename F> __device__ __forceinline__ NsItem ns_item(const NsTable& t, int id, F first)
+{
+    if (t.count == 1) return t.one;
+    return t.all[ns_find(t.count, id, [&](int i) { return first(t.all[i]); })];
+}
+
 __global__ void ns_setup_kernel(NsItems items, int count, NsItem* __restrict__ tab)
 {
     if ((int)threadIdx.x < count) tab[threadIdx.x] = items.it[threadIdx.x];
@@ -95,11 +111,11 @@ __device__ __forceinline__ float ns_momentum(float g, float buf, const float* h)
 __device__ __forceinline__ float ns_update(float g, float buf, const float* h) { const float gs = g * h[4]; return h[3] != 0.f ? fmaf(h[1], buf - gs, gs) : buf; }
 
 // ---- sums of squares (and the momentum update): float64 partials of NS_NORM elements each, summed in index order by the pack pass ------------
-template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_norm_kernel(const NsItem* __restrict__ tab, int count, const float* __restrict__ hyper, double* __restrict__ part)
+template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_norm_kernel(NsTable tab, const float* __restrict__ hyper, double* __restrict__ part)
 {
     __shared__ double s_sum[4];
     const int id = blockIdx.x;
-    const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].p_norm; })];
+    const NsItem it = ns_item(tab, id, [&](const NsItem& t) { return t.p_norm; });
     const long total = (long)it.rows * it.cols, e0 = (long)(id - it.p_norm) * NS_NORM;
     float h[5] = {0.f, 0.f, 0.f, 0.f, 1.f};
     if (MUON) for (int i = 0; i < 5; ++i) h[i] = hyper[i];
@@ -128,12 +144,12 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_norm_
 }
 
 // ---- X0 and X0^T as scaled float16 pairs: a workgroup takes 64 x 64 elements --------------------------------------------------------
-template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_kernel(const NsItem* __restrict__ tab, int count, const float* __restrict__ hyper, const double* __restrict__ part, float eps, float sx)
+template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_kernel(NsTable tab, const float* __restrict__ hyper, const double* __restrict__ part, float eps, float sx)
 {
     __shared__ float s_t[64][65];
     __shared__ double s_sum[4];
     const int tid = threadIdx.x, id = blockIdx.x;
-    const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].p_pack; })];
+    const NsItem it = ns_item(tab, id, [&](const NsItem& t) { return t.p_pack; });
     const NsView v(it);
     float h[5] = {0.f, 0.f, 0.f, 0.f, 1.f};
     if (MUON) for (int i = 0; i < 5; ++i) h[i] = hyper[i];
@@ -397,7 +413,14 @@ __device__ __forceinline__ int ns_dealt(const NsDeal& d, int id)
 // written.  blockIdx.y picks the product: the two of one phase are independent.  The tiles behind the first split.full are cut along the reduction into
 // split.s parts, whose float32 sums go to memory in accumulator order for ns_finish_kernel.
 struct NsProd { int a, b, e, f, d; float alpha, beta, gamma, diag; };          // diag: added to the diagonal of a product with an E
-struct NsProds { NsProd p[2]; };
+struct NsProds {
+    NsProd p[2];
+    __device__ __forceinline__ NsProd of(int y) const
+    {
+        const NsProd u = p[0], v = p[1];
+        return NsProd{y ? v.a : u.a, y ? v.b : u.b, y ? v.e : u.e, y ? v.f : u.f, y ? v.d : u.d, y ? v.alpha : u.alpha, y ? v.beta : u.beta, y ? v.gamma : u.gamma, y ? v.diag : u.diag};
+    }
+};
 
 // blends E and F into a whole tile and stores it with its mirror image
 template <class Core> __device__ __forceinline__ void ns_prod_end(const NsView& v, const NsProd& p, int ti, int tj, f32x16 (&acc)[Core::TM][Core::TN], unsigned char* smem)
@@ -417,17 +440,17 @@ template <class Core> __device__ __forceinline__ void ns_prod_end(const NsView& 
     Tile::store_t(acc, alpha, v.sym(p.d) + oji, ls, rj, ri, ti == tj, smem);
     if (ti != tj) Tile::store(acc, alpha, v.sym(p.d) + oij, ls, ri, rj, smem);
 }
-template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) void ns_prod_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr, NsDeal deal, int tail)
+template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) void ns_prod_kernel(NsTable tab, int kind, NsProds pr, NsDeal deal, int tail)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     constexpr int T = Core::BM;
     // (deal ends at the first cut tile of a single matrix: its parts follow in launch order, behind a whole number of rounds)
     const int id = (int)blockIdx.x < tail ? ns_dealt(deal, blockIdx.x) : deal.b[8] + (int)blockIdx.x - tail;
     if (id < 0) return;
-    const NsProd p = blockIdx.y ? pr.p[1] : pr.p[0];
-    const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].split[kind].p; })];
+    const NsProd p = pr.of(blockIdx.y);
+    const NsItem it = ns_item(tab, id, [&](const NsItem& t) { return t.split[kind].p; });
     const NsView v(it);
-    const NsSplit sl = it.split[kind];
+    const NsSplit sl = it.of(kind);
     const int nt = (v.mp + T - 1) / T, cut = nt * (nt + 1) / 2 - sl.full;
     int t = id - sl.p, sp = 0, parts = 1, ti, tj;
     if (t >= sl.full) { sp = (t - sl.full) / cut; t = sl.full + (t - sl.full) % cut; parts = sl.s; }       // neighbours work on one stretch of the reduction
@@ -447,13 +470,13 @@ template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) voi
     ns_prod_end<Core>(v, p, ti, tj, acc, smem);
 }
 // one accumulator quad of a cut tile a thread; blockIdx.x = tile * quads + quad
-template <class Core> __global__ __launch_bounds__(Core::NT) void ns_finish_kernel(const NsItem* __restrict__ tab, int count, int kind, NsProds pr)
+template <class Core> __global__ __launch_bounds__(Core::NT) void ns_finish_kernel(NsTable tab, int kind, NsProds pr)
 {
     constexpr int T = Core::BM, N = NsQuads<Core>::N;
     const int id = blockIdx.x / N, q = blockIdx.x % N;
-    const NsProd p = blockIdx.y ? pr.p[1] : pr.p[0];
-    const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].split[kind].c; })];
-    const NsSplit sl = it.split[kind];
+    const NsProd p = pr.of(blockIdx.y);
+    const NsItem it = ns_item(tab, id, [&](const NsItem& t) { return t.split[kind].c; });
+    const NsSplit sl = it.of(kind);
     const int t = sl.full + id - sl.c;
     const NsView v(it);
     const int nt = (v.mp + T - 1) / T, cut = nt * (nt + 1) / 2 - sl.full;
@@ -503,13 +526,13 @@ __device__ __forceinline__ void ns_rates(const float* hyper, int rows, int cols,
 }
 
 // X <- alpha Q X + beta X.  MODE 0: back to X and the other X^T; 1: to the caller's matrix; 2: the Muon update of the caller's parameter
-template <class Core, typename T, int MODE> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) void ns_apply_kernel(const NsItem* __restrict__ tab, int count, int q, int xt, float alpha, float beta, const float* __restrict__ hyper, int adjust, NsDeal deal)
+template <class Core, typename T, int MODE> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) void ns_apply_kernel(NsTable tab, int q, int xt, float alpha, float beta, const float* __restrict__ hyper, int adjust, NsDeal deal)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     constexpr int B = Core::BM;
     const int id = ns_dealt(deal, blockIdx.x);
     if (id < 0) return;
-    const NsItem it = tab[ns_find(count, id, [&](int i) { return tab[i].p_app; })];
+    const NsItem it = ns_item(tab, id, [&](const NsItem& t) { return t.p_app; });
     const NsView v(it);
     int ti, tj;
     nt_band(id - it.p_app, (v.np + B - 1) / B, (v.mp + B - 1) / B, tj, ti);
@@ -979,20 +1002,20 @@ static bool ns_schedule(const saunet_ns_desc* d, int first, int later, NsSchedul
     return true;
 }
 
-template <class Core, typename T, int MODE> static void ns_launch_apply(const saunet_ns_desc* d, const NsPlan& p, const NsItem* tab, const NsOp& o, const float* hyper, hipStream_t st)
+template <class Core, typename T, int MODE> static void ns_launch_apply(const saunet_ns_desc* d, const NsPlan& p, const NsTable& tab, const NsOp& o, const float* hyper, hipStream_t st)
 {
     static DeviceOnce once;
     if (once.first()) (void)hipFuncSetAttribute((const void*)ns_apply_kernel<Core, T, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
-    hipLaunchKernelGGL((ns_apply_kernel<Core, T, MODE>), dim3(ns_deal_grid(p.deal[NS_KINDS])), dim3(Core::NT), Core::LDS, st, tab, (int)p.large, o.q, o.xt, o.alpha, o.beta, hyper, d->adjust, p.deal[NS_KINDS]);
+    hipLaunchKernelGGL((ns_apply_kernel<Core, T, MODE>), dim3(ns_deal_grid(p.deal[NS_KINDS])), dim3(Core::NT), Core::LDS, st, tab, o.q, o.xt, o.alpha, o.beta, hyper, d->adjust, p.deal[NS_KINDS]);
 }
-template <class Core> static void ns_launch_prod(const NsPlan& p, const NsItem* tab, const NsOp& o, hipStream_t st)
+template <class Core> static void ns_launch_prod(const NsPlan& p, const NsTable& tab, const NsOp& o, hipStream_t st)
 {
     const int kind = o.gram ? NS_GRAM : o.ny == 2 ? NS_TWO : NS_ONE;
     static DeviceOnce once;
     if (once.first()) (void)hipFuncSetAttribute((const void*)ns_prod_kernel<Core>, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
     const unsigned dealt = ns_deal_grid(p.deal[kind]);
-    hipLaunchKernelGGL((ns_prod_kernel<Core>), dim3(dealt + (unsigned)(p.grid[kind] - p.deal[kind].b[8]), o.ny), dim3(Core::NT), Core::LDS, st, tab, (int)p.large, kind, o.pr, p.deal[kind], (int)dealt);
-    if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(Core::NT), 0, st, tab, (int)p.large, kind, o.pr);
+    hipLaunchKernelGGL((ns_prod_kernel<Core>), dim3(dealt + (unsigned)(p.grid[kind] - p.deal[kind].b[8]), o.ny), dim3(Core::NT), Core::LDS, st, tab, kind, o.pr, p.deal[kind], (int)dealt);
+    if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(Core::NT), 0, st, tab, kind, o.pr);
 }
 
 // The matrices with up to NS_MID rows and the others are two chains of launches: the short ones go step by step and keep the digits that composing would cost
@@ -1042,17 +1065,17 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
         SAUNET_CHECK_LAUNCH("nss_apply");
     }
     if (!p.large) return SAUNET_OK;
-    NsItem* tab = (NsItem*)(ws + p.tab_at);
+    const NsTable tab = {(const NsItem*)(ws + p.tab_at), (int)p.large, large[0]};
     double* part = (double*)(ws + p.part_at);
     const int n = (int)p.large;
-    for (int i = 0; i < n; i += NS_CHUNK) {
+    for (int i = 0; n > 1 && i < n; i += NS_CHUNK) {
         NsItems ch;
         const int k = n - i < NS_CHUNK ? n - i : NS_CHUNK;
         memcpy(ch.it, large + i, sizeof(NsItem) * k);
-        hipLaunchKernelGGL(ns_setup_kernel, dim3(1), dim3(64), 0, st, ch, k, tab + i);
+        hipLaunchKernelGGL(ns_setup_kernel, dim3(1), dim3(64), 0, st, ch, k, (NsItem*)tab.all + i);
     }
-    hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)p.norm), dim3(256), 0, st, tab, n, hyper, part);
-    hipLaunchKernelGGL((ns_pack_kernel<T, MUON>), dim3((unsigned)p.pack), dim3(256), 0, st, tab, n, hyper, part, d->eps, w.sx);
+    hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)p.norm), dim3(256), 0, st, tab, hyper, part);
+    hipLaunchKernelGGL((ns_pack_kernel<T, MUON>), dim3((unsigned)p.pack), dim3(256), 0, st, tab, hyper, part, d->eps, w.sx);
     SAUNET_CHECK_LAUNCH("ns_pack");
     for (int i = 0; i < w.count; ++i) {
         const NsOp& o = w.op[i];

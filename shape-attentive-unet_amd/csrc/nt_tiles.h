@@ -64,7 +64,7 @@ struct NtF16Pair {
         c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a[0]), __builtin_bit_cast(f16x8_t, b[0]), c, 0, 0, 0);
     }
 };
-// two such blocks a stage: half the barriers, for tiles that do not need two workgroups a CU
+// two such blocks a stage: half the barriers
 struct NtF16Pair2 : NtF16Pair {
     static constexpr int RB = 256, KSUB = 4, FLUSH = 4;
     static __device__ __forceinline__ int chunk(int ks, int part, int half) { return (ks >> 1) * 8 + part * 4 + (ks & 1) * 2 + half; }
