@@ -203,16 +203,18 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_
 typedef NtCore<NtF16Pair, 128, 128, 2, 2, 2> NsCore128;
 typedef NtCore<NtF16Pair2, 64, 64, 2, 2, 2> NsCore64;
 typedef NtCore<NtF16Pair, 128, 128, 4, 2, 2> NsCore128W;         // eight waves, for launches without a second workgroup for every CU (six 1000 x 1024 matrices 755 -> 701 us; 4096 x 4096 with it throughout 4219 -> 4699)
+typedef NtCore<NtF16Pair2, 32, 32, 1, 1, 4, 4> NsCore32;           // four waves share one reduction; never cut
 constexpr int NS_SLOTS = 512;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4_t;
 typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 
 // Accumulator quad b of a thread: the four rows i .. i + 3 of column j, relative to the tile
 template <class Core> struct NsQuads {
-    static constexpr int N = Core::TM * Core::TN * 4, FLOATS = Core::BM * Core::BN;
+    static constexpr int N = Core::TM * Core::TN * 4 / Core::KW, FLOATS = Core::BM * Core::BN;          // (of a shared reduction a wave keeps group `wave`)
+    static __device__ __forceinline__ int group(int b) { return Core::KW > 1 ? (int)threadIdx.x >> 6 : b & 3; }
     static __device__ __forceinline__ void at(int b, int& i, int& j)
     {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ti = b / (4 * Core::TN), tj = b / 4 % Core::TN, g = b & 3;
+        const int lane = threadIdx.x & 63, wave = Core::KW > 1 ? 0 : threadIdx.x >> 6, ti = b / (4 * Core::TN), tj = b / 4 % Core::TN, g = group(b);
         i = (wave / Core::WGN) * (Core::BM / Core::WGM) + ti * 32 + g * 8 + (lane >> 5) * 4;
         j = (wave % Core::WGN) * (Core::BN / Core::WGN) + tj * 32 + (lane & 31);
     }
@@ -268,7 +270,7 @@ template <class Core> struct NsTile {
         unsigned t0, tx, u0, ux;                       // row start and chunk swap of either
         __device__ __forceinline__ Where()
         {
-            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31, t = l & 3;
+            const int lane = threadIdx.x & 63, wave = Core::KW > 1 ? 0 : threadIdx.x >> 6, half = lane >> 5, l = lane & 31, t = l & 3;
             const int wi = (wave / Core::WGN) * (B / Core::WGM), wj = (wave % Core::WGN) * (B / Core::WGN);
             t0 = (wj + l) * ROW + half * 8;
             tx = ((wi / 32 * 8) ^ (l & (CH - 1))) * 16;
@@ -277,12 +279,12 @@ template <class Core> struct NsTile {
         }
         __device__ __forceinline__ unsigned tile_t(int b) const          // quad b of tile (ti, tj), group g
         {
-            const int ti = b / (4 * Core::TN), tj = b / 4 % Core::TN, g = b & 3;
+            const int ti = b / (4 * Core::TN), tj = b / 4 % Core::TN, g = Quads::group(b);
             return t0 + tj * 32 * ROW + (tx ^ ((ti * 8 + g) * 16));
         }
         __device__ __forceinline__ unsigned tile(int b) const
         {
-            const int ti = b / (4 * Core::TN), tj = b / 4 % Core::TN, g = b & 3;
+            const int ti = b / (4 * Core::TN), tj = b / 4 % Core::TN, g = Quads::group(b);
             return u0 + (ti * 32 + g * 8) * ROW + (ux ^ (((tj * 8) ^ ((g * 8) & (CH - 1))) * 16));
         }
     };
@@ -422,6 +424,23 @@ struct NsProds {
     }
 };
 
+// The waves of a shared reduction add their sums, in the order of the waves: wave w ends with quad w of each lane
+template <class Core> __device__ __forceinline__ void ns_join(f32x16 (&acc)[Core::TM][Core::TN], unsigned char* smem)
+{
+    static_assert(Core::KW == 4 && Core::NW == 4 && Core::LDS >= 16384, "a 32 x 32 tile");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    nt_wait_barrier<0>();
+    f32x4* s = (f32x4*)smem;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) s[(wave * 4 + g) * 64 + lane] = f32x4{acc[0][0][g * 4], acc[0][0][g * 4 + 1], acc[0][0][g * 4 + 2], acc[0][0][g * 4 + 3]};
+    __syncthreads();
+    f32x4 c = s[wave * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) { const f32x4 x = s[(w * 4 + wave) * 64 + lane]; for (int r = 0; r < 4; ++r) c[r] += x[r]; }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[0][0][r] = c[r];
+}
+
 // blends E and F into a whole tile and stores it with its mirror image
 template <class Core> __device__ __forceinline__ void ns_prod_end(const NsView& v, const NsProd& p, int ti, int tj, f32x16 (&acc)[Core::TM][Core::TN], unsigned char* smem)
 {
@@ -461,6 +480,7 @@ template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) voi
     const char* b = (p.a == NS_X ? v.x : v.sym(p.b)) + (long)k0 * Core::RB;
     f32x16 acc[Core::TM][Core::TN] = {};
     Core::run(a + ti * T * ld, (unsigned)ld, v.mp - ti * T, b + tj * T * ld, (unsigned)ld, v.mp - tj * T, k1 - k0, smem, acc);
+    if constexpr (Core::KW > 1) ns_join<Core>(acc, smem);
     typedef NsQuads<Core> Quads;
     if (parts > 1) {
         float* d = v.part() + (((long)blockIdx.y * cut + t - sl.full) * parts + sp) * Quads::FLOATS + threadIdx.x * 4;
@@ -539,6 +559,7 @@ template <class Core, typename T, int MODE> __global__ __launch_bounds__(Core::N
     f32x16 acc[Core::TM][Core::TN] = {};
     const long ld = (long)v.mp * 4;
     Core::run(v.sym(q) + ti * B * ld, (unsigned)ld, v.mp - ti * B, v.xt(xt) + tj * B * ld, (unsigned)ld, v.np - tj * B, v.mp * 4 / Core::RB, smem, acc);
+    if constexpr (Core::KW > 1) ns_join<Core>(acc, smem);
     typedef NsQuads<Core> Quads;
     typedef NsTile<Core> Tile;
     const long oji = (long)tj * B * ld + ti * B * 4;
@@ -782,17 +803,17 @@ static bool ns_is_small(const saunet_ns_desc* d, const saunet_ns_item& t)
     for (int i = 1; i < d->steps; ++i) grow *= (double)d->a * d->a;
     return (t.rows < t.cols ? t.rows : t.cols) <= 32 && grow <= 1e8;
 }
-// Cuts along the reduction, for one kind of launch (ny products a tile, steps[i] reduction steps of matrix i).  A tile longer than an even share of the
+// Cuts along the reduction, for one kind of launch (ny products a tile, steps[i] reduction steps of matrix i; none if `whole`).  A tile longer than an even share of the
 // launch's work is cut into shares (sixteen steps at least) where that saves 32 steps: they are 11 us, the finishing launch costs 8 (six 1000 x 1024
 // matrices in two parts of sixteen: 41 -> 33 us for the products, 14 more to finish).  A single matrix of a few rounds of NS_SLOTS workgroups whose last
 // round is less than half full has that round's tiles cut: 4096 x 4096, 528 tiles on 512 slots, 262 us -> 200 + 11.
-static void ns_cut(int kind, int ny, NsPlan& p, const int* tiles, const int* steps, int count, NsItem* out)
+static void ns_cut(int kind, int ny, bool whole, NsPlan& p, const int* tiles, const int* steps, int count, NsItem* out)
 {
     long total = 0, at = 0, work = 0;
     for (int i = 0; i < count; ++i) { total += (long)tiles[i] * ny; work += (long)tiles[i] * ny * steps[i]; }
     const long share = work / NS_SLOTS > 16 ? work / NS_SLOTS : 16;
     long tail = 0, tail_s = 1;
-    if (count == 1 && total > NS_SLOTS && total < 4 * NS_SLOTS && total % NS_SLOTS && total % NS_SLOTS <= NS_SLOTS / 2) {
+    if (!whole && count == 1 && total > NS_SLOTS && total < 4 * NS_SLOTS && total % NS_SLOTS && total % NS_SLOTS <= NS_SLOTS / 2) {
         tail = (total % NS_SLOTS + ny - 1) / ny;
         tail_s = NS_SLOTS / (tail * ny);
         if (tail_s > steps[0] / 8) tail_s = steps[0] / 8;
@@ -802,7 +823,7 @@ static void ns_cut(int kind, int ny, NsPlan& p, const int* tiles, const int* ste
     for (int i = 0; i < count; ++i) {
         NsSplit s = {(int)at, tiles[i], 1, (int)p.cut[kind]};
         if (tail) { s.full = tiles[i] - (int)tail; s.s = (int)tail_s; }
-        else if (steps[i] >= share + 32) { s.full = 0; s.s = (int)((steps[i] + share - 1) / share); }
+        else if (!whole && steps[i] >= share + 32) { s.full = 0; s.s = (int)((steps[i] + share - 1) / share); }
         p.cut[kind] += tiles[i] - s.full;
         at += s.full + (long)(tiles[i] - s.full) * s.s;
         out[i].split[kind] = s;
@@ -843,7 +864,7 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
 {
     static thread_local int tiles[2][4096], gram[4096], sym[4096];
     p = NsPlan();
-    long w128 = 0, a128 = 0, g128 = 0;
+    long w128 = 0, a128 = 0, g128 = 0, w64 = 0, a64 = 0, longest = 0;
     for (int i = 0; i < d->count; ++i) {
         const saunet_ns_item& t = d->item[i];
         const long m = t.rows < t.cols ? t.rows : t.cols, n = t.rows < t.cols ? t.cols : t.rows;
@@ -859,6 +880,9 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
         o.src = t.src; o.dst = t.dst; o.buf = (float*)t.buf; o.ld_src = (int)t.ld_src; o.ld_dst = (int)t.ld_dst; o.rows = t.rows; o.cols = t.cols;
         w128 += (m + 127) / 128 * ((m + 127) / 128 + 1) / 2 * ((m + 31) / 32);
         a128 += (m + 127) / 128 * ((n + 127) / 128);
+        w64 += (m + 63) / 64 * ((m + 63) / 64 + 1) / 2;
+        a64 += (m + 63) / 64 * ((n + 63) / 64);
+        longest = n > longest ? n : longest;
         g128 += (m + 127) / 128 * ((m + 127) / 128 + 1) / 2 * ((n + 31) / 32);
         if (p.large == 1 || m < p.shortest) p.shortest = m;
     }
@@ -870,22 +894,29 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
     p.tile_g = g128 <= 1024 ? 64 : 128;
     p.tile_m = w128 <= 2048 ? 64 : 128;
     p.tile_n = a128 <= 128 ? 64 : 128;
+    // 32 x 32 tiles, whose waves share one reduction, where even the 64 x 64 ones leave CUs idle: four times the workgroups, a third of the LDS traffic in each
+    // (us a call, replayed; 64 against 32).  m x m products: 3 tiles of 64 98 -> 92, 36 196 -> 156, 90 117 -> 113, but 136 302 -> 337.  Products with X: 8 tiles
+    // 92 -> 86, 126 119 -> 115, but 188 142 -> 144, 240 113 -> 125.  Gram products where they would not be cut: 128 x 1000 130 -> 103, 768 x 1000
+    // 202 -> 194, but 512 x 2000 156 -> 156, 200 x 3000 142 -> 160.
+    if (p.tile_m == 64 && w64 <= 96) p.tile_m = 32;
+    if (p.tile_n == 64 && a64 <= 128) p.tile_n = 32;
+    if (p.tile_g == 64 && w64 <= 96 && longest < 1536) p.tile_g = 32;
     for (long i = 0; i < p.large; ++i) {
         NsItem& o = large[i];
         const long m = o.rows < o.cols ? o.rows : o.cols, n = o.rows < o.cols ? o.cols : o.rows, mp = (m + 63) / 64 * 64, np = (n + 63) / 64 * 64;
-        const long tm = (m + p.tile_m - 1) / p.tile_m, tg = (m + p.tile_g - 1) / p.tile_g;
+        const long tm = (mp + p.tile_m - 1) / p.tile_m, tg = (mp + p.tile_g - 1) / p.tile_g;
         o.p_norm = (int)p.norm; o.p_pack = (int)p.pack; o.p_app = (int)p.app;
         tiles[0][i] = (int)(tg * (tg + 1) / 2); tiles[1][i] = (int)(tm * (tm + 1) / 2); gram[i] = (int)(np / 32); sym[i] = (int)(mp / 32);
         p.norm += (m * n + NS_NORM - 1) / NS_NORM;
         p.pack += ((mp + 63) / 64) * ((np + 63) / 64);
-        p.app += ((m + p.tile_n - 1) / p.tile_n) * ((n + p.tile_n - 1) / p.tile_n);
+        p.app += ((mp + p.tile_n - 1) / p.tile_n) * ((np + p.tile_n - 1) / p.tile_n);
         p.tile += tiles[1][i] + tiles[0][i];
         if (p.norm > 0x3fffffff || p.pack > 0x3fffffff || p.app > 0x3fffffff || p.tile > 0x3ffffff) return set_error(SAUNET_BAD_SHAPE, "newton_schulz: the list is too large for one call");
     }
     if (p.large) {
-        ns_cut(NS_GRAM, 1, p, tiles[0], gram, (int)p.large, large);
-        ns_cut(NS_ONE, 1, p, tiles[1], sym, (int)p.large, large);
-        ns_cut(NS_TWO, 2, p, tiles[1], sym, (int)p.large, large);
+        ns_cut(NS_GRAM, 1, p.tile_g == 32, p, tiles[0], gram, (int)p.large, large);
+        ns_cut(NS_ONE, 1, p.tile_m == 32, p, tiles[1], sym, (int)p.large, large);
+        ns_cut(NS_TWO, 2, p.tile_m == 32, p, tiles[1], sym, (int)p.large, large);
         static thread_local NsRun run[2 * 4096];
         for (int k = 0; k < NS_KINDS; ++k) {
             int n = 0;
@@ -1015,7 +1046,7 @@ template <class Core> static void ns_launch_prod(const NsPlan& p, const NsTable&
     if (once.first()) (void)hipFuncSetAttribute((const void*)ns_prod_kernel<Core>, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
     const unsigned dealt = ns_deal_grid(p.deal[kind]);
     hipLaunchKernelGGL((ns_prod_kernel<Core>), dim3(dealt + (unsigned)(p.grid[kind] - p.deal[kind].b[8]), o.ny), dim3(Core::NT), Core::LDS, st, tab, kind, o.pr, p.deal[kind], (int)dealt);
-    if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(Core::NT), 0, st, tab, kind, o.pr);
+    if constexpr (Core::KW == 1) if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(Core::NT), 0, st, tab, kind, o.pr);
 }
 
 // The matrices with up to NS_MID rows and the others are two chains of launches: the short ones go step by step and keep the digits that composing would cost
@@ -1081,12 +1112,14 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
         const NsOp& o = w.op[i];
         if (o.apply) {
             constexpr int LAST = MUON ? 2 : 1;
-            if (p.tile_n == 64) o.last ? ns_launch_apply<NsCore64, T, LAST>(d, p, tab, o, hyper, st) : ns_launch_apply<NsCore64, T, 0>(d, p, tab, o, hyper, st);
+            if (p.tile_n == 32) o.last ? ns_launch_apply<NsCore32, T, LAST>(d, p, tab, o, hyper, st) : ns_launch_apply<NsCore32, T, 0>(d, p, tab, o, hyper, st);
+            else if (p.tile_n == 64) o.last ? ns_launch_apply<NsCore64, T, LAST>(d, p, tab, o, hyper, st) : ns_launch_apply<NsCore64, T, 0>(d, p, tab, o, hyper, st);
             else o.last ? ns_launch_apply<NsCore128, T, LAST>(d, p, tab, o, hyper, st) : ns_launch_apply<NsCore128, T, 0>(d, p, tab, o, hyper, st);
             SAUNET_CHECK_LAUNCH("ns_apply");
         } else {
             const int kind = o.gram ? NS_GRAM : o.ny == 2 ? NS_TWO : NS_ONE;
-            if ((o.gram ? p.tile_g : p.tile_m) == 64) ns_launch_prod<NsCore64>(p, tab, o, st);
+            if ((o.gram ? p.tile_g : p.tile_m) == 32) ns_launch_prod<NsCore32>(p, tab, o, st);
+            else if ((o.gram ? p.tile_g : p.tile_m) == 64) ns_launch_prod<NsCore64>(p, tab, o, st);
             else if (p.grid[kind] * o.ny <= NS_SLOTS / 2) ns_launch_prod<NsCore128W>(p, tab, o, st);
             else ns_launch_prod<NsCore128>(p, tab, o, st);
             SAUNET_CHECK_LAUNCH("ns_prod");

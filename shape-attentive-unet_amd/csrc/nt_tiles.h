@@ -80,15 +80,16 @@ struct NtI8 {
     }
 };
 
-// BM x BN tile by WGM x WGN waves; wave (wm, wn) owns TM x TN blocks of 32 x 32.  Accumulator element r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4
+// BM x BN tile by WGM x WGN waves; wave (wm, wn) owns TM x TN blocks of 32 x 32.  KW > 1: KW such sets of waves, each of which takes a KW-th of every
+// stage and ends with a sum of its own; the caller adds them.  Accumulator element r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4
 // (operand A), column l % 32 (operand B).
-template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore {
-    static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, ST = ST_, RB = Op::RB;
-    static constexpr int NW = WGM * WGN, NT = NW * 64, TM = BM / WGM / 32, TN = BN / WGN / 32;
+template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_, int KW_ = 1> struct NtCore {
+    static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, ST = ST_, KW = KW_, RB = Op::RB, MY = Op::KSUB / KW;          // MY: steps of a stage that are a wave's
+    static constexpr int NW = WGM * WGN * KW, NT = NW * 64, TM = BM / WGM / 32, TN = BN / WGN / 32;
     static constexpr int STAGE = (BM + BN) * RB, LDS = ST * STAGE, CPR = RB / 16, RPI = 1024 / RB;
     static constexpr int QA = BM * RB / 1024 / NW, QB = BN * RB / 1024 / NW, LPW = QA + QB;
     static_assert(QA * NW * 1024 == BM * RB && QB * NW * 1024 == BN * RB, "every wave requests whole instructions of one operand");
-    static_assert(ST >= 2 && ST <= 8 && (ST - 1) * LPW < 64 && (Op::KSUB == 2 || Op::KSUB == 4), "vmcnt counts to 63");
+    static_assert(ST >= 2 && ST <= 8 && (ST - 1) * LPW < 64 && (MY == 1 || MY == 2 || MY == 4), "vmcnt counts to 63");
     typedef typename Op::Acc Acc;
 
     // 256 bytes of LDS answer at once: 1 (2, 4) rows of the tile beside each other, so rows that agree modulo 1 (2, 4) have to differ in their key
@@ -101,7 +102,7 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
         a = nt_uniform(a); b = nt_uniform(b);
         ksteps = __builtin_amdgcn_readfirstlane(ksteps);
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const int wm = wave / WGN, wn = wave % WGN;
+        const int wk = wave / (WGM * WGN), wm = wave / WGN % WGM, wn = wave % WGN;
         const unsigned lds0 = (unsigned)(uintptr_t)smem;
         unsigned voff[LPW];
 #pragma unroll
@@ -123,24 +124,25 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
         u32x4 fa[2][TM][Op::PARTS], fb[2][TN][Op::PARTS];
         Acc part[TM][TN] = {};
         Acc (&acc)[TM][TN] = Op::FLUSH ? part : total;
-        auto read = [&](int s, int ks) {
+        // step ks of stage s into fragments f
+        auto read = [&](int s, int ks, int f) {
             const unsigned char* st = smem + (s % ST) * STAGE;
             const unsigned char* sa = st + (wm * (BM / WGM) + r0) * RB;
             const unsigned char* sb = st + BM * RB + (wn * (BN / WGN) + r0) * RB;
 #pragma unroll
             for (int p = 0; p < Op::PARTS; ++p) {
-                const int at = (Op::chunk(ks, p, half) ^ k0) * 16;
+                const int at = (Op::chunk(KW > 1 ? wk * MY + ks : ks, p, half) ^ k0) * 16;
 #pragma unroll
-                for (int i = 0; i < TM; ++i) fa[ks & 1][i][p] = *(const u32x4*)(sa + i * 32 * RB + at);
+                for (int i = 0; i < TM; ++i) fa[f][i][p] = *(const u32x4*)(sa + i * 32 * RB + at);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) fb[ks & 1][j][p] = *(const u32x4*)(sb + j * 32 * RB + at);
+                for (int j = 0; j < TN; ++j) fb[f][j][p] = *(const u32x4*)(sb + j * 32 * RB + at);
             }
         };
-        auto mma = [&](int ks) {
+        auto mma = [&](int f) {
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) Op::mma(fa[ks & 1][i], fb[ks & 1][j], acc[i][j]);
+                for (int j = 0; j < TN; ++j) Op::mma(fa[f][i], fb[f][j], acc[i][j]);
         };
         // this wave's LDS reads are in registers, its requests of all but the newest `young` stages have landed; then the workgroup's have
         auto settle = [&](int young) {
@@ -157,22 +159,22 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
         };
         for (int s = 0; s < ST && s < ksteps; ++s) issue(s);
         settle((ksteps < ST ? ksteps : ST) - 1);
-        read(0, 0);
-        for (int s = 0; s < ksteps; ++s) {
+        read(0, 0, 0);
+        auto stage = [&](int s, int odd) {                                              // odd: the fragments that hold its first step
 #pragma unroll
-            for (int ks = 0; ks + 1 < Op::KSUB; ++ks) {
-                read(s, ks + 1);
+            for (int ks = 0; ks + 1 < MY; ++ks) {
+                read(s, ks + 1, (ks + 1) & 1);
                 __builtin_amdgcn_sched_barrier(0);
-                mma(ks);
+                mma(ks & 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (s + 1 < ksteps) {
                 settle(ksteps - 2 - s < ST - 2 ? ksteps - 2 - s : ST - 2);          // stage s + 1 is there; nobody reads stage s any more
                 if (s + ST < ksteps) issue(s + ST);
-                read(s + 1, 0);
+                read(s + 1, 0, MY == 1 ? odd ^ 1 : 0);
             }
             __builtin_amdgcn_sched_barrier(0);
-            mma(Op::KSUB - 1);
+            mma(MY == 1 ? odd : 1);
             __builtin_amdgcn_sched_barrier(0);
             if (Op::FLUSH && ((s & (Op::FLUSH - 1)) == Op::FLUSH - 1 || s + 1 == ksteps)) {
 #pragma unroll
@@ -180,6 +182,11 @@ template <class Op, int BM_, int BN_, int WGM_, int WGN_, int ST_> struct NtCore
 #pragma unroll
                     for (int j = 0; j < TN; ++j) { total[i][j] += part[i][j]; part[i][j] = Acc{}; }
             }
+        };
+        if constexpr (MY == 1) {
+            for (int s = 0; s < ksteps; s += 2) { stage(s, 0); if (s + 1 < ksteps) stage(s + 1, 1); }
+        } else {
+            for (int s = 0; s < ksteps; ++s) stage(s, 0);
         }
     }
 };
