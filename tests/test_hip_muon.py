@@ -129,6 +129,31 @@ def test_newton_schulz_sizes(m, n, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(832, 840), (833, 900), (900, 833), (500, 1535), (1537, 500), (129, 2700), (128, 4096), (4100, 128), (65, 8321), (35, 36)])
+def test_newton_schulz_on_either_side_of_the_tile_rules(m, n):
+    """13 and 14 blocks of 64 rows, Gram sums of up to and above 1536 columns, up to and above 128 blocks of 64 x 64 of X"""
+    g = matrix(m, n, m + n, torch.float32, "lowrank").cuda()
+    check(HF.newton_schulz(g), g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [96, 97, 130])
+def test_lists_on_either_side_of_the_tile_rules(count):
+    """one 64-row block each: 32 x 32 tiles up to 96 of them, 64 x 64 behind; the parameters of a Muon step get what the same matrices get alone"""
+    gs = [matrix(33 + i % 32, 34 + (i * 7) % 60, i).cuda() for i in range(count)]
+    for i, out in enumerate(HF.newton_schulz(gs)):
+        check(out, gs[i])
+    ps = [torch.nn.Parameter(torch.zeros_like(g)) for g in gs]
+    opt = optim.FusedMuon(ps, lr=0.5, momentum=0.0, weight_decay=0.0, nesterov=False)
+    for p, g in zip(ps, gs):
+        p.grad = g.clone()
+    opt.step()
+    for p, g in zip(ps, gs):
+        rate = 0.5 * math.sqrt(max(1.0, g.shape[0] / g.shape[1]))
+        check(-p.detach() / rate, g, noise=4 * 2.0 ** -24)              # the rate, its product, this division and the subtraction: half a step each
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("steps", [1, 2, 3, 4, 6, 7, 8, 9, 12])
 def test_newton_schulz_steps(steps):
     for m, n in ((40, 200), (200, 70), (20, 50), (50, 7)):
