@@ -864,7 +864,7 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
 {
     static thread_local int tiles[2][4096], gram[4096], sym[4096];
     p = NsPlan();
-    long w128 = 0, a128 = 0, g128 = 0, w64 = 0, a64 = 0, longest = 0;
+    long a128 = 0, g128 = 0, w64 = 0, a64 = 0, longest = 0;
     for (int i = 0; i < d->count; ++i) {
         const saunet_ns_item& t = d->item[i];
         const long m = t.rows < t.cols ? t.rows : t.cols, n = t.rows < t.cols ? t.cols : t.rows;
@@ -878,7 +878,6 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
         }
         NsItem& o = large[p.large++];
         o.src = t.src; o.dst = t.dst; o.buf = (float*)t.buf; o.ld_src = (int)t.ld_src; o.ld_dst = (int)t.ld_dst; o.rows = t.rows; o.cols = t.cols;
-        w128 += (m + 127) / 128 * ((m + 127) / 128 + 1) / 2 * ((m + 31) / 32);
         a128 += (m + 127) / 128 * ((n + 127) / 128);
         w64 += (m + 63) / 64 * ((m + 63) / 64 + 1) / 2;
         a64 += (m + 63) / 64 * ((n + 63) / 64);
@@ -888,11 +887,22 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
     }
     // the longest reductions first: what starts last is short
     std::sort(large, large + p.large, [](const NsItem& x, const NsItem& y) { return (x.rows < x.cols ? x.rows : x.cols) > (y.rows < y.cols ? y.rows : y.cols); });
-    // 64 x 64 tiles where the work would leave CUs idle: Gram products by their steps (512 x 13824, 4320 of them: 398 us a call with 64, 380 with 128;
-    // 128 x 256, 8: 217 against 228), the m x m products likewise (SAUNet's list, 1100: 1090 against 1173; six 1000 x 1024, 6900: 942 against 803), the
-    // products with X by their tiles (128 x 256, 2: 196 against 217; 512 x 13824, 432: 423 against 398)
-    p.tile_g = g128 <= 1024 ? 64 : 128;
-    p.tile_m = w128 <= 2048 ? 64 : 128;
+    // 64 x 64 tiles where 128 x 128 ones would leave CUs idle or be mostly padding (us a call, replayed; 128 against 64).
+    // m x m products: as long as the small tiles fill the NS_SLOTS once (1200 x 1300 548 -> 364, 1900 x 2000 865 -> 738, fourteen 500 x 1000 450 -> 391; but
+    // fifteen 512 x 512, 540 tiles, 401 -> 425) or what starts behind that is short (the network's 162 matrices, one of 1000 rows and 60 of 128: 1202 -> 1102),
+    // and twice where the reductions are long (2200^2, 630, 1268 -> 1179; two 1500^2, 600, 917 -> 863; but four 1000 x 1024, 544, 570 -> 618).
+    // Gram products: by their steps (300 x 3000, 564: 150 -> 139; 512 x 4000, 1250: 179 -> 172; but 512 x 8000, 2500: 203 -> 211), and of short sums as the m x m ones
+    // (1900 x 2000 738 -> 716, thirteen 512 x 512 334 -> 325; but 1000 x 3000 342 -> 352).
+    // Products with X: by their tiles (1000 x 1024, 64: 335 -> 304; 512 x 4000, 128: 188 -> 179; but three 1000 x 1024, 192: 535 -> 542).
+    long second = 0, longest_m = 0;                                       // rows of the first small tile of the second round, of the first
+    for (long i = 0, at = 0; i < p.large && !second; ++i) {
+        const long m = large[i].rows < large[i].cols ? large[i].rows : large[i].cols;
+        if (!i) longest_m = m;
+        at += (m + 63) / 64 * ((m + 63) / 64 + 1) / 2;
+        if (at > NS_SLOTS) second = m;
+    }
+    p.tile_m = second * 4 <= longest_m || (w64 <= 2 * NS_SLOTS && p.shortest >= 1200) ? 64 : 128;
+    p.tile_g = g128 <= 1400 || (p.tile_m == 64 && longest <= 2560) ? 64 : 128;
     p.tile_n = a128 <= 128 ? 64 : 128;
     // 32 x 32 tiles, whose waves share one reduction, where even the 64 x 64 ones leave CUs idle: four times the workgroups, a third of the LDS traffic in each
     // (us a call, replayed; 64 against 32).  m x m products: 3 tiles of 64 98 -> 92, 36 196 -> 156, 90 117 -> 113, but 136 302 -> 337.  Products with X: 8 tiles

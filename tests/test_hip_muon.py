@@ -137,6 +137,15 @@ def test_newton_schulz_on_either_side_of_the_tile_rules(m, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(520, 530)] + [(130, 131)] * 100, [(200, 210)] * 60, [(516, 140)] + [(300, 290)] * 30], ids=["short behind", "uniform", "two rounds"])
+def test_lists_of_more_than_one_round_of_tiles(shapes):
+    """more 64 x 64 tiles than run at once, with short and with equal reductions behind the first round"""
+    gs = [matrix(*s, 11 + i).cuda() for i, s in enumerate(shapes)]
+    for out, g in zip(HF.newton_schulz(gs), gs):
+        check(out, g)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("count", [96, 97, 130])
 def test_lists_on_either_side_of_the_tile_rules(count):
     """one 64-row block each: 32 x 32 tiles up to 96 of them, 64 x 64 behind; the parameters of a Muon step get what the same matrices get alone"""
