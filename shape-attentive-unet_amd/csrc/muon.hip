@@ -202,7 +202,8 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_
 // 64 for it.
 typedef NtCore<NtF16Pair, 128, 128, 2, 2, 2> NsCore128;
 typedef NtCore<NtF16Pair2, 64, 64, 2, 2, 2> NsCore64;
-typedef NtCore<NtF16Pair, 128, 128, 4, 2, 2> NsCore128W;         // eight waves, for launches without a second workgroup for every CU (six 1000 x 1024 matrices 755 -> 701 us; 4096 x 4096 with it throughout 4219 -> 4699)
+typedef NtCore<NtF16Pair, 128, 128, 4, 2, 2> NsCore128W;         // eight waves, for launches without a second workgroup for every CU (six 1000 x 1024 matrices 755 -> 701 us, the same with two sets of four waves that
+                                                                 // share the reduction; 4096 x 4096 with it throughout 4219 -> 4699)
 typedef NtCore<NtF16Pair2, 32, 32, 1, 1, 4, 4> NsCore32;           // four waves share one reduction; never cut
 constexpr int NS_SLOTS = 512;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4_t;
@@ -1061,7 +1062,7 @@ template <class Core> static void ns_launch_prod(const NsPlan& p, const NsTable&
 
 // The matrices with up to NS_MID rows and the others are two chains of launches: the short ones go step by step and keep the digits that composing would cost
 // them.  A Muon step does not need those -- its result is multiplied by the learning rate and added to a rounded parameter -- so there a list with both
-// goes through one chain (SAUNet's matrices: 956 us, in two chains 1136).  k: 0 the short ones, 1 the others
+// goes through one chain (SAUNet's matrices, with 64 x 64 tiles for both: 956 us, in two chains 1136).  k: 0 the short ones, 1 the others
 constexpr int NS_MID = 128;
 static saunet_ns_desc ns_part(const saunet_ns_desc* d, bool muon, int k, saunet_ns_item* item)
 {
@@ -1087,8 +1088,8 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
     int rc = ns_plan(d, p, large, small, ws);
     if (rc) return rc;
     if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255)) return set_error(SAUNET_BAD_SHAPE, "%s: the workspace has to hold %ld bytes on a 256-byte border", who, p.bytes);
-    // Steps composed at once: see the head of this file.  The longest matrix is the first.  (Short ones in twos would gain little: one of 128 x 256 183 us,
-    // step by step 171; sixty of 128 x 64 .. 992 299 us against 324.)
+    // Steps composed at once: see the head of this file.  The longest matrix is the first.  (Short ones in twos would gain little, measured with 64 x 64
+    // tiles: one of 128 x 256 183 us, step by step 171; sixty of 128 x 64 .. 992 299 us against 324.)
     const bool compose = p.large && (large[0].rows < large[0].cols ? large[0].rows : large[0].cols) > NS_MID && p.shortest > 32 && (double)d->a * d->a <= 16.0;
     const int first = !compose ? 1 : !MUON && p.shortest < 256 ? 2 : 3, later = compose ? 2 : 1;
     if (!go && !ns_schedule(d, first, later, w)) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
