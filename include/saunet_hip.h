@@ -513,8 +513,8 @@ int saunet_bucket_copy(const saunet_tensor_list* tl /*0:tensor 1:flat+offset*/, 
 /* Newton-Schulz orthogonalisation of a list of matrices (any shapes, one dtype) in one chain of launches:
  *   X = G / max(|G|_F, eps), then `steps` times  X <- (a I + b S + c S^2) X,  S = X X^T  (rows <= cols; the transpose otherwise).
  * Intermediate matrices are float16 pairs (float32-class products); float32 accumulation, float64 norm.  A matrix that holds an Inf or NaN comes
- * out as NaN and leaves the others alone; a zero matrix stays zero.  SAUNET_UNSUPPORTED, nothing launched: coefficients under which the
- * iteration leaves the range that the pairs can hold.  src may equal dst.
+ * out as NaN and leaves the others alone; a zero matrix stays zero.  SAUNET_UNSUPPORTED, nothing launched: coefficients under which some
+ * starting singular value in [0, 1] leaves the range that the pairs can hold.  src may equal dst.
  * workspace: saunet_newton_schulz_workspace(d) bytes on a 256-byte border, private to the call until it has completed on `stream`. */
 typedef struct saunet_ns_item {
     const void* src; void* dst;    /* matrix and result, row-major; Muon: gradient and parameter */
@@ -530,7 +530,7 @@ typedef struct saunet_ns_desc {
     int32_t adjust;                /* Muon: learning rate times sqrt(max(1, rows / cols)) (0) or 0.2 sqrt(max(rows, cols)) (1) */
     float a, b, c, eps;
 } saunet_ns_desc;
-int64_t saunet_newton_schulz_workspace(const saunet_ns_desc* d);      /* < 0: saunet_status */
+int64_t saunet_newton_schulz_workspace(const saunet_ns_desc* d);      /* < 0: saunet_status, also of coefficients that neither entry takes */
 int saunet_newton_schulz(const saunet_ns_desc* d, void* workspace, int64_t workspace_bytes, void* stream);
 /* One Muon step (float32): buf <- momentum buf + (1 - momentum) g;  u = nesterov ? (1 - momentum) g + momentum buf : buf;
  * p <- (1 - lr weight_decay) p - lr adjust NewtonSchulz(u).   hyper (DEVICE) = {lr, momentum, weight_decay, nesterov(0/1), grad_scale} */

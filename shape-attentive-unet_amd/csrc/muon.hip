@@ -962,13 +962,51 @@ static int ns_plan(const saunet_ns_desc* d, NsPlan& p, NsItem* large, NssItem* s
     return SAUNET_OK;
 }
 
-// Largest magnitude that a matrix with eigenvalue f(s), s in [0, 1] the first singular values, can hold: its power-of-two scale leaves a factor of two
-// below the largest float16.  The grid is even in s^(1/4): small singular values grow fastest.  0: out of range.
-constexpr int NS_GRID = 96;
-static float ns_scale(const double* v)
+// What the matrices of the chain can hold.  They are functions of one variable, the singular value x in [0, 1] that a direction starts with, and the host
+// carries intervals of it through the recurrences: the image of an interval under one polynomial is exact (its ends and the polynomial's own extrema), so no
+// peak lies between two samples -- with (1.5012, -3.8716, 1.2536) one of 2e8 did between 97 points.  Only the product of the composed factors is bounded as a
+// product of intervals, hence the cells; 192 of them, denser towards zero, where singular values grow fastest, overstate it by a few per cent.
+constexpr int NS_CELLS = 192;
+struct NsSpan { double lo, hi; };
+// f over the span: f has no extremum but at the points e
+template <typename F> static NsSpan ns_image(const NsSpan& s, const double* e, int n, F f)
+{
+    const double u = f(s.lo), v = f(s.hi);
+    NsSpan r = {u < v ? u : v, u < v ? v : u};
+    for (int i = 0; i < n; ++i)
+        if (e[i] > s.lo && e[i] < s.hi) { const double w = f(e[i]); r.lo = w < r.lo ? w : r.lo; r.hi = w > r.hi ? w : r.hi; }
+    return r;
+}
+// real roots of p + q s + r s^2
+static int ns_roots(double p, double q, double r, double* e)
+{
+    const double d = q * q - 4.0 * p * r;
+    if (!(d >= 0.0)) return 0;
+    const double t = -0.5 * (q + (q < 0.0 ? -sqrt(d) : sqrt(d)));
+    int n = 0;
+    if (r != 0.0) e[n++] = t / r;
+    if (t != 0.0) e[n++] = p / t;
+    return n;
+}
+static NsSpan ns_square(const NsSpan& s)
+{
+    const double u = s.lo * s.lo, v = s.hi * s.hi;
+    return NsSpan{s.lo <= 0.0 && s.hi >= 0.0 ? 0.0 : u < v ? u : v, u < v ? v : u};
+}
+static NsSpan ns_times(const NsSpan& s, const NsSpan& t)
+{
+    const double v[4] = {s.lo * t.lo, s.lo * t.hi, s.hi * t.lo, s.hi * t.hi};
+    return NsSpan{*std::min_element(v, v + 4), *std::max_element(v, v + 4)};
+}
+// The power-of-two scale of a matrix whose eigenvalues lie in the spans leaves a factor of two below the largest float16.  0: out of range.
+static float ns_scale(const NsSpan* v)
 {
     double top = 1e-3;
-    for (int i = 0; i <= NS_GRID; ++i) { const double a = v[i] < 0 ? -v[i] : v[i]; if (!(a <= 4096.0)) return 0.f; if (a > top) top = a; }
+    for (int i = 0; i < NS_CELLS; ++i) {
+        if (!(v[i].lo >= -4096.0) || !(v[i].hi <= 4096.0)) return 0.f;
+        if (-v[i].lo > top) top = -v[i].lo;
+        if (v[i].hi > top) top = v[i].hi;
+    }
     double s = 1.0;
     while (s * top > 32768.0) s *= 0.5;
     while (s * top * 2.0 <= 32768.0) s *= 2.0;
@@ -979,13 +1017,22 @@ static float ns_scale(const double* v)
 struct NsOp { int apply, ny; NsProds pr; int q, xt; float alpha, beta; bool gram, last; };
 struct NsSchedule { int count; float sx; NsOp op[32 * 4]; };
 
-// first, later: steps composed at once in the first block and in the others (see the head of this file)
-static bool ns_schedule(const saunet_ns_desc* d, int first, int later, NsSchedule& w)
+// first, later: steps composed at once in the first block and in the others (see the head of this file).  False: the coefficients drive singular values
+// out of range
+static bool ns_build_schedule(const saunet_ns_desc* d, int first, int later, NsSchedule& w)
 {
-    double x[NS_GRID + 1], S[NS_GRID + 1], P[NS_GRID + 1], Q[NS_GRID + 1], R[NS_GRID + 1];
-    const double b = d->b, c = d->c;
-    for (int i = 0; i <= NS_GRID; ++i) { const double u = (double)i / NS_GRID; x[i] = u * u * u * u * (1.0 + 1e-6); }
-    float sx = w.sx = ns_scale(x);
+    NsSpan X[NS_CELLS], S[NS_CELLS], P[NS_CELLS], T[NS_CELLS], V[NS_CELLS];
+    const double a0 = d->a, b = d->b, c = d->c;
+    for (int i = 0; i < NS_CELLS; ++i) {
+        const double u = (double)i / NS_CELLS, v = (double)(i + 1) / NS_CELLS;
+        X[i] = NsSpan{u * u * u * u, v * v * v * v * (1.0 + 1e-6)};
+    }
+    // extrema of b s + c s^2, of s (a + b s + c s^2) and, in x, of x (a + b x^2 + c x^4)
+    double ep[1], er[2], ex[4];
+    const int np = c != 0.0 ? (ep[0] = -b / (2.0 * c), 1) : 0, nr = ns_roots(a0, 2.0 * b, 3.0 * c, er);
+    int nx = ns_roots(a0, 3.0 * b, 5.0 * c, ex);
+    for (int i = 0, n = nx; i < n; ++i) { ex[i] = sqrt(ex[i]); ex[nx++] = -ex[i]; }           // (a NaN lies in no span)
+    float sx = w.sx = ns_scale(X);
     w.count = 0;
     int xt = 0;
     auto push = [&](int ny, const NsProds& pr, bool gram) { w.op[w.count++] = NsOp{0, ny, pr, 0, 0, 0.f, 0.f, gram, false}; };
@@ -993,25 +1040,29 @@ static bool ns_schedule(const saunet_ns_desc* d, int first, int later, NsSchedul
         const int left = d->steps - done, most = done ? later : first, nb = left < most ? left : most;
         // P is kept as b S + c S^2 in the first block, where most s are small, and as that + (a - 1) I, near zero where s is near 1, later: its rounding
         // counts in units of what is kept (300 x 500, five steps: 3.1e-6 of |X| without the shift, 1.6e-6 with it)
-        const double a = done ? 1.0 : (double)d->a, shift = (double)d->a - a;
-        for (int i = 0; i <= NS_GRID; ++i) S[i] = x[i] * x[i];
+        const double a = done ? 1.0 : a0, shift = a0 - a;
+        for (int i = 0; i < NS_CELLS; ++i) S[i] = ns_square(X[i]);
         float sa = ns_scale(S), sp, sq = 0;
         if (sa == 0.f) return false;
         push(1, NsProds{{{NS_X, NS_X, -1, -1, NS_A, sa / (sx * sx), 0.f, 0.f}, {}}}, true);
         double q = 0;
         int Qb = NS_Q0;
         for (int j = 0; j < nb; ++j) {
-            for (int i = 0; i <= NS_GRID; ++i) P[i] = b * S[i] + c * S[i] * S[i] + shift;
+            for (int i = 0; i < NS_CELLS; ++i) P[i] = ns_image(S[i], ep, np, [&](double s) { return (c * s + b) * s + shift; });
             sp = ns_scale(P);
             if (sp == 0.f) return false;
             const int Pb = j ? NS_P : NS_Q0;
             push(1, NsProds{{{NS_A, NS_A, NS_A, -1, Pb, (float)(c * sp / ((double)sa * sa)), (float)(b * sp / sa), 0.f, (float)(shift * sp)}, {}}}, false);
             NsProds pr = {};
             int ny = 0;
-            if (j == 0) { for (int i = 0; i <= NS_GRID; ++i) Q[i] = P[i]; sq = sp; q = a; }
+            // T: the product of the factors a + P so far; what is kept of it is T - q I
+            if (j == 0) { for (int i = 0; i < NS_CELLS; ++i) T[i] = NsSpan{P[i].lo + a, P[i].hi + a}; sq = sp; q = a; }
             else {
-                for (int i = 0; i <= NS_GRID; ++i) Q[i] = a * Q[i] + q * P[i] + P[i] * Q[i];
-                const float s2 = ns_scale(Q);
+                for (int i = 0; i < NS_CELLS; ++i) {
+                    T[i] = ns_times(T[i], NsSpan{P[i].lo + a, P[i].hi + a});
+                    V[i] = NsSpan{T[i].lo - q * a, T[i].hi - q * a};
+                }
+                const float s2 = ns_scale(V);
                 if (s2 == 0.f) return false;
                 const int to = Qb == NS_Q0 ? NS_Q1 : NS_Q0;
                 pr.p[ny++] = {NS_P, Qb, Qb, NS_P, to, (float)(s2 / ((double)sp * sq)), (float)(a * s2 / sq), (float)(q * s2 / sp)};
@@ -1019,29 +1070,45 @@ static bool ns_schedule(const saunet_ns_desc* d, int first, int later, NsSchedul
             }
             float sr = 0;
             if (j < nb - 1) {
-                for (int i = 0; i <= NS_GRID; ++i) R[i] = (a + P[i]) * S[i];
-                sr = ns_scale(R);
+                for (int i = 0; i < NS_CELLS; ++i) V[i] = ns_image(S[i], er, nr, [&](double s) { return ((c * s + b) * s + a0) * s; });
+                sr = ns_scale(V);
                 if (sr == 0.f) return false;
                 pr.p[ny++] = {Pb, NS_A, NS_A, -1, NS_R, (float)(sr / ((double)sp * sa)), (float)(a * sr / sa), 0.f};
             }
             if (ny) push(ny, pr, false);
+            for (int i = 0; i < NS_CELLS; ++i) X[i] = ns_image(X[i], ex, nx, [&](double x) { return ((c * x * x + b) * x * x + a0) * x; });
             if (j < nb - 1) {
-                for (int i = 0; i <= NS_GRID; ++i) S[i] = (a + P[i]) * R[i];
+                for (int i = 0; i < NS_CELLS; ++i) S[i] = ns_square(X[i]);
                 const float s2 = ns_scale(S);
                 if (s2 == 0.f) return false;
                 push(1, NsProds{{{NS_R, Pb, NS_R, -1, NS_A, (float)(s2 / ((double)sr * sp)), (float)(a * s2 / sr), 0.f}, {}}}, false);
                 sa = s2;
             }
         }
-        for (int i = 0; i <= NS_GRID; ++i) x[i] = (q + Q[i]) * x[i];
         done += nb;
         const bool last = done >= d->steps;
-        const float s2 = last ? 1.f : ns_scale(x);
+        const float s2 = last ? 1.f : ns_scale(X);
         if (s2 == 0.f) return false;
         w.op[w.count++] = NsOp{1, 0, {}, Qb, xt, (float)(s2 / ((double)sq * sx)), (float)(q * s2 / sx), false, last};
         xt ^= 1; sx = s2;
     }
     return true;
+}
+// The schedule is a function of the numbers below alone and costs some 50 us of host time, so a thread keeps the last few: an optimiser asks for the same
+// one or two in every step
+static const NsSchedule* ns_schedule(const saunet_ns_desc* d, int first, int later)
+{
+    struct Key { float a, b, c; int steps, first, later; };
+    struct Entry { Key key; bool ok; NsSchedule w; };
+    static thread_local Entry kept[4];
+    static thread_local int next = 0;
+    const Key k = {d->a, d->b, d->c, d->steps, first, later};
+    for (Entry& e : kept) if (e.key.steps && !memcmp(&e.key, &k, sizeof k)) return e.ok ? &e.w : nullptr;
+    Entry& e = kept[next];
+    next = (next + 1) & 3;
+    e.key = k;
+    e.ok = ns_build_schedule(d, first, later, e.w);
+    return e.ok ? &e.w : nullptr;
 }
 
 template <class Core, typename T, int MODE> static void ns_launch_apply(const saunet_ns_desc* d, const NsPlan& p, const NsTable& tab, const NsOp& o, const float* hyper, hipStream_t st)
@@ -1078,8 +1145,16 @@ static saunet_ns_desc ns_part(const saunet_ns_desc* d, bool muon, int k, saunet_
     return r;
 }
 
-// go: false looks only whether the call can be made, and leaves its schedule in w
-template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool go, NsSchedule& w, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
+// Steps composed at once: see the head of this file.  The longest matrix is the first.  (Short ones in twos would gain little, measured with 64 x 64
+// tiles: one of 128 x 256 183 us, step by step 171; sixty of 128 x 64 .. 992 299 us against 324.)
+static const NsSchedule* ns_plan_schedule(const saunet_ns_desc* d, bool muon, const NsPlan& p, const NsItem* large)
+{
+    const bool compose = p.large && (large[0].rows < large[0].cols ? large[0].rows : large[0].cols) > NS_MID && p.shortest > 32 && (double)d->a * d->a <= 16.0;
+    return ns_schedule(d, !compose ? 1 : !muon && p.shortest < 256 ? 2 : 3, compose ? 2 : 1);
+}
+
+// go: false looks only whether the call can be made
+template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool go, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
 {
     static thread_local NsItem large[4096];
     static thread_local NssItem small[4096];
@@ -1088,11 +1163,8 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
     int rc = ns_plan(d, p, large, small, ws);
     if (rc) return rc;
     if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255)) return set_error(SAUNET_BAD_SHAPE, "%s: the workspace has to hold %ld bytes on a 256-byte border", who, p.bytes);
-    // Steps composed at once: see the head of this file.  The longest matrix is the first.  (Short ones in twos would gain little, measured with 64 x 64
-    // tiles: one of 128 x 256 183 us, step by step 171; sixty of 128 x 64 .. 992 299 us against 324.)
-    const bool compose = p.large && (large[0].rows < large[0].cols ? large[0].rows : large[0].cols) > NS_MID && p.shortest > 32 && (double)d->a * d->a <= 16.0;
-    const int first = !compose ? 1 : !MUON && p.shortest < 256 ? 2 : 3, later = compose ? 2 : 1;
-    if (!go && !ns_schedule(d, first, later, w)) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
+    const NsSchedule* w = ns_plan_schedule(d, MUON, p, large);
+    if (!w) return set_error(SAUNET_UNSUPPORTED, "%s: the coefficients drive singular values out of range", who);
     if (!go) return SAUNET_OK;
     for (long i = 0; i < p.small; i += NSS_CHUNK) {
         NssItems ch;
@@ -1117,10 +1189,10 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
         hipLaunchKernelGGL(ns_setup_kernel, dim3(1), dim3(64), 0, st, ch, k, (NsItem*)tab.all + i);
     }
     hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)p.norm), dim3(256), 0, st, tab, hyper, part);
-    hipLaunchKernelGGL((ns_pack_kernel<T, MUON>), dim3((unsigned)p.pack), dim3(256), 0, st, tab, hyper, part, d->eps, w.sx);
+    hipLaunchKernelGGL((ns_pack_kernel<T, MUON>), dim3((unsigned)p.pack), dim3(256), 0, st, tab, hyper, part, d->eps, w->sx);
     SAUNET_CHECK_LAUNCH("ns_pack");
-    for (int i = 0; i < w.count; ++i) {
-        const NsOp& o = w.op[i];
+    for (int i = 0; i < w->count; ++i) {
+        const NsOp& o = w->op[i];
         if (o.apply) {
             constexpr int LAST = MUON ? 2 : 1;
             if (p.tile_n == 32) o.last ? ns_launch_apply<NsCore32, T, LAST>(d, p, tab, o, hyper, st) : ns_launch_apply<NsCore32, T, 0>(d, p, tab, o, hyper, st);
@@ -1142,11 +1214,10 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
 template <typename T, bool MUON> static int ns_run_all(const saunet_ns_desc* d, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
 {
     static thread_local saunet_ns_item item[4096];
-    static thread_local NsSchedule w[2];
     for (int pass = 0; pass < 2; ++pass)
         for (int k = 0; k < 2; ++k) {
             const saunet_ns_desc part = ns_part(d, MUON, k, item);
-            const int rc = part.count ? ns_run<T, MUON>(&part, pass == 1, w[k], hyper, workspace, workspace_bytes, st, who) : SAUNET_OK;
+            const int rc = part.count ? ns_run<T, MUON>(&part, pass == 1, hyper, workspace, workspace_bytes, st, who) : SAUNET_OK;
             if (rc) return rc;
         }
     return SAUNET_OK;
@@ -1166,12 +1237,15 @@ int64_t saunet_newton_schulz_workspace(const saunet_ns_desc* d)
     NsPlan p;
     int rc = ns_check(d, "newton_schulz");
     int64_t most = 0;
+    bool bad[2] = {false, false};                 // a use whose schedules leave the range: the step composes otherwise than the plain call
     for (int k = 0; k < 4 && !rc; ++k) {          // one chain behind the other, in the same memory; for either use
         const saunet_ns_desc part = ns_part(d, k & 2, k & 1, item);
         if (!part.count) continue;
         rc = ns_plan(&part, p, large, small, nullptr);
         if (p.bytes > most) most = p.bytes;
+        if (!rc && !ns_plan_schedule(&part, k & 2, p, large)) bad[k >> 1] = true;
     }
+    if (!rc && bad[0] && bad[1]) return set_error(SAUNET_UNSUPPORTED, "newton_schulz: the coefficients drive singular values out of range");
     return rc ? rc : most;
 }
 

@@ -1,0 +1,103 @@
+"""What the Newton-Schulz kernels and the Muon step do at the borders of their domain: coefficients beside the range that the float16 pairs hold, matrices
+below eps, lists that outgrow one workspace, lists of long and short matrices, arguments that have to be refused."""
+import ctypes as C
+import math
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from saunet_amd import functional as HF, lib as L, optim
+
+COEFF = (3.4445, -4.7750, 2.0315)
+
+
+def chain(g, dtype, steps=5, coeff=COEFF, eps=1e-7):
+    a, b, c = coeff
+    x = g.to(dtype)
+    tall = x.shape[0] > x.shape[1]
+    x = x.t().contiguous() if tall else x
+    x = x / x.double().norm().clamp(min=eps).to(dtype)
+    for _ in range(steps):
+        s = x @ x.t()
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x.t().contiguous() if tall else x
+
+
+# ------------------------------------------------------------------------------------------------ coefficients (no GPU needed)
+def workspace(rows, cols, steps, coeff):
+    """bytes, or the status of a call that cannot be made: nothing is launched"""
+    d, hold = HF.ns_desc([0, 0, 0, cols, cols, rows, cols], L.F32, steps, coeff, 1e-7)
+    return L.load().saunet_newton_schulz_workspace(C.byref(d))
+
+
+def largest(steps, coeff, first, later, x):
+    """the largest |eigenvalue| of anything that the chain keeps, over the starting singular values x: X, S = X^2, R = (a + P) S and, of the composed
+    product of the factors a + P, what is kept of it"""
+    a, b, c = (float(np.float32(v)) for v in coeff)
+    top, done = 0.0, 0
+    with np.errstate(all="ignore"):
+        while done < steps:
+            nb = min(steps - done, later if done else first)
+            base = 1.0 if done else a
+            t = np.ones_like(x)
+            for j in range(nb):
+                s = x * x
+                f = a + (c * s + b) * s
+                t = t * f
+                kept = [s, f - base, t - base ** (j + 1)] + ([f * s] if j < nb - 1 else [])
+                top = max([top] + [float(np.abs(v).max()) for v in kept])
+                x = f * x
+            done += nb
+            if done < steps:
+                top = max(top, float(np.abs(x).max()))
+    return top
+
+
+def test_a_peak_between_two_samples_is_refused():
+    # a polynomial of degree 5^5 whose largest value, 2e8, is taken on an interval far narrower than a hundredth of its domain
+    for steps in (5, 6, 8):
+        assert workspace(300, 400, steps, (1.5012, -3.8716, 1.2536)) == -5
+    assert b"out of range" in L.load().saunet_last_error()
+    assert workspace(300, 400, 5, COEFF) > 0
+
+
+def test_accepted_coefficients_stay_in_range():
+    """everything kept stays below 4096, the limit of the scales, on a fine grid; and the usual
+    coefficients are accepted"""
+    x = np.linspace(0, 1, 200001) ** 4
+    rng = random.Random(5)
+    accepted = 0
+    for i in range(600):
+        coeff, steps = (rng.uniform(0.5, 4.0), rng.uniform(-8, 1), rng.uniform(-1, 4)), (3, 5, 8)[i % 3]
+        rows, first, later = ((64, 1, 1), (200, 2, 2), (300, 3, 2))[i // 3 % 3]
+        if workspace(rows, 400, steps, coeff) < 0:
+            continue
+        accepted += 1
+        # (float32's rounding of the coefficients aside, the host's interval is exact)
+        assert largest(steps, coeff, first, later, x) <= 4096 * (1 + 1e-6), (coeff, steps, rows)
+    assert accepted > 60
+    for coeff in (COEFF, (1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (1.875, -1.25, 0.375), (4.0848, -6.8946, 2.9270)):
+        for rows in (20, 64, 200, 300):
+            for steps in (1, 5, 12, 32):
+                assert workspace(rows, 400, steps, coeff) > 0
+
+
+@pytest.mark.gpu
+def test_a_narrow_finite_peak_comes_out_finite():
+    """one singular value where (a + P) S reaches 1346 and X 451, twenty times what the neighbourhood suggests.
+
+    Tolerance: after three steps X = 1.55 carries the rounding of a product kept to 30 with 2^-21 of it, 1.4e-5; the two steps behind multiply that by their
+    slopes, 30 and 860: 0.4 of 451, and as much again from the second block's own matrices (289 kept with 2^-21): below one per cent."""
+    coeff, peak = (3.04314876, -6.77973318, 2.62109327), 0.9766965
+    gen = torch.Generator().manual_seed(4)
+    m, n = 260, 300
+    u, v = torch.linalg.qr(torch.randn(m, m, generator=gen, dtype=torch.float64))[0], torch.linalg.qr(torch.randn(n, m, generator=gen, dtype=torch.float64))[0]
+    s = torch.full((m,), math.sqrt((1 - peak * peak) / (m - 1)), dtype=torch.float64)
+    s[0] = peak
+    g = ((u * s) @ v.t()).float()
+    out = HF.newton_schulz(g.cuda(), coefficients=coeff).cpu()
+    ref = chain(g, torch.float64, coeff=coeff)
+    assert 400 < float(ref.norm()) < 500 and torch.isfinite(out).all()
+    assert float((out.double() - ref).norm()) <= 0.01 * float(ref.norm())
