@@ -111,7 +111,8 @@ class _FusedBase(torch.optim.Optimizer):
     def _live(self, group):
         ps = [p for p in group["params"] if p.grad is not None]
         for p in ps:
-            if not p.is_cuda:
+            # (the hyper-parameter array lies where the group's first parameter does, whether that one has a gradient or not)
+            if not p.is_cuda or not group["params"][0].is_cuda:
                 raise RuntimeError("fused optimisers run on the GPU only (no CPU fallback)")
             if p.grad.dtype != torch.float32 or not p.grad.is_contiguous() or not p.is_contiguous():
                 raise RuntimeError("fused optimisers need contiguous float32 params/grads")
@@ -284,7 +285,7 @@ class FusedMuon(_FusedBase):
             rows = []
             ps = [p for p in self._live(g) if p.numel()]
             for p in ps:
-                if p.dtype != torch.float32 or p.device != ps[0].device:
+                if p.dtype != torch.float32 or p.device != g["params"][0].device:
                     raise RuntimeError("FusedMuon takes float32 parameters on one device a group")
                 st = self.state[p]
                 if "momentum_buffer" not in st:

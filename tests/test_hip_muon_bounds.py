@@ -101,3 +101,16 @@ def test_a_narrow_finite_peak_comes_out_finite():
     ref = chain(g, torch.float64, coeff=coeff)
     assert 400 < float(ref.norm()) < 500 and torch.isfinite(out).all()
     assert float((out.double() - ref).norm()) <= 0.01 * float(ref.norm())
+
+
+# ------------------------------------------------------------------------------------------------ the step's arguments
+@pytest.mark.gpu
+@pytest.mark.parametrize("make", [lambda ps: optim.FusedMuon(ps), lambda ps: optim.FusedSGD(ps, lr=0.1), lambda ps: optim.FusedAdam(ps), lambda ps: optim.FusedRAdam(ps)],
+                         ids=["muon", "sgd", "adam", "radam"])
+def test_a_group_that_begins_on_the_cpu_is_refused(make):
+    """the hyper-parameters lie beside the group's first parameter: on the CPU no kernel may read them"""
+    host, dev = torch.nn.Parameter(torch.ones(4, 4)), torch.nn.Parameter(torch.ones(4, 4).cuda())
+    dev.grad = torch.ones_like(dev)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        make([host, dev]).step()
+    assert (dev == 1).all()
