@@ -251,7 +251,8 @@ class FusedMuon(_FusedBase):
       p <- (1 - lr weight_decay) p - lr adjust NewtonSchulz(u)
 
     ``adjust_lr_fn``: "original" (None): sqrt(max(1, rows / cols));  "match_rms_adamw": 0.2 sqrt(max(rows, cols)) -- learning rate and decay tuned for
-    Adam carry over.  Arguments, defaults and state as torch.optim.Muon has them; a convolution weight [O, I, kh, kw] is the matrix O x (I kh kw).
+    Adam carry over.  Arguments, defaults and state as torch.optim.Muon has them, a closure among them.  A parameter of more dimensions is the matrix of
+    its first one by all others: a convolution weight [O, I, kh, kw] is O x (I kh kw), a transposed convolution's [I, O, kh, kw] is I x (O kh kw).
     Parameters with fewer than two dimensions belong to another optimiser (create_optimizers("muon", ...) pairs it with FusedAdam).  The whole list is
     one chain of launches, float32-class throughout; the step can be captured (graph.GraphedStep): lr, momentum, weight decay and grad_scale
     are read from the device array."""
@@ -279,6 +280,10 @@ class FusedMuon(_FusedBase):
 
     @torch.no_grad()
     def step(self, closure=None, upload=True):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
         if upload:
             self.upload_hyper()
         for g in self.param_groups:
@@ -305,6 +310,7 @@ class FusedMuon(_FusedBase):
                     ws = HF.ns_workspace(d, ps[0].device)
                     L.call("saunet_muon_step", C.byref(d), self._hyper(g).data_ptr(), ws.data_ptr(), ws.numel(), L.stream())
         HF.PACKS.invalidate()
+        return loss
 
 
 def create_optimizers(unet, optimizer="sgd", lr=5e-4, momentum=0.9, weight_decay=1e-4):

@@ -114,3 +114,27 @@ def test_a_group_that_begins_on_the_cpu_is_refused(make):
     with pytest.raises(RuntimeError, match="GPU only"):
         make([host, dev]).step()
     assert (dev == 1).all()
+
+
+@pytest.mark.gpu
+def test_muon_step_evaluates_its_closure():
+    torch.manual_seed(0)
+    w = torch.nn.Parameter(torch.randn(8, 12).cuda())
+    x = torch.randn(12, 5).cuda()
+    ref = torch.nn.Parameter(w.detach().clone())
+    a, b = optim.FusedMuon([w], lr=0.1), optim.FusedMuon([ref], lr=0.1)
+
+    def closure():
+        a.zero_grad()
+        loss = (w @ x).square().sum()
+        loss.backward()
+        return loss
+
+    for _ in range(2):
+        want = (ref @ x).square().sum()
+        b.zero_grad()
+        want.backward()
+        loss = a.step(closure)
+        b.step()
+        assert torch.equal(loss, want) and torch.equal(w, ref)
+    assert b.step() is None
