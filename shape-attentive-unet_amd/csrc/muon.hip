@@ -45,11 +45,11 @@ constexpr int NS_NORM = 4096;                // elements a workgroup of the norm
 enum { NS_X = -1, NS_A = 0, NS_P, NS_R, NS_Q0, NS_Q1, NS_NSYM };
 struct NsView {
     int m, n, mp, np, tall;
-    char *x, *s0; long bx, bs;
+    char *x, *s0; float* t0; long bx, bs;
     static long bytes(int rows, int cols)
     {
         const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows, mp = (m + 63) / 64 * 64, np = (n + 63) / 64 * 64;
-        return 3 * mp * np * 4 + NS_NSYM * mp * mp * 4;
+        return 256 + 3 * mp * np * 4 + NS_NSYM * mp * mp * 4;
     }
     __device__ explicit NsView(const NsItem& it)
     {
@@ -57,11 +57,15 @@ struct NsView {
         m = tall ? it.cols : it.rows; n = tall ? it.rows : it.cols;
         mp = (m + 63) / 64 * 64; np = (n + 63) / 64 * 64;
         bx = (long)mp * np * 4; bs = (long)mp * mp * 4;
-        x = it.ws; s0 = x + 3 * bx;
+        t0 = (float*)it.ws; x = it.ws + 256; s0 = x + 3 * bx;
     }
     __device__ __forceinline__ char* xt(int i) const { return x + (1 + i) * bx; }
     __device__ __forceinline__ char* sym(int i) const { return s0 + i * bs; }
     __device__ __forceinline__ float* part() const { return (float*)(s0 + NS_NSYM * bs); }
+    // A matrix whose norm is below eps is kept as X / t, so that its elements do not sink below what a float16 pair resolves (norm = 1e-6 eps, 300 x 500: 4e-4 of
+    // the result before, 1e-7 now).  t starts as the power of two t0 >= norm / eps and grows with every application of a polynomial by a power of two that
+    // bounds its growth, up to 1; `grown` is the product of those bounds.  All other matrices have t0 = 1, for which nothing below changes a bit.
+    __device__ __forceinline__ float t(float grown) const { const float v = *t0 * grown; return v < 1.f ? v : 1.f; }
 };
 
 // the matrix whose workgroups include `id`: the last whose first(i) is not above it; two rounds of one load a lane (count <= 4096)
@@ -170,7 +174,11 @@ template <typename T, bool MUON> __global__ __launch_bounds__(256) void ns_pack_
     if ((tid & 63) == 0) s_sum[tid >> 6] = sum;
     __syncthreads();
     const double norm = sqrt(((s_sum[0] + s_sum[1]) + s_sum[2]) + s_sum[3]);
-    const double inv = (double)sx / (norm <= (double)eps ? (double)eps : norm);      // a NaN norm stays NaN
+    // (a NaN norm stays NaN)
+    double t0 = 1.0;
+    if (norm < (double)eps && norm > 0.0) { t0 = ldexp(1.0, (int)ceil(log2(norm / (double)eps))); t0 = t0 < 0x1p-126 ? 0x1p-126 : t0; }
+    if (id == it.p_pack && tid == 0) *v.t0 = (float)t0;
+    const double inv = (double)sx / ((norm <= (double)eps ? (double)eps : norm) * t0);
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
         // (a padding element is zero, not zero times a scale that may be NaN)
@@ -443,13 +451,12 @@ template <class Core> __device__ __forceinline__ void ns_join(f32x16 (&acc)[Core
 }
 
 // blends E and F into a whole tile and stores it with its mirror image
-template <class Core> __device__ __forceinline__ void ns_prod_end(const NsView& v, const NsProd& p, int ti, int tj, f32x16 (&acc)[Core::TM][Core::TN], unsigned char* smem)
+template <class Core> __device__ __forceinline__ void ns_prod_end(const NsView& v, const NsProd& p, float alpha, int ti, int tj, f32x16 (&acc)[Core::TM][Core::TN], unsigned char* smem)
 {
     typedef NsTile<Core> Tile;
     constexpr int T = Core::BM;
     const long ls = (long)v.mp * 4, oij = (long)ti * T * ls + tj * T * 4, oji = (long)tj * T * ls + ti * T * 4;       // tile (ti, tj) and its mirror image
     const int ri = v.mp - ti * T, rj = v.mp - tj * T;
-    float alpha = p.alpha;
     if (p.e >= 0) { Tile::blend(acc, alpha, p.beta, v.sym(p.e) + oji, ls, rj, ri, smem); alpha = 1.f; }
     if (p.f >= 0) Tile::blend(acc, alpha, p.gamma, v.sym(p.f) + oji, ls, rj, ri, smem);
     if (p.diag != 0.f && ti == tj)
@@ -460,7 +467,7 @@ template <class Core> __device__ __forceinline__ void ns_prod_end(const NsView& 
     Tile::store_t(acc, alpha, v.sym(p.d) + oji, ls, rj, ri, ti == tj, smem);
     if (ti != tj) Tile::store(acc, alpha, v.sym(p.d) + oij, ls, ri, rj, smem);
 }
-template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) void ns_prod_kernel(NsTable tab, int kind, NsProds pr, NsDeal deal, int tail)
+template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) void ns_prod_kernel(NsTable tab, int kind, NsProds pr, float grown, NsDeal deal, int tail)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     constexpr int T = Core::BM;
@@ -479,6 +486,7 @@ template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) voi
     const long ld = (long)steps * Core::RB;
     const char* a = (p.a == NS_X ? v.x : v.sym(p.a)) + (long)k0 * Core::RB;
     const char* b = (p.a == NS_X ? v.x : v.sym(p.b)) + (long)k0 * Core::RB;
+    const float t2 = p.a == NS_X ? v.t(grown) * v.t(grown) : 1.f;
     f32x16 acc[Core::TM][Core::TN] = {};
     Core::run(a + ti * T * ld, (unsigned)ld, v.mp - ti * T, b + tj * T * ld, (unsigned)ld, v.mp - tj * T, k1 - k0, smem, acc);
     if constexpr (Core::KW > 1) ns_join<Core>(acc, smem);
@@ -488,10 +496,10 @@ template <class Core> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) voi
         Quads::each([&](int b, int, int) { float q[4]; Quads::quad(acc, b, q); *(f32x4*)(d + b * Core::NT * 4) = f32x4{q[0], q[1], q[2], q[3]}; });
         return;
     }
-    ns_prod_end<Core>(v, p, ti, tj, acc, smem);
+    ns_prod_end<Core>(v, p, p.alpha * t2, ti, tj, acc, smem);
 }
 // one accumulator quad of a cut tile a thread; blockIdx.x = tile * quads + quad
-template <class Core> __global__ __launch_bounds__(Core::NT) void ns_finish_kernel(NsTable tab, int kind, NsProds pr)
+template <class Core> __global__ __launch_bounds__(Core::NT) void ns_finish_kernel(NsTable tab, int kind, NsProds pr, float grown)
 {
     constexpr int T = Core::BM, N = NsQuads<Core>::N;
     const int id = blockIdx.x / N, q = blockIdx.x % N;
@@ -511,9 +519,10 @@ template <class Core> __global__ __launch_bounds__(Core::NT) void ns_finish_kern
     i += ti * T; j += tj * T;
     if (i >= v.mp || j >= v.mp) return;
     const long ls = (long)v.mp * 4;
+    const float alpha = p.a == NS_X ? p.alpha * (v.t(grown) * v.t(grown)) : p.alpha;
     float w[4], x[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) w[r] = p.alpha * c[r];
+    for (int r = 0; r < 4; ++r) w[r] = alpha * c[r];
     if (p.e >= 0) {
         ns_read4(v.sym(p.e), ls, j, i, x);
 #pragma unroll
@@ -547,7 +556,7 @@ __device__ __forceinline__ void ns_rates(const float* hyper, int rows, int cols,
 }
 
 // X <- alpha Q X + beta X.  MODE 0: back to X and the other X^T; 1: to the caller's matrix; 2: the Muon update of the caller's parameter
-template <class Core, typename T, int MODE> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) void ns_apply_kernel(NsTable tab, int q, int xt, float alpha, float beta, const float* __restrict__ hyper, int adjust, NsDeal deal)
+template <class Core, typename T, int MODE> __global__ __launch_bounds__(Core::NT, 512 / Core::NT) void ns_apply_kernel(NsTable tab, int q, int xt, float alpha, float beta, float grown, float grown_to, const float* __restrict__ hyper, int adjust, NsDeal deal)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     constexpr int B = Core::BM;
@@ -557,6 +566,8 @@ template <class Core, typename T, int MODE> __global__ __launch_bounds__(Core::N
     const NsView v(it);
     int ti, tj;
     nt_band(id - it.p_app, (v.np + B - 1) / B, (v.mp + B - 1) / B, tj, ti);
+    const float t = MODE == 0 ? v.t(grown) / v.t(grown_to) : v.t(grown);          // (powers of two)
+    alpha *= t; beta *= t;
     f32x16 acc[Core::TM][Core::TN] = {};
     const long ld = (long)v.mp * 4;
     Core::run(v.sym(q) + ti * B * ld, (unsigned)ld, v.mp - ti * B, v.xt(xt) + tj * B * ld, (unsigned)ld, v.np - tj * B, v.mp * 4 / Core::RB, smem, acc);
@@ -998,10 +1009,10 @@ static NsSpan ns_times(const NsSpan& s, const NsSpan& t)
     const double v[4] = {s.lo * t.lo, s.lo * t.hi, s.hi * t.lo, s.hi * t.hi};
     return NsSpan{*std::min_element(v, v + 4), *std::max_element(v, v + 4)};
 }
-// The power-of-two scale of a matrix whose eigenvalues lie in the spans leaves a factor of two below the largest float16.  0: out of range.
-static float ns_scale(const NsSpan* v)
+// The power-of-two scale of a matrix whose eigenvalues lie in the spans leaves a factor of two below the largest float16.  0: out of range.  (top: of X, which
+// a matrix below eps has as X / t, up to 1)
+static float ns_scale(const NsSpan* v, double top = 1e-3)
 {
-    double top = 1e-3;
     for (int i = 0; i < NS_CELLS; ++i) {
         if (!(v[i].lo >= -4096.0) || !(v[i].hi <= 4096.0)) return 0.f;
         if (-v[i].lo > top) top = -v[i].lo;
@@ -1014,7 +1025,7 @@ static float ns_scale(const NsSpan* v)
 }
 
 // The launches behind the pack pass
-struct NsOp { int apply, ny; NsProds pr; int q, xt; float alpha, beta; bool gram, last; };
+struct NsOp { int apply, ny; NsProds pr; int q, xt; float alpha, beta; bool gram, last; float grown, grown_to; };      // grown: NsView::t
 struct NsSchedule { int count; float sx; NsOp op[32 * 4]; };
 
 // first, later: steps composed at once in the first block and in the others (see the head of this file).  False: the coefficients drive singular values
@@ -1035,7 +1046,8 @@ static bool ns_build_schedule(const saunet_ns_desc* d, int first, int later, NsS
     float sx = w.sx = ns_scale(X);
     w.count = 0;
     int xt = 0;
-    auto push = [&](int ny, const NsProds& pr, bool gram) { w.op[w.count++] = NsOp{0, ny, pr, 0, 0, 0.f, 0.f, gram, false}; };
+    float grown = 1.f;
+    auto push = [&](int ny, const NsProds& pr, bool gram) { w.op[w.count++] = NsOp{0, ny, pr, 0, 0, 0.f, 0.f, gram, false, grown, 1.f}; };
     for (int done = 0; done < d->steps;) {
         const int left = d->steps - done, most = done ? later : first, nb = left < most ? left : most;
         // P is kept as b S + c S^2 in the first block, where most s are small, and as that + (a - 1) I, near zero where s is near 1, later: its rounding
@@ -1087,10 +1099,13 @@ static bool ns_build_schedule(const saunet_ns_desc* d, int first, int later, NsS
         }
         done += nb;
         const bool last = done >= d->steps;
-        const float s2 = last ? 1.f : ns_scale(X);
+        const float s2 = last ? 1.f : ns_scale(X, 1.0);
         if (s2 == 0.f) return false;
-        w.op[w.count++] = NsOp{1, 0, {}, Qb, xt, (float)(s2 / ((double)sq * sx)), (float)(q * s2 / sx), false, last};
-        xt ^= 1; sx = s2;
+        double growth = 1.0;
+        for (int i = 0; i < NS_CELLS; ++i) while (T[i].hi > growth || -T[i].lo > growth) growth *= 2.0;
+        const float to = grown * growth < 0x1p126 ? (float)(grown * growth) : 0x1p126f;
+        w.op[w.count++] = NsOp{1, 0, {}, Qb, xt, (float)(s2 / ((double)sq * sx)), (float)(q * s2 / sx), false, last, grown, to};
+        xt ^= 1; sx = s2; grown = to;
     }
     return true;
 }
@@ -1115,7 +1130,7 @@ template <class Core, typename T, int MODE> static void ns_launch_apply(const sa
 {
     static DeviceOnce once;
     if (once.first()) (void)hipFuncSetAttribute((const void*)ns_apply_kernel<Core, T, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
-    hipLaunchKernelGGL((ns_apply_kernel<Core, T, MODE>), dim3(ns_deal_grid(p.deal[NS_KINDS])), dim3(Core::NT), Core::LDS, st, tab, o.q, o.xt, o.alpha, o.beta, hyper, d->adjust, p.deal[NS_KINDS]);
+    hipLaunchKernelGGL((ns_apply_kernel<Core, T, MODE>), dim3(ns_deal_grid(p.deal[NS_KINDS])), dim3(Core::NT), Core::LDS, st, tab, o.q, o.xt, o.alpha, o.beta, o.grown, o.grown_to, hyper, d->adjust, p.deal[NS_KINDS]);
 }
 template <class Core> static void ns_launch_prod(const NsPlan& p, const NsTable& tab, const NsOp& o, hipStream_t st)
 {
@@ -1123,8 +1138,8 @@ template <class Core> static void ns_launch_prod(const NsPlan& p, const NsTable&
     static DeviceOnce once;
     if (once.first()) (void)hipFuncSetAttribute((const void*)ns_prod_kernel<Core>, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
     const unsigned dealt = ns_deal_grid(p.deal[kind]);
-    hipLaunchKernelGGL((ns_prod_kernel<Core>), dim3(dealt + (unsigned)(p.grid[kind] - p.deal[kind].b[8]), o.ny), dim3(Core::NT), Core::LDS, st, tab, kind, o.pr, p.deal[kind], (int)dealt);
-    if constexpr (Core::KW == 1) if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(Core::NT), 0, st, tab, kind, o.pr);
+    hipLaunchKernelGGL((ns_prod_kernel<Core>), dim3(dealt + (unsigned)(p.grid[kind] - p.deal[kind].b[8]), o.ny), dim3(Core::NT), Core::LDS, st, tab, kind, o.pr, o.grown, p.deal[kind], (int)dealt);
+    if constexpr (Core::KW == 1) if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(Core::NT), 0, st, tab, kind, o.pr, o.grown);
 }
 
 // The matrices with up to NS_MID rows and the others are two chains of launches: the short ones go step by step and keep the digits that composing would cost

@@ -103,6 +103,51 @@ def test_a_narrow_finite_peak_comes_out_finite():
     assert float((out.double() - ref).norm()) <= 0.01 * float(ref.norm())
 
 
+# ------------------------------------------------------------------------------------------------ matrices below eps
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(40, 90), (300, 500), (700, 140), (1100, 1200), (20, 60), (200, 4000)])
+def test_matrices_whose_norm_is_below_eps_keep_their_digits(m, n):
+    """X = G / eps there, far below one: the result is small and as exact as any other.  Matrices of both kinds in one call.
+
+    Tolerance, in half steps d = 2^-24 of float32, for singular values so small that every factor is a I + (next to nothing): a composed factor keeps
+    q + Q with |Q| below q's size, 2 d + 4 d (its two operands) + 4 d (the dropped low parts) a product, at most six products and three applications of it, the
+    stored X, 2 d each time, and the result's own rounding: below 100 d.  Where s is not small the float32 chain is the yardstick as everywhere."""
+    gen = torch.Generator().manual_seed(m)
+    gs, ratio = [], [1e3, 0.7, 1e-2, 1e-4, 1e-6, 1e-9, 1e-14, 1e-30]
+    for r in ratio:
+        g = torch.randn(m, n, generator=gen)
+        gs.append((g.double() / g.double().norm() * 1e-7 * r).float() if r > 1e-20 else torch.zeros(m, n).index_put_((torch.tensor(m - 1), torch.tensor(1)), torch.tensor(1e-37)))
+    for out, g, r in zip(HF.newton_schulz([g.cuda() for g in gs]), gs, ratio):
+        ref = chain(g, torch.float64)
+        d32 = (chain(g, torch.float32).double() - ref).norm()
+        tol = 4 * float(d32) + 100 * 2.0 ** -24 * float(ref.norm()) + 2.0 ** -149 * (m * n) ** 0.5
+        assert float((out.cpu().double() - ref).norm()) <= tol, (r, float((out.cpu().double() - ref).norm()), float(ref.norm()))
+    for dtype in (torch.bfloat16, torch.float16):
+        g = gs[2].to(dtype) if dtype == torch.bfloat16 else (gs[2] * 1e4).half()
+        eps = 1e-7 if dtype == torch.bfloat16 else 1e-2
+        out = HF.newton_schulz(g.cuda(), eps=eps).cpu()
+        ref = chain(g, torch.float64, eps=eps)
+        tol = 4 * float((chain(g, torch.float32, eps=eps).double() - ref).norm()) + (100 * 2.0 ** -24 + torch.finfo(dtype).eps / 2) * float(ref.norm())
+        assert float((out.double() - ref).norm()) <= tol + (2.0 ** -25 * (m * n) ** 0.5 if dtype == torch.float16 else 0)
+
+
+@pytest.mark.gpu
+def test_muon_update_of_a_gradient_below_eps():
+    gen = torch.Generator().manual_seed(8)
+    ps, gs = [], []
+    for m, n, r in ((60, 100, 1e-5), (300, 400, 1e-5), (24, 50, 1e-5), (90, 80, 1e3)):
+        g = torch.randn(m, n, generator=gen)
+        gs.append((g.double() / g.double().norm() * 1e-7 * r).float())
+        ps.append(torch.nn.Parameter(torch.zeros(m, n).cuda()))
+        ps[-1].grad = gs[-1].cuda()
+    optim.FusedMuon(ps, lr=0.5, momentum=0.0, weight_decay=0.0, nesterov=False).step()
+    for p, g in zip(ps, gs):
+        ref = -0.5 * math.sqrt(max(1.0, g.shape[0] / g.shape[1])) * chain(g, torch.float64)
+        d32 = -0.5 * math.sqrt(max(1.0, g.shape[0] / g.shape[1])) * chain(g, torch.float32).double() - ref
+        # as above; the rate and the product with it two roundings more
+        assert float((p.detach().cpu().double() - ref).norm()) <= 4 * float(d32.norm()) + 102 * 2.0 ** -24 * float(ref.norm())
+
+
 # ------------------------------------------------------------------------------------------------ the step's arguments
 @pytest.mark.gpu
 @pytest.mark.parametrize("make", [lambda ps: optim.FusedMuon(ps), lambda ps: optim.FusedSGD(ps, lr=0.1), lambda ps: optim.FusedAdam(ps), lambda ps: optim.FusedRAdam(ps)],
