@@ -515,7 +515,9 @@ int saunet_bucket_copy(const saunet_tensor_list* tl /*0:tensor 1:flat+offset*/, 
  * Intermediate matrices are float16 pairs (float32-class products); float32 accumulation, float64 norm.  A matrix that holds an Inf or NaN comes
  * out as NaN and leaves the others alone; a zero matrix stays zero.  SAUNET_UNSUPPORTED, nothing launched: coefficients under which some
  * starting singular value in [0, 1] leaves the range that the pairs can hold.  src may equal dst.
- * workspace: saunet_newton_schulz_workspace(d) bytes on a 256-byte border, private to the call until it has completed on `stream`. */
+ * workspace: saunet_newton_schulz_workspace(d) bytes on a 256-byte border, private to the call until it has completed on `stream`.  A matrix m x n,
+ * m <= n, takes 12 m n + 20 m^2 bytes of it (both rounded up to 64; 0.5 MB at most for m <= 32); a list that comes to more than 4 GiB goes in parts,
+ * one behind the other in the same memory: 4 GiB or the largest matrix, and some 0.1 GiB for cut tiles. */
 typedef struct saunet_ns_item {
     const void* src; void* dst;    /* matrix and result, row-major; Muon: gradient and parameter */
     float* buf;                    /* Muon: momentum buffer, contiguous */

@@ -1160,6 +1160,38 @@ static saunet_ns_desc ns_part(const saunet_ns_desc* d, bool muon, int k, saunet_
     return r;
 }
 
+// A list goes through the chain in parts of so many bytes of workspace, one behind the other in the same memory (a part holds one matrix at least): X, two
+// of X^T and five m x m matrices for each would come to eight times the parameters of a square one.  ms a call with parts of 1, 2, 4, 16 GiB: forty 2048 x 2048
+// 24.0, 23.7, 23.6, 23.4; sixty 512 x 13824 8.8, 8.0, 7.8, 7.8; 1500 of 256 x 1024 11.7, 11.2, 11.2, 10.9; nine 4096 x 11008 56.9, 59.7, 59.0, 59.3.
+constexpr long NS_PART = 4L << 30;
+// how many of the matrices from `from` on make the next part
+static int ns_next(const saunet_ns_desc* d, int from)
+{
+    long sum = 0;
+    for (int i = from; i < d->count; ++i) {
+        const saunet_ns_item& t = d->item[i];
+        const long elements = (long)t.rows * t.cols, cols = ((t.rows < t.cols ? t.cols : t.rows) + NSS_COLS - 1) / NSS_COLS;
+        sum += ns_is_small(d, t) ? (1 + (cols < 64 ? cols : 64)) * 8192 : NsView::bytes(t.rows, t.cols) + elements / (NS_NORM / 8);
+        if (sum > NS_PART && i > from) return i - from;
+    }
+    return d->count - from;
+}
+// fn(part) for every part of either chain until one returns an error
+template <typename F> static int ns_parts(const saunet_ns_desc* d, bool muon, saunet_ns_item* item, F fn)
+{
+    for (int k = 0; k < 2; ++k) {
+        const saunet_ns_desc chain = ns_part(d, muon, k, item);
+        for (int at = 0, n; at < chain.count; at += n) {
+            saunet_ns_desc part = chain;
+            part.item += at;
+            part.count = n = ns_next(&chain, at);
+            const int rc = fn(part);
+            if (rc) return rc;
+        }
+    }
+    return SAUNET_OK;
+}
+
 // Steps composed at once: see the head of this file.  The longest matrix is the first.  (Short ones in twos would gain little, measured with 64 x 64
 // tiles: one of 128 x 256 183 us, step by step 171; sixty of 128 x 64 .. 992 299 us against 324.)
 static const NsSchedule* ns_plan_schedule(const saunet_ns_desc* d, bool muon, const NsPlan& p, const NsItem* large)
@@ -1229,12 +1261,10 @@ template <typename T, bool MUON> static int ns_run(const saunet_ns_desc* d, bool
 template <typename T, bool MUON> static int ns_run_all(const saunet_ns_desc* d, const float* hyper, void* workspace, int64_t workspace_bytes, hipStream_t st, const char* who)
 {
     static thread_local saunet_ns_item item[4096];
-    for (int pass = 0; pass < 2; ++pass)
-        for (int k = 0; k < 2; ++k) {
-            const saunet_ns_desc part = ns_part(d, MUON, k, item);
-            const int rc = part.count ? ns_run<T, MUON>(&part, pass == 1, hyper, workspace, workspace_bytes, st, who) : SAUNET_OK;
-            if (rc) return rc;
-        }
+    for (int pass = 0; pass < 2; ++pass) {
+        const int rc = ns_parts(d, MUON, item, [&](const saunet_ns_desc& part) { return ns_run<T, MUON>(&part, pass == 1, hyper, workspace, workspace_bytes, st, who); });
+        if (rc) return rc;
+    }
     return SAUNET_OK;
 }
 
@@ -1253,13 +1283,14 @@ int64_t saunet_newton_schulz_workspace(const saunet_ns_desc* d)
     int rc = ns_check(d, "newton_schulz");
     int64_t most = 0;
     bool bad[2] = {false, false};                 // a use whose schedules leave the range: the step composes otherwise than the plain call
-    for (int k = 0; k < 4 && !rc; ++k) {          // one chain behind the other, in the same memory; for either use
-        const saunet_ns_desc part = ns_part(d, k & 2, k & 1, item);
-        if (!part.count) continue;
-        rc = ns_plan(&part, p, large, small, nullptr);
-        if (p.bytes > most) most = p.bytes;
-        if (!rc && !ns_plan_schedule(&part, k & 2, p, large)) bad[k >> 1] = true;
-    }
+    for (int use = 0; use < 2 && !rc; ++use)
+        rc = ns_parts(d, use == 1, item, [&](const saunet_ns_desc& part) {
+            const int status = ns_plan(&part, p, large, small, nullptr);
+            if (status) return status;
+            if (p.bytes > most) most = p.bytes;
+            if (!ns_plan_schedule(&part, use == 1, p, large)) bad[use] = true;
+            return (int)SAUNET_OK;
+        });
     if (!rc && bad[0] && bad[1]) return set_error(SAUNET_UNSUPPORTED, "newton_schulz: the coefficients drive singular values out of range");
     return rc ? rc : most;
 }

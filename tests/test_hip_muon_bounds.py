@@ -103,6 +103,47 @@ def test_a_narrow_finite_peak_comes_out_finite():
     assert float((out.double() - ref).norm()) <= 0.01 * float(ref.norm())
 
 
+# ------------------------------------------------------------------------------------------------ lists that outgrow one workspace
+def test_the_workspace_of_a_long_list_is_bounded():
+    def need(shapes):
+        d, hold = HF.ns_desc([v for m, n in shapes for v in (0, 0, 0, n, n, m, n)], L.F32, 5, COEFF, 1e-7)
+        return L.load().saunet_newton_schulz_workspace(C.byref(d))
+
+    one = need([(4096, 4096)])
+    assert 32 * 4096 ** 2 <= one <= 32 * 4096 ** 2 + (1 << 27)
+    cap = (4 << 30) + (1 << 28)
+    for shapes in ([(4096, 4096)] * 32, [(4096, 11008)] * 100, [(300, 700)] * 4000, [(24, 1152), (2000, 2100), (100, 9000)] * 1300):
+        assert one < need(shapes) <= cap
+    assert need([(16384, 16384)] * 3) <= need([(16384, 16384)]) + (1 << 28)            # a matrix of 8 GiB is a part of its own
+    assert need([(30, 30)] * 4096) < 1 << 28
+
+
+@pytest.mark.gpu
+def test_a_list_that_goes_in_parts():
+    """1400 matrices, 7 GiB of intermediate matrices: each as exact as alone, the first, the last and those around the border between the parts among them.
+    The Muon step of the same list too.  Tolerance: see the matrices below eps; s is not small here, so 128 d bounds the chain's own roundings of the last step"""
+    shapes = [(600, 700), (310, 40), (20, 300), (450, 460)]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    gs = [1e-2 * torch.randn(*shapes[i % 4], generator=gen, device="cuda") for i in range(1400)]
+    d, hold = HF.ns_desc([v for g in gs for v in (0, 0, 0, g.shape[1], g.shape[1], *g.shape)], L.F32, 5, COEFF, 1e-7)
+    assert sum(12 * m * n + 20 * min(m, n) ** 2 for m, n in (g.shape for g in gs)) > L.load().saunet_newton_schulz_workspace(C.byref(d)) > 1 << 31
+    outs = HF.newton_schulz(gs)
+    flat = [torch.nn.Parameter(torch.zeros_like(g)) for g in gs]
+    for p, g in zip(flat, gs):
+        p.grad = g
+    optim.FusedMuon(flat, lr=0.5, momentum=0.0, weight_decay=0.0, nesterov=False).step()
+    for i, (g, out, p) in enumerate(zip(gs, outs, flat)):
+        size = 0.5 * math.sqrt(max(1.0, g.shape[0] / g.shape[1]))
+        near = (-p.detach() / size - out).norm() <= 2e-5 * out.norm()        # all of them are there (a matrix left out or mixed up is off by its size)
+        assert near and out.norm() > 0, i
+        if i % 97 and i not in (1, 1398, 1399):
+            continue
+        ref = chain(g.cpu(), torch.float64)
+        tol = 4 * float((chain(g.cpu(), torch.float32).double() - ref).norm()) + 128 * 2.0 ** -24 * float(ref.norm())
+        assert float((out.cpu().double() - ref).norm()) <= tol
+        assert float((-p.detach().cpu().double() / size - ref).norm()) <= tol + 4 * 2.0 ** -24 * float(ref.norm())
+
+
 # ------------------------------------------------------------------------------------------------ matrices below eps
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n", [(40, 90), (300, 500), (700, 140), (1100, 1200), (20, 60), (200, 4000)])
