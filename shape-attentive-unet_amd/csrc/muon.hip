@@ -3,15 +3,20 @@
 //   X0 = G / max(|G|_F, eps);   S = X X^T,  X <- (a I + b S + c S^2) X,  `steps` times          (rows <= columns; the transpose otherwise)
 //
 // One call takes any number of matrices of any shapes: every launch below covers one phase of ALL of them, a workgroup finds its matrix in a
-// table of tile prefixes.  The whole chain is some twenty launches whatever the list is (two chains where it holds both short and long matrices).
+// table of tile prefixes.  The chain is some twenty launches for five steps whatever the list is, and one more behind each launch that cuts tiles (4096 x 4096:
+// 34 in all); two chains where newton_schulz gets both short and long matrices.
 //
 // Composition.  S_k+1 = P_k S_k P_k with P_k = a I + b S_k + c S_k^2, and all of them commute, so some steps run on the m x m matrices alone (S and
 // the product of the P_k) before X is touched: three, then two at a time; 6 m^2 n + 14 m^3 operations for five steps against 5 (3 m^2 n + m^3).  Equal for
 // a square, 2.4x less at n = 27 m.  What it costs in digits: an error of S grows by a^2 = 12 with every step it is carried through, and the product is
 // kept as (P_2 P_1 P_0 - a^3 I), up to 41 in size where s is near 1, for a result near 1.  In the first block the s^2 add up to 1, so the 41 are divided by
 // sqrt(m): three from m = 256 on, two before.  Later most s are near 1, so there P is kept as (a - 1) I + b S + c S^2, near zero, and two steps are composed.
-// Matrices of up to 128 rows go step by step.  Distance from float64 over that of the same chain in float32 matrices, gradient-like input, five steps:
-// 0.6 - 1.2 for 33 .. 128 rows (three + two: 1.4 - 4.6), 0.9 - 1.1 for 129 .. 255 (three + two: 1.2 - 3.8), 1.2 at 300, 0.8 at 512, 0.4 at 1000 and above.
+// newton_schulz takes matrices of up to 128 rows step by step, in a chain of their own.  Distance from float64 over that of the same chain in float32
+// matrices, gradient-like input, five steps: 0.6 - 1.2 for 33 .. 128 rows (three + two: 1.4 - 4.6), 0.9 - 1.1 for 129 .. 255 (three + two: 1.2 - 3.8), 1.2 at
+// 300, 0.8 at 512, 0.4 at 1000 and above.
+// A Muon step whose list holds a matrix of more than 128 rows takes ALL its matrices of more than 32 through one chain of three + two, at the distances in
+// brackets (33 x 40 3.9, 64 x 576 1.5, 128 x 736 1.1; two + two + one: 1.4, 0.6, 0.6): there the update is multiplied by the rate and added to a rounded
+// parameter.  SAUNet's step 936 us; with two + two + one 1112, in two chains 1090.
 //
 // Number format.  Every matrix between the first and the last pass is a pair of float16 planes, x = hi + lo to 2^-24 (nt_tiles.h: 128-byte blocks of 32
 // elements), scaled by a power of two that the host derives from the singular values' range.  A product is then three float16 MFMAs with float32

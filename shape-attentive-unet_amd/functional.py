@@ -2294,7 +2294,9 @@ def newton_schulz(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
 
     ``g``: [..., m, n] in float32, bfloat16 or float16 (leading dimensions: a batch), or a list of such tensors of any shapes and one dtype on
     one device.  Returns the same shapes and dtype (a list for a list).  Every intermediate is of float32 class whatever the dtype; all matrices of the
-    call go through one chain of about twenty launches (two where short and long ones meet).  A matrix that holds an Inf or NaN comes out as NaN; a zero matrix stays zero.
+    call go through one chain of launches -- twenty to thirty-five -- or two where matrices of up to 128 and of more rows meet, in parts where their
+    intermediates would take more than 4 GiB.  A call repeats itself bit for bit; the same matrix in another list may differ in its last digits, because tiles
+    and cuts of the sums follow the whole list.  A matrix that holds an Inf or NaN comes out as NaN; a zero matrix stays zero.
     Coefficients under which singular values in [0, 1] grow out of range are refused.  Not differentiable: an optimiser's update is its use."""
     ns_check_hyper(steps, coefficients, eps)
     many = isinstance(g, (list, tuple))

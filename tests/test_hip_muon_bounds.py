@@ -144,6 +144,21 @@ def test_a_list_that_goes_in_parts():
         assert float((-p.detach().cpu().double() / size - ref).norm()) <= tol + 4 * 2.0 ** -24 * float(ref.norm())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes,dtype", [([(1000, 1024)] * 6, torch.bfloat16), ([(300, 900)], torch.float32), ([(520, 530)] + [(130, 131)] * 100, torch.float32),
+                                          ([(200, 210)] * 60, torch.float16), ([(64, 5000), (30, 40)], torch.float32)],
+                         ids=["stack", "one", "short behind", "uniform", "wide"])
+def test_a_call_repeats_itself_bit_for_bit(shapes, dtype):
+    """whatever the workspace held before"""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    gs = [(1e-2 * torch.randn(*s, generator=gen, device="cuda")).to(dtype) for s in shapes]
+    ref = [x.clone() for x in HF.newton_schulz(gs)]
+    for i in range(4):
+        junk = torch.full((1 << 27,), (float("nan"), 1e30, float("-inf"), 0.0)[i], device="cuda")
+        del junk
+        assert all(torch.equal(a, b) for a, b in zip(HF.newton_schulz(gs), ref))
+
+
 # ------------------------------------------------------------------------------------------------ matrices below eps
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n", [(40, 90), (300, 500), (700, 140), (1100, 1200), (20, 60), (200, 4000)])
@@ -187,6 +202,76 @@ def test_muon_update_of_a_gradient_below_eps():
         d32 = -0.5 * math.sqrt(max(1.0, g.shape[0] / g.shape[1])) * chain(g, torch.float32).double() - ref
         # as above; the rate and the product with it two roundings more
         assert float((p.detach().cpu().double() - ref).norm()) <= 4 * float(d32.norm()) + 102 * 2.0 ** -24 * float(ref.norm())
+
+
+# ------------------------------------------------------------------------------------------------ lists of long and short matrices
+def composed(g, dtype, first=3, later=2, coeff=COEFF, eps=1e-7):
+    """five steps of the chain with `first` and then `later` of them composed on the m x m matrices before X is touched: S' = (a + P)^2 S and Q, the product
+    of the factors a + P less the product of the a, with P = b S + c S^2 in the first block and (a - 1) more, a = 1, behind it"""
+    a0, b, c = coeff
+    x = g.to(dtype)
+    tall = x.shape[0] > x.shape[1]
+    x = x.t().contiguous() if tall else x
+    x = x / x.double().norm().clamp(min=eps).to(dtype)
+    done = 0
+    while done < 5:
+        nb = min(5 - done, later if done else first)
+        a = 1.0 if done else a0
+        s = x @ x.t()
+        eye = torch.eye(s.shape[0], dtype=dtype)
+        for j in range(nb):
+            p = b * s + c * (s @ s) + (a0 - a) * eye
+            big, q = (p, a) if j == 0 else (a * big + q * p + p @ big, q * a)
+            if j < nb - 1:
+                r = a * s + p @ s
+                s = a * r + r @ p
+        x = q * x + big @ x
+        done += nb
+    return x.t().contiguous() if tall else x
+
+
+LISTS = {"40 to 300 rows": [(40, 90), (300, 500), (700, 200), (20, 60), (33, 40), (171, 70), (128, 736), (64, 576), (257, 33)],
+         "wide and tall": [(520, 4000), (33, 50), (4000, 520), (100, 3000)],
+         "few": [(130, 140), (40, 50)]}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(LISTS))
+@pytest.mark.parametrize("kind", ["gauss", "lowrank"])
+def test_muon_update_in_a_list_of_long_and_short_matrices(name, kind):
+    """One matrix of more than 128 rows takes the whole list of a Muon step into the composed chain; the bare update (parameters zero) of each.
+
+    Tolerance: an operand of a product is off by 2^-23 of itself and the dropped low parts are another 2^-22 of the product, four times float32's two half
+    steps; so four times the distance of the same composed recurrences in float32, and 128 half steps of the result for inputs on which those are exact by
+    luck.  The rate, its product, this division and the subtraction are half a step each.  Both rules of the rate, and a parameter that is not zero."""
+    gen = torch.Generator().manual_seed(12)
+    shapes = LISTS[name]
+    gs = []
+    for m, n in shapes:
+        g = torch.randn(m, n, generator=gen)
+        if kind == "lowrank":
+            r = max(1, min(m, n) // 16)
+            g = torch.randn(m, r, generator=gen) @ torch.randn(r, n, generator=gen) / r ** 0.5 + 0.5 * g
+        gs.append(1e-3 * g)
+    refs, tols = [], []
+    for g in gs:
+        ref = chain(g, torch.float64)
+        assert float((composed(g, torch.float64) - ref).norm()) <= 1e-9 * float(ref.norm())
+        own = chain if min(g.shape) <= 32 else composed
+        refs.append(ref)
+        tols.append(4 * float((own(g, torch.float32).double() - ref).norm()) + 128 * 2.0 ** -24 * float(ref.norm()))
+    for adjust, wd, p0 in ((None, 0.0, 0.0), ("match_rms_adamw", 0.1, 0.5)):
+        starts = [p0 * torch.randn(g.shape, generator=gen) for g in gs]
+        ps = [torch.nn.Parameter(p.cuda()) for p in starts]
+        for p, g in zip(ps, gs):
+            p.grad = g.cuda()
+        optim.FusedMuon(ps, lr=0.25, momentum=0.0, weight_decay=wd, nesterov=False, adjust_lr_fn=adjust).step()
+        for p, start, ref, tol in zip(ps, starts, refs, tols):
+            m, n = ref.shape
+            rate = 0.25 * (0.2 * math.sqrt(max(m, n)) if adjust else math.sqrt(max(1, m / n)))
+            want = start.double() * (1 - 0.25 * wd) - rate * ref
+            d = float((p.detach().cpu().double() - want).norm())
+            assert d <= rate * (tol + 4 * 2.0 ** -24 * float(ref.norm())) + 3 * 2.0 ** -24 * float(start.norm() + want.norm()), (m, n, d / rate, tol)
 
 
 # ------------------------------------------------------------------------------------------------ the step's arguments
