@@ -271,7 +271,7 @@ template <typename T, class Core> static int mm8_tiles(I8Args g, hipStream_t st)
     if (once.first()) (void)hipFuncSetAttribute((const void*)matmul_int8_kernel<T, Core>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     g.tn = cdiv(g.n, Core::BM);
     const long tiles = (g.m + Core::BN - 1) / Core::BN * g.tn;
-    if (tiles > 0x7fffffff) return set_error(SAUNET_BAD_SHAPE, "matmul_int8: %ld tiles", tiles);
+    if (tiles > 0xffffffffL / Core::NT) return set_error(SAUNET_BAD_SHAPE, "matmul_int8: %ld rows of %d channels are too much for one launch", g.m, g.n);
     hipLaunchKernelGGL((matmul_int8_kernel<T, Core>), dim3((unsigned)tiles), dim3(Core::NT), LDS, st, g);
     SAUNET_CHECK_LAUNCH("matmul_int8");
     return SAUNET_OK;
@@ -464,13 +464,17 @@ int saunet_quantize_rows(int dtype, const void* x, int64_t ldx, int64_t rows, in
     if (rows == 0) return SAUNET_OK;
     if (!x || !q || !s || (!scale) != (!shift)) return set_error(SAUNET_BAD_SHAPE, "quantize_rows: missing memory");
     if ((uintptr_t)q & 15) return set_error(SAUNET_BAD_ALIGN, "quantize_rows: q has to lie on a 16-byte border");
-    if (rows > 0x7fffffffL * 4) return set_error(SAUNET_BAD_SHAPE, "quantize_rows: %lld rows", (long long)rows);
     const int size = dtype == SAUNET_F32 ? 4 : 2;
-    QArgs a = {x, ldx, rows, k, scale, shift, relu, (signed char*)q, ldq, s, !(((uintptr_t)x | (uintptr_t)scale | (uintptr_t)shift) & 15) && !(ldx * size & 15)};
     hipStream_t st = (hipStream_t)stream;
-    if (scale || relu) dtype == SAUNET_F32 ? q_launch<float, true>(a, st) : dtype == SAUNET_BF16 ? q_launch<u16, true>(a, st) : q_launch<_Float16, true>(a, st);
-    else dtype == SAUNET_F32 ? q_launch<float, false>(a, st) : dtype == SAUNET_BF16 ? q_launch<u16, false>(a, st) : q_launch<_Float16, false>(a, st);
-    SAUNET_CHECK_LAUNCH("quantize_rows");
+    constexpr int64_t MOST = 1 << 23;                // rows a launch: up to 256 threads a row, and a launch has fewer than 2^32
+    for (int64_t r0 = 0; r0 < rows; r0 += MOST) {
+        const char* xr = (const char*)x + r0 * ldx * size;
+        const QArgs a = {xr, ldx, rows - r0 < MOST ? rows - r0 : MOST, k, scale, shift, relu, (signed char*)q + r0 * ldq, ldq, s + r0,
+                         !(((uintptr_t)xr | (uintptr_t)scale | (uintptr_t)shift) & 15) && !(ldx * size & 15)};
+        if (scale || relu) dtype == SAUNET_F32 ? q_launch<float, true>(a, st) : dtype == SAUNET_BF16 ? q_launch<u16, true>(a, st) : q_launch<_Float16, true>(a, st);
+        else dtype == SAUNET_F32 ? q_launch<float, false>(a, st) : dtype == SAUNET_BF16 ? q_launch<u16, false>(a, st) : q_launch<_Float16, false>(a, st);
+        SAUNET_CHECK_LAUNCH("quantize_rows");
+    }
     return SAUNET_OK;
 }
 
