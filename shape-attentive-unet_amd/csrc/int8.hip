@@ -257,6 +257,13 @@ template <typename T, class Core> __global__ __launch_bounds__(Core::NT) void ma
 //   2048 x 2048, K 2048  (1024 tiles)  22.4    19.7     15.5      15.8     33.5
 //   8192 x 256, K 8192    (512 tiles)  42.6    33.2     49.8      40.8      101      too few large tiles to fill the card: the smallest that do
 //   512 x 512, K 512       (64 tiles)   4.4     5.4      5.7       6.2     14.1
+// Where one side is short a wide tile multiplies rows that do not exist.  Up to 64 the smallest tile wins whatever the work, the largest one from some 192 on:
+//   200000 x 8, K 1024                 34.1    49.6      42.6      45.4     88.5
+//   60000 x 40, K 2048                 22.3    28.7      23.1      24.3     38.2
+//   64 x 200000, K 1024                37.0    37.1      45.0      46.0     86.7
+//   200000 x 65, K 1024                75.5    59.5      59.6      65.2      104
+//   200000 x 160, K 1024               86.9    96.4      81.9      84.2     93.6
+//   200000 x 200, K 1024                124     107      95.5      95.5      100
 typedef NtCore<NtI8, 64, 64, 2, 2, 4> I8Core64;
 typedef NtCore<NtI8, 128, 64, 2, 2, 4> I8CoreTall;
 typedef NtCore<NtI8, 128, 128, 2, 4, 2> I8Core128;
@@ -420,7 +427,9 @@ template <typename T> static int mm8_launch(const I8Args& g, hipStream_t st)
         return SAUNET_OK;
     }
     const long t64 = ((g.m + 63) / 64) * ((g.n + 63) / 64);
-    if (t64 >= 192 * 16 && g.ksteps >= 8) return mm8_tiles<T, I8Core256>(g, st);
+    const long side = g.m < g.n ? g.m : g.n;
+    if (side <= 64) return mm8_tiles<T, I8Core64>(g, st);
+    if (t64 >= 192 * 16 && g.ksteps >= 8 && side > 192) return mm8_tiles<T, I8Core256>(g, st);
     if (t64 <= 384) return mm8_tiles<T, I8Core64>(g, st);
     if (t64 <= 768) return mm8_tiles<T, I8CoreTall>(g, st);
     return g.ksteps >= 64 ? mm8_tiles<T, I8Core128L>(g, st) : mm8_tiles<T, I8Core128>(g, st);
