@@ -2350,8 +2350,9 @@ def _int8_stride(k):
 class Int8Rows:
     """Rows of int8 with one float32 scale each -- quantised tokens (pixels) or the output channels of a weight: row r stands for q[r] * scale[r].
 
-    Storage is padded with zeros to whole 64-byte steps of the reduction, once, so that the products need no tail.  Build it with ``quantize_rows``
-    or from existing ``q`` [..., k] int8 and ``scale`` [...] float32 (copied when the layout asks for it)."""
+    Storage is padded with zeros to whole 64-byte steps of the reduction, once, so that the products need no tail.  Build it with ``quantize_rows``,
+    whose rows have that layout, or from existing ``q`` [..., k] int8 and ``scale`` [...] float32: contiguous rows on a 16-byte border with k a multiple
+    of 64 are shared with the caller (a later change of ``q`` or ``scale`` is seen by the products); any others are copied, a full pass over them."""
 
     def __init__(self, q, scale):
         _check_dev(q); _check_dev(scale)
@@ -2423,6 +2424,8 @@ def quantize_rows(x, affine=None, relu=False):
             _check_dev(t)
             if t.dtype != torch.float32 or t.numel() != k or not t.is_contiguous() or t.device != x.device:
                 raise RuntimeError("quantize_rows: affine is two contiguous float32 vectors of %d elements beside x" % k)
+            if torch.is_grad_enabled() and t.requires_grad:
+                raise RuntimeError("quantize_rows serves inference: call it under torch.no_grad() or with a detached affine")
     rows, ld = v.shape[0], _int8_stride(k)
     data = torch.empty(rows, ld, dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
@@ -2455,6 +2458,8 @@ def _int8_bias(bias, n, device):
         return None
     if bias.numel() != n or bias.device != device:
         raise RuntimeError("bias has to hold %d elements on %s" % (n, device))
+    if torch.is_grad_enabled() and bias.requires_grad:
+        raise RuntimeError("int8 products serve inference: call them under torch.no_grad() or with a detached bias")
     return bias if bias.dtype == torch.float32 and bias.is_contiguous() else bias.detach().float().contiguous()
 
 

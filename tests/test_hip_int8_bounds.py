@@ -42,3 +42,37 @@ def test_tall_and_narrow_products(m, k, n):
     ref, size = (p + bias.double()).clamp(min=0), p.abs() + bias.double().abs()
     tol = 4 * 2.0 ** -24 * size + 2.0 ** -8 * (ref + 4 * 2.0 ** -24 * size)
     assert ((y.double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+def test_a_bias_or_affine_that_asks_for_a_gradient_is_refused():
+    x, w = rows(5, 96, 1).cuda(), HF.quantize_rows(rows(7, 96, 2).cuda())
+    bias, sc, sh = (torch.randn(n).cuda().requires_grad_() for n in (7, 96, 96))
+    a = HF.quantize_rows(x)
+    for f in (lambda: HF.matmul_int8(a, w, bias=bias), lambda: HF.linear_int8(x, w, bias=bias), lambda: HF.quantize_rows(x, affine=(sc, sh)),
+              lambda: HF.quantize_rows(x, affine=(sc.detach(), sh)), lambda: HF.pointwise_int8(x.view(5, 96, 1, 1), w, bias)):
+        with pytest.raises(RuntimeError, match="inference"):
+            f()
+    with torch.no_grad():
+        y, r = HF.linear_int8(x, w, bias=bias), HF.quantize_rows(x, affine=(sc, sh))
+    assert torch.equal(y, HF.linear_int8(x, w, bias=bias.detach())) and torch.equal(r.data, HF.quantize_rows(x, affine=(sc.detach(), sh.detach())).data)
+
+
+@pytest.mark.gpu
+def test_int8_rows_share_or_copy():
+    q, s = torch.randint(-127, 128, (6, 128), dtype=torch.int8).cuda(), torch.rand(6).cuda()
+    shared, copied = HF.Int8Rows(q, s), HF.Int8Rows(q[:, :100], s)
+    assert shared.data.data_ptr() == q.data_ptr() and copied.data.data_ptr() != q.data_ptr()
+    w = HF.quantize_rows(rows(9, 128, 3).cuda())
+    before = HF.matmul_int8(shared, w, dtype=torch.float32)
+    q.zero_()
+    assert before.any() and not HF.matmul_int8(shared, w, dtype=torch.float32).any() and copied.q.any()
+
+
+@pytest.mark.gpu
+def test_pointwise_int8_of_an_empty_batch_and_one_pixel():
+    w = HF.quantize_rows(rows(20, 64, 4).cuda())
+    assert HF.pointwise_int8(torch.zeros(0, 64, 8, 8).cuda(), w).shape == (0, 20, 8, 8)
+    x = rows(1, 64, 5).cuda()
+    y = HF.pointwise_int8(x.view(1, 64, 1, 1), w)
+    assert torch.equal(y.view(1, 20), HF.linear_int8(x, w))
