@@ -2269,7 +2269,7 @@ def ns_desc(rows, dtype, steps, coefficients, eps, adjust=0):
     n = len(rows) // 7
     items = struct.pack("@" + "PPPqqii" * n, *rows)
     buf = C.create_string_buffer(items, len(items))
-    return L.NsDesc(C.addressof(buf), n, dtype, steps, adjust, coefficients[0], coefficients[1], coefficients[2], eps), buf
+    return L.NsDesc(C.addressof(buf), n, dtype, int(steps), adjust, coefficients[0], coefficients[1], coefficients[2], eps), buf
 
 
 def ns_workspace(d, device):

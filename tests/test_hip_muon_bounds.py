@@ -275,6 +275,12 @@ def test_muon_update_in_a_list_of_long_and_short_matrices(name, kind):
 
 
 # ------------------------------------------------------------------------------------------------ the step's arguments
+def test_whole_steps_of_any_number_type():
+    for steps in (5, 5.0, np.int64(5), np.float32(5)):
+        HF.ns_check_hyper(steps, COEFF, 1e-7)
+        assert HF.ns_desc([0] * 7, L.F32, steps, COEFF, 1e-7)[0].steps == 5
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("make", [lambda ps: optim.FusedMuon(ps), lambda ps: optim.FusedSGD(ps, lr=0.1), lambda ps: optim.FusedAdam(ps), lambda ps: optim.FusedRAdam(ps)],
                          ids=["muon", "sgd", "adam", "radam"])
