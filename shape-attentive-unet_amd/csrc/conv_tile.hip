@@ -2053,8 +2053,9 @@ __global__ __launch_bounds__(512, 1) void conv3x3_wgrad_sc_kernel(ScArgs a)
     auto tf_activate = [&](u32x4& v, int j, const Cur& c) {
         const int id = j * 8 + wave;
         if (id < SC_DY_PIECES || id >= SC_PIECES) return;
-        // per channel pair: unpack (2), v_pk_fma_f32 (1), v_cvt_pk_bf16_f32 (1), ReLU on the PACKED pair as v_pk_max_i16 against 0 (a negative
-        // bf16 is a negative int16) (1), mask (1): 24 VALU instructions per 16 bytes instead of 40 -- the activation is what bounds this kernel
+        // per channel pair: unpack (2), multiply-add (2; the build keeps the packed float32 one out, _build.py), v_cvt_pk_bf16_f32 (1), ReLU on the
+        // PACKED pair as v_pk_max_i16 against 0 (a negative bf16 is a negative int16) (1), mask (1): 28 VALU instructions per 16 bytes instead of 40
+        // -- the activation is what bounds this kernel
         const unsigned okm = inside(j, c) ? 0xffffffffu : 0u;
         typedef __attribute__((ext_vector_type(2))) float f32x2_t;
         typedef __attribute__((ext_vector_type(2))) short s16x2_t;

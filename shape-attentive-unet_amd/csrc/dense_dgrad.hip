@@ -1311,9 +1311,9 @@ __global__ __launch_bounds__(512) void dense_conv1_dgrad_pair_kernel(DenseDgradP
         TSTAMP(97);
         // layer l's product (matrix pipe) runs under layer l - 1's half of the epilogue (vector pipe): the two waves of a SIMD are in the same
         // phase (one barrier per step), so the overlap has to be in the instruction stream
-        // Two pixels per instruction: v_pk_fma_f32 / v_pk_add_f32 on register pairs (the accumulator rows r, r + 1 are consecutive pixels of the
-        // lane's channel) -- 23 vector instructions per pixel pair instead of 34; with two waves per SIMD in the same phase the epilogue's
-        // issue time is the stage's longest part.
+        // Two pixels at a time, on register pairs (the accumulator rows r, r + 1 are consecutive pixels of the lane's channel).  Packed float32
+        // instructions made that 23 vector instructions a pixel pair instead of 34; the build keeps them out of the code (_build.py), so each is two
+        // again.  With two waves per SIMD in the same phase the epilogue's issue time is the stage's longest part.
         typedef float f2 __attribute__((ext_vector_type(2)));
         const bool cok = j * LY::BN + col < a.Cin;
         f2 s1a = {0.f, 0.f}, s2a = {0.f, 0.f}, s1b = {0.f, 0.f}, s2b = {0.f, 0.f};

@@ -18,10 +18,11 @@
 // brackets (33 x 40 3.9, 64 x 576 1.5, 128 x 736 1.1; two + two + one: 1.4, 0.6, 0.6): there the update is multiplied by the rate and added to a rounded
 // parameter.  SAUNet's step 936 us; with two + two + one 1112, in two chains 1090.
 //
-// Number format.  Every matrix between the first and the last pass is a pair of float16 planes, x = hi + lo to 2^-24 (nt_tiles.h: 128-byte blocks of 32
+// Number format.  Every matrix between the first and the last pass is a pair of float16 planes, x = hi + lo to 2^-23 (nt_tiles.h: 128-byte blocks of 32
 // elements), scaled by a power of two that the host derives from the singular values' range.  A product is then three float16 MFMAs with float32
-// accumulation, at a sixth of the cost of the float32 MFMA and with no more error.  Products of symmetric matrices compute the lower tiles only and
-// write both halves.  X and X^T are both kept: each is the operand with the contiguous reduction index in one of the two rectangular products.
+// accumulation, at a sixth of the cost of the float32 MFMA; its operands and the dropped low parts can cost four times float32's half steps, measured the whole
+// chain is about as far from float64 as the float32 one (above).  Products of symmetric matrices compute the lower tiles only and write both halves.
+// X and X^T are both kept: each is the operand with the contiguous reduction index in one of the two rectangular products.
 #include "nt_tiles.h"
 #include <algorithm>
 

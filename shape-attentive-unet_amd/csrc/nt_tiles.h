@@ -49,8 +49,9 @@ __device__ __forceinline__ void nt_band(int t, int rows, int cols, int& r, int& 
     c = in / h;
 }
 
-// float16 pairs: a row is a sequence of blocks of 32 elements, each 64 bytes of high parts followed by 64 bytes of low parts (x = hi + lo to 2^-24
-// of x).  hi hi + hi lo + lo hi in float32; what is dropped, lo lo, is below 2^-24 of |a| |b|.
+// float16 pairs: a row is a sequence of blocks of 32 elements, each 64 bytes of high parts followed by 64 bytes of low parts.  Two
+// significands of 11 bits and the sign of lo are 23 bits: x = hi + lo to 2^-23 of x (a quarter of the float32 numbers in [1, 2) are off by more than 2^-24).
+// hi hi + hi lo + lo hi in float32; |lo| <= 2^-11 |x|, so what is dropped, lo lo, is up to 2^-22 of |a| |b|.
 struct NtF16Pair {
     // the MFMA's adder cuts off instead of rounding, which over a long sum of one sign is a bias: 256 additions cost 6e-6 of the sum.  Every FLUSH stages the
     // accumulators are added to a float32 total and start again.

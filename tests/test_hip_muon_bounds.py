@@ -25,6 +25,18 @@ def chain(g, dtype, steps=5, coeff=COEFF, eps=1e-7):
     return x.t().contiguous() if tall else x
 
 
+# ------------------------------------------------------------------------------------------------ the number format (no GPU needed)
+def test_what_a_pair_of_float16_holds():
+    """the figures that the tolerances below count with: x = hi + lo to 2^-23 of x, and |lo| <= 2^-11 |x|"""
+    x = np.float32(1) + np.random.default_rng(0).integers(0, 1 << 23, 1 << 20).astype(np.float32) * np.float32(2.0 ** -23)
+    hi = x.astype(np.float16)
+    rest = x - hi.astype(np.float32)                                     # exact
+    lo = rest.astype(np.float16)
+    off = np.abs(x.astype(np.float64) - hi.astype(np.float64) - lo.astype(np.float64)) / x
+    assert off.max() <= 2.0 ** -23 and (np.abs(lo.astype(np.float64)) <= 2.0 ** -11 * x).all()
+    assert 0.2 < (off > 2.0 ** -24).mean() < 0.3
+
+
 # ------------------------------------------------------------------------------------------------ coefficients (no GPU needed)
 def workspace(rows, cols, steps, coeff):
     """bytes, or the status of a call that cannot be made: nothing is launched"""
