@@ -556,7 +556,7 @@ typedef struct saunet_int8_desc {
 int saunet_matmul_int8(const saunet_int8_desc* d, void* stream);
 /* the same from m floating-point rows x (dtype x_dtype, ldx elements a row), quantised as saunet_quantize_rows does; a, a_scale and lda are not used.
  * workspace: m (k rounded up to 64) + 4 m bytes on a 16-byte border, private to the call until it has completed on `stream` (not touched, and
- * may be NULL, for one row of up to 16384 elements) */
+ * may be NULL, for one row of up to 16384 elements).  y must not overlap x. */
 int saunet_linear_int8(const saunet_int8_desc* d, int x_dtype, const void* x, int64_t ldx, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

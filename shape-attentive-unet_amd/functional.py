@@ -2486,7 +2486,7 @@ def matmul_int8(a, b, bias=None, relu=False, dtype=torch.bfloat16, out=None):
 
 def linear_int8(x, w, bias=None, relu=False, dtype=None, out=None):
     """A linear layer over rows x [..., k] with an int8 weight ``w`` (Int8Rows [n, k]): the rows are quantised on the way (quantize_rows), the product is
-    matmul_int8's -- the same result as the two calls, bit for bit.  ``dtype``: the result's, x's by default."""
+    matmul_int8's -- the same result as the two calls, bit for bit.  ``dtype``: the result's, x's by default.  ``out`` may lie in x's memory."""
     v, k = _float_rows(x, "linear_int8")
     if not isinstance(w, Int8Rows) or len(w.lead) != 1:
         raise RuntimeError("linear_int8 takes an Int8Rows weight [n, k]")
@@ -2494,6 +2494,9 @@ def linear_int8(x, w, bias=None, relu=False, dtype=None, out=None):
         raise RuntimeError("linear_int8: %s on %s does not meet %s on %s" % (tuple(x.shape), x.device, w.shape, w.device))
     rows, n = v.shape[0], w.lead[0]
     dtype = x.dtype if dtype is None else dtype
+    if out is not None and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
+        # every workgroup of the one-launch form reads all rows: they have to be quantised before the first result is written
+        return matmul_int8(quantize_rows(x), w, bias, relu, dtype, out=out)
     y, yv = _int8_out(x.shape[:-1], rows, n, dtype, x.device, out)
     bias = _int8_bias(bias, n, x.device)
     if rows and n:

@@ -76,3 +76,15 @@ def test_pointwise_int8_of_an_empty_batch_and_one_pixel():
     x = rows(1, 64, 5).cuda()
     y = HF.pointwise_int8(x.view(1, 64, 1, 1), w)
     assert torch.equal(y.view(1, 20), HF.linear_int8(x, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k", [(1, 4096), (3, 1024), (8, 512), (40, 300)])
+def test_linear_int8_into_its_own_input(m, k):
+    x, w = rows(m, k, 7).cuda(), HF.quantize_rows((rows(k, k, 8) / k).cuda())
+    ref = HF.linear_int8(x, w)
+    wide = torch.zeros(m, k + 8, device="cuda")
+    wide[:, 8:] = x
+    for buf, out in ((x.clone(), None), (wide[:, 8:], wide[:, :k])):        # the same memory, and rows shifted against each other
+        out = buf if out is None else out
+        assert HF.linear_int8(buf, w, out=out) is out and torch.equal(out, ref)
