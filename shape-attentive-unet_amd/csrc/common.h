@@ -246,6 +246,16 @@ struct DeviceOnce {
         __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
         return true;
     }
+    // the attribute itself, marked as set only behind it: a second thread never launches in front of it
+    void lds(const void* kernel, int bytes)
+    {
+        int dev = 0;
+        (void)hipGetDevice(&dev);
+        const unsigned long long bit = 1ull << (dev & 63);
+        if (__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit) return;
+        (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
+    }
 };
 // the same for launch sites whose requirement grows with the problem: true when `lds` exceeds what this device was last given
 struct DeviceMaxLds {

@@ -275,7 +275,7 @@ template <typename T, class Core> static int mm8_tiles(I8Args g, hipStream_t st)
     constexpr int EPI = Core::BM * 8 + Core::NW * 32 * (Core::BM / Core::WGM * (int)sizeof(T) + 16), LDS = Core::LDS > EPI ? Core::LDS : EPI;
     static_assert(LDS <= 160 * 1024, "the wave's rows fit");
     static DeviceOnce once;
-    if (once.first()) (void)hipFuncSetAttribute((const void*)matmul_int8_kernel<T, Core>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    once.lds((const void*)matmul_int8_kernel<T, Core>, LDS);
     g.tn = cdiv(g.n, Core::BM);
     const long tiles = (g.m + Core::BN - 1) / Core::BN * g.tn;
     if (tiles > 0xffffffffL / Core::NT) return set_error(SAUNET_BAD_SHAPE, "matmul_int8: %ld rows of %d channels are too much for one launch", g.m, g.n);

@@ -1135,14 +1135,14 @@ static const NsSchedule* ns_schedule(const saunet_ns_desc* d, int first, int lat
 template <class Core, typename T, int MODE> static void ns_launch_apply(const saunet_ns_desc* d, const NsPlan& p, const NsTable& tab, const NsOp& o, const float* hyper, hipStream_t st)
 {
     static DeviceOnce once;
-    if (once.first()) (void)hipFuncSetAttribute((const void*)ns_apply_kernel<Core, T, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
+    once.lds((const void*)ns_apply_kernel<Core, T, MODE>, Core::LDS);
     hipLaunchKernelGGL((ns_apply_kernel<Core, T, MODE>), dim3(ns_deal_grid(p.deal[NS_KINDS])), dim3(Core::NT), Core::LDS, st, tab, o.q, o.xt, o.alpha, o.beta, o.grown, o.grown_to, hyper, d->adjust, p.deal[NS_KINDS]);
 }
 template <class Core> static void ns_launch_prod(const NsPlan& p, const NsTable& tab, const NsOp& o, hipStream_t st)
 {
     const int kind = o.gram ? NS_GRAM : o.ny == 2 ? NS_TWO : NS_ONE;
     static DeviceOnce once;
-    if (once.first()) (void)hipFuncSetAttribute((const void*)ns_prod_kernel<Core>, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
+    once.lds((const void*)ns_prod_kernel<Core>, Core::LDS);
     const unsigned dealt = ns_deal_grid(p.deal[kind]);
     hipLaunchKernelGGL((ns_prod_kernel<Core>), dim3(dealt + (unsigned)(p.grid[kind] - p.deal[kind].b[8]), o.ny), dim3(Core::NT), Core::LDS, st, tab, kind, o.pr, o.grown, p.deal[kind], (int)dealt);
     if constexpr (Core::KW == 1) if (p.cut[kind]) hipLaunchKernelGGL((ns_finish_kernel<Core>), dim3((unsigned)(p.cut[kind] * NsQuads<Core>::N), o.ny), dim3(Core::NT), 0, st, tab, kind, o.pr, o.grown);

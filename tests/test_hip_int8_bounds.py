@@ -1,5 +1,8 @@
 """What the int8 operators do at the borders of their domain: more rows than a launch has threads for, arguments that would lose a gradient, tall and narrow
 products, memory that is shared or copied."""
+import ctypes as C
+import threading
+
 import pytest
 import torch
 
@@ -88,3 +91,31 @@ def test_linear_int8_into_its_own_input(m, k):
     for buf, out in ((x.clone(), None), (wide[:, 8:], wide[:, :k])):        # the same memory, and rows shifted against each other
         out = buf if out is None else out
         assert HF.linear_int8(buf, w, out=out) is out and torch.equal(out, ref)
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once():
+    """each on a stream of its own, the first calls of several kernels among them"""
+    x, w = rows(700, 900, 1).cuda(), HF.quantize_rows(rows(5000, 900, 2).cuda())
+    g = [1e-2 * rows(m, n, m).cuda() for m, n in ((20, 70), (150, 400), (500, 600))]
+    torch.cuda.synchronize()
+    outs, errors = {}, []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    outs[k] = (HF.linear_int8(x, w), HF.linear_int8(x[:1], w), *HF.newton_schulz(g, steps=5 + k))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:              # noqa: BLE001 -- reported by the assertion below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for k in range(2):
+        want = (HF.linear_int8(x, w), HF.linear_int8(x[:1], w), *HF.newton_schulz(g, steps=5 + k))
+        assert all(torch.equal(a, b) for a, b in zip(outs[k], want))

@@ -131,6 +131,22 @@ def test_the_workspace_of_a_long_list_is_bounded():
 
 
 @pytest.mark.gpu
+def test_a_list_of_more_matrices_than_a_call_takes():
+    gs = [1e-2 * torch.randn(3 + i % 5, 4 + i % 3, generator=torch.Generator().manual_seed(i)) for i in range(L.NS_ITEMS_MAX + 5)]
+    outs = HF.newton_schulz([g.cuda() for g in gs])
+    ps = [torch.nn.Parameter(torch.zeros(g.shape).cuda()) for g in gs]
+    for p, g in zip(ps, gs):
+        p.grad = g.cuda()
+    optim.FusedMuon(ps, lr=0.5, momentum=0.0, weight_decay=0.0, nesterov=False).step()
+    for i in list(range(0, 40)) + list(range(L.NS_ITEMS_MAX - 3, L.NS_ITEMS_MAX + 5)):
+        ref = chain(gs[i], torch.float64)
+        tol = 4 * float((chain(gs[i], torch.float32).double() - ref).norm()) + 128 * 2.0 ** -24 * float(ref.norm())
+        assert float((outs[i].cpu().double() - ref).norm()) <= tol
+        rate = 0.5 * math.sqrt(max(1.0, ref.shape[0] / ref.shape[1]))
+        assert float((-ps[i].detach().cpu().double() / rate - ref).norm()) <= tol + 4 * 2.0 ** -24 * float(ref.norm())
+
+
+@pytest.mark.gpu
 def test_a_list_that_goes_in_parts():
     """1400 matrices, 7 GiB of intermediate matrices: each as exact as alone, the first, the last and those around the border between the parts among them.
     The Muon step of the same list too.  Tolerance: see the matrices below eps; s is not small here, so 128 d bounds the chain's own roundings of the last step"""
