@@ -548,7 +548,7 @@ int saunet_quantize_rows(int dtype, const void* x, int64_t ldx, int64_t rows, in
 typedef struct saunet_int8_desc {
     const void* a; const float* a_scale; int64_t lda, m;      /* tokens (pixels); strides in bytes, multiples of 16 that cover k rounded up to 64 */
     const void* b; const float* b_scale; int64_t ldb;         /* n weight rows (channels) */
-    int32_t n, k;                                             /* k <= 131071 */
+    int32_t n, k;                                             /* n <= 2^30, k <= 131071 */
     const float* bias;                                        /* or NULL */
     void* y; int64_t ldy;                                     /* m rows of n, row stride in elements */
     int32_t dtype, relu;                                      /* of y: SAUNET_F32 / _BF16 / _F16 */

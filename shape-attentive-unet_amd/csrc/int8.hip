@@ -437,7 +437,7 @@ template <typename T> static int mm8_launch(const I8Args& g, hipStream_t st)
 
 static int int8_check(const saunet_int8_desc* d, const char* who)
 {
-    if (!d || d->m < 0 || d->n < 1 || d->k < 1 || d->k > 131071) return set_error(SAUNET_BAD_SHAPE, "%s: bad sizes", who);
+    if (!d || d->m < 0 || d->n < 1 || d->n > (1 << 30) || d->k < 1 || d->k > 131071) return set_error(SAUNET_BAD_SHAPE, "%s: bad sizes", who);
     const int64_t kp = (d->k + 63) / 64 * 64;
     if (d->ldb < kp || (d->ldb & 15) || d->ldb > (1 << 22) || d->ldy < d->n) return set_error(SAUNET_BAD_SHAPE, "%s: bad strides (%lld, %lld)", who, (long long)d->ldb, (long long)d->ldy);
     if (d->dtype != SAUNET_F32 && d->dtype != SAUNET_BF16 && d->dtype != SAUNET_F16) return set_error(SAUNET_BAD_DTYPE, "%s: dtype %d", who, d->dtype);

@@ -2439,6 +2439,8 @@ def quantize_rows(x, affine=None, relu=False):
 
 def _int8_out(lead, rows, n, dtype, device, out):
     """-> (what the caller gets, its [rows, n] view)"""
+    if n > 1 << 30:
+        raise RuntimeError("int8 products have up to 2^30 channels, not %d" % n)
     if dtype not in _MATRIX_CODES:
         raise RuntimeError("int8 products come as float32, bfloat16 or float16, not %s" % dtype)
     lead = tuple(lead)

@@ -14,6 +14,13 @@ def rows(m, k, seed, dtype=torch.float32):
     return (torch.randn(m, k, generator=g) * torch.exp(torch.randn(1, k, generator=g))).to(dtype)
 
 
+def test_more_channels_than_an_index_holds_are_refused():
+    d = L.Int8Desc(4096, 4096, 64, 1, 4096, 4096, 64, (1 << 30) + 1, 64, None, 4096, (1 << 30) + 1, L.F32, 0)
+    assert L.load().saunet_matmul_int8(C.byref(d), None) == -1 and L.load().saunet_linear_int8(C.byref(d), L.F32, 4096, 64, 4096, 1 << 20, None) == -1
+    with pytest.raises(RuntimeError, match="channels"):
+        HF._int8_out((1,), 1, (1 << 30) + 1, torch.float32, torch.device("cuda:0"), None)
+
+
 @pytest.mark.gpu
 def test_quantize_rows_in_more_than_one_launch():
     """2^23 rows are one launch; each row is a function of itself alone: the same as in a short call"""
