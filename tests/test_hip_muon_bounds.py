@@ -216,6 +216,23 @@ def test_matrices_whose_norm_is_below_eps_keep_their_digits(m, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(40, 90), (150, 120), (300, 500)])
+@pytest.mark.parametrize("steps", [8, 11, 14, 20])
+def test_matrices_below_eps_grow_into_range(m, n, steps):
+    """X grows by 3.4445 a step until it arrives near one, in the middle of a block or between two: the scale t ends at 1 wherever that is"""
+    gen = torch.Generator().manual_seed(m + steps)
+    gs = []
+    for r in (0.3, 1e-2, 1e-4, 1e-5, 1e-6, 1e-8):
+        g = torch.randn(m, n, generator=gen)
+        gs.append((g.double() / g.double().norm() * 1e-7 * r).float())
+    for out, g in zip(HF.newton_schulz([g.cuda() for g in gs], steps=steps), gs):
+        ref = chain(g, torch.float64, steps=steps)
+        # as above, one more product and application for every further step (100 / 5 a step)
+        tol = 4 * float((chain(g, torch.float32, steps=steps).double() - ref).norm()) + 20 * steps * 2.0 ** -24 * float(ref.norm())
+        assert float((out.cpu().double() - ref).norm()) <= tol, (float(g.double().norm()), float((out.cpu().double() - ref).norm()), tol)
+
+
+@pytest.mark.gpu
 def test_muon_update_of_a_gradient_below_eps():
     gen = torch.Generator().manual_seed(8)
     ps, gs = [], []
