@@ -2100,8 +2100,8 @@ class _DenseBlock(torch.autograd.Function):
 
 # int8 conv1 of a dense layer (dense_block_infer): on maps of at most so many pixels, from so many input channels.  The products win everywhere, but the
 # pass that quantises the activations reads and writes them once more.  us, bf16 against int8 (128 output channels):
-#   pixels   256: 512 channels  9.0 / 7.6, 992 15.1 / 10.1      1024: 256 channels 6.1 / 7.5, 992 15.3 / 10.8
-#   pixels  4096: 256 channels  6.2 / 7.8, 512 9.2 / 9.1, 992 15.3 / 12.4      8192: 512 channels 9.5 / 11.2      32768: 1024 channels 28 / 34
+#   pixels   256: 512 channels  9.0 / 6.0, 992 15.1 / 7.6      1024: 256 channels 6.0 / 6.5, 992 15.3 / 8.7
+#   pixels  4096: 256 channels  6.2 / 7.7, 480 9.3 / 9.2, 512 9.4 / 9.0, 992 15.3 / 12.2      8192: 512 channels 9.6 / 11.2      32768: 1024 channels 28 / 34
 INT8_PIXELS_MAX, INT8_CHANNELS_MIN = 4096, 448
 
 
