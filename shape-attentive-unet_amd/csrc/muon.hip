@@ -1150,7 +1150,7 @@ template <class Core> static void ns_launch_prod(const NsPlan& p, const NsTable&
 
 // The matrices with up to NS_MID rows and the others are two chains of launches: the short ones go step by step and keep the digits that composing would cost
 // them.  A Muon step does not need those -- its result is multiplied by the learning rate and added to a rounded parameter -- so there a list with both
-// goes through one chain (SAUNet's matrices, with 64 x 64 tiles for both: 956 us, in two chains 1136).  k: 0 the short ones, 1 the others
+// goes through one chain (SAUNet's matrices 936 us, in two chains 1090).  k: 0 the short ones, 1 the others
 constexpr int NS_MID = 128;
 static saunet_ns_desc ns_part(const saunet_ns_desc* d, bool muon, int k, saunet_ns_item* item)
 {
